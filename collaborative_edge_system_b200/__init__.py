@@ -24,6 +24,17 @@ from .cache import KVCache, LayerKVCache, assign_tokens, ring_decode_attention
 from .comm import CommStats, CommWork, Communicator, NetworkConfig, NetworkEmulator, adopt, dist_ready
 from .launcher import init_distributed, launch_local
 from .mesh import ParallelContext
+from .paged import (
+    OutOfPages,
+    PageAllocator,
+    PagedBatch,
+    PagedKVCache,
+    copy_pages,
+    paged_append,
+    paged_attend_into,
+    paged_attention,
+    paged_attention_with_lse,
+)
 from .partition import HeadShard, SequenceLayout, default_kv_map, offsets_of, partition_heads, split_sizes
 from .sequence_parallel import (
     distributed_kv_attention,
@@ -45,6 +56,10 @@ __all__ = [
     "LayerKVCache",
     "NetworkConfig",
     "NetworkEmulator",
+    "OutOfPages",
+    "PageAllocator",
+    "PagedBatch",
+    "PagedKVCache",
     "ParallelContext",
     "SequenceLayout",
     "accumulation_dtype",
@@ -53,6 +68,7 @@ __all__ = [
     "attend_into",
     "attention",
     "attention_with_lse",
+    "copy_pages",
     "default_kv_map",
     "dist_ready",
     "distributed_kv_attention",
@@ -66,6 +82,10 @@ __all__ = [
     "merge_attention",
     "merge_attention_list",
     "offsets_of",
+    "paged_append",
+    "paged_attend_into",
+    "paged_attention",
+    "paged_attention_with_lse",
     "partition_heads",
     "ring_attention",
     "ring_decode_attention",

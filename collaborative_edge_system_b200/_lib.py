@@ -30,6 +30,8 @@ NOALLOC_SCRATCH_BYTES = 8 << 20
 
 KIND_NONE, KIND_TC, KIND_DECODE, KIND_SIMT = 0, 1, 2, 3
 DEV_TIMEOUT_PRODUCER, DEV_TIMEOUT_MMA, DEV_TIMEOUT_SOFTMAX, DEV_TIMEOUT_DECODE, DEV_TIMEOUT_PEER = range(0x101, 0x106)
+DEV_BAD_PAGE, DEV_BAD_BATCH = 0x106, 0x107
+PAGED_TC, PAGED_DECODE, PAGED_SIMT = 1, 2, 4
 
 _i64x2 = ctypes.c_int64 * 2
 _i64x3 = ctypes.c_int64 * 3
@@ -227,6 +229,81 @@ class KvAppendParams(ctypes.Structure):
     ]
 
 
+class PagedAttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("q_stride", _i64x2),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("o_stride", _i64x2),
+        ("lse_stride", _i64x2),
+        ("table_stride", ctypes.c_int64),
+        ("B", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("min_q_len", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+        ("causal", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("q_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("k_stride", _i64x2),
+        ("v_stride", _i64x2),
+        ("kp_stride", _i64x3),
+        ("vp_stride", _i64x3),
+        ("table_stride", ctypes.c_int64),
+        ("B", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("elem_bytes", ctypes.c_int32),
+    ]
+
+
+class CopyPagesParams(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_stride", _i64x2),
+        ("v_stride", _i64x2),
+        ("page_bytes", ctypes.c_int64),
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("n", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
 EXPORTS = (
     "cea_attn_fwd",
     "cea_attn_workspace_size",
@@ -241,6 +318,11 @@ EXPORTS = (
     "cea_add_rmsnorm",
     "cea_rope",
     "cea_silu_mul",
+    "cea_paged_attn",
+    "cea_paged_attn_workspace_size",
+    "cea_paged_attn_kernels",
+    "cea_paged_append",
+    "cea_copy_pages",
     "cea_device_status",
     "cea_last_error",
     "cea_abi_version",
@@ -288,6 +370,11 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             ("cea_add_rmsnorm", [ctypes.POINTER(RmsNormParams), P], ctypes.c_int),
             ("cea_rope", [ctypes.POINTER(RopeParams), P], ctypes.c_int),
             ("cea_silu_mul", [ctypes.POINTER(SiluMulParams), P], ctypes.c_int),
+            ("cea_paged_attn", [ctypes.POINTER(PagedAttnParams), P], ctypes.c_int),
+            ("cea_paged_attn_workspace_size", [ctypes.POINTER(PagedAttnParams)], ctypes.c_size_t),
+            ("cea_paged_attn_kernels", [ctypes.POINTER(PagedAttnParams)], ctypes.c_int),
+            ("cea_paged_append", [ctypes.POINTER(PagedAppendParams), P], ctypes.c_int),
+            ("cea_copy_pages", [ctypes.POINTER(CopyPagesParams), P], ctypes.c_int),
             ("cea_device_status", [ctypes.POINTER(ctypes.c_int), ctypes.c_int, P], ctypes.c_int),
             ("cea_last_error", [], ctypes.c_char_p),
             ("cea_abi_version", [], ctypes.c_int),
@@ -683,6 +770,39 @@ def _append_chunks(B: int, n: int, toks: int):
         for b0 in range(B):
             for s0 in range(0, n, toks):
                 yield b0, 1, s0, min(toks, n - s0)
+
+
+def _on_device(fn, p, device: torch.device, what: str) -> None:
+    """``fn(p, stream)`` on ``device``'s current stream, with ``device`` current while it launches."""
+    if device.index == torch.cuda.current_device():
+        _check(fn(ctypes.byref(p), _stream_ptr(device)), what)
+        return
+    with torch.cuda.device(device):
+        _check(fn(ctypes.byref(p), _stream_ptr(device)), what)
+
+
+def paged_attn(p: PagedAttnParams, device: torch.device) -> None:
+    """Run cea_paged_attn on ``device``'s current stream with a fresh workspace."""
+    lib = _lib if _lib is not None else load()
+    need = lib.cea_paged_attn_workspace_size(ctypes.byref(p))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    _on_device(lib.cea_paged_attn, p, device, "cea_paged_attn")
+
+
+def paged_attn_kernels(p: PagedAttnParams) -> int:
+    return load().cea_paged_attn_kernels(ctypes.byref(p))
+
+
+def paged_append(p: PagedAppendParams, device: torch.device) -> None:
+    lib = _lib if _lib is not None else load()
+    _on_device(lib.cea_paged_append, p, device, "cea_paged_append")
+
+
+def copy_pages(p: CopyPagesParams, device: torch.device) -> None:
+    lib = _lib if _lib is not None else load()
+    _on_device(lib.cea_copy_pages, p, device, "cea_copy_pages")
 
 
 def device_status(clear: bool = True, device: Optional[torch.device] = None) -> int:

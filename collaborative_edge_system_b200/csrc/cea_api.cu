@@ -20,6 +20,7 @@
 #include "wire.cuh"
 #include "llama_ops.cuh"
 #include "peer_merge.cuh"
+#include "paged.cuh"
 
 using namespace cea;
 
@@ -1026,9 +1027,15 @@ int cea_device_status(int* status_out, int clear, void* stream) {
   if (cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream)) != cudaSuccess) return cuda_check("cea_device_status");
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_cea_status, sizeof(int)) != cudaSuccess) return cuda_check("cea_device_status");
+  // what a paged kernel found in its batch, if no wait expired
+  int paged = 0;
+  if (cudaMemcpyFromSymbol(&paged, g_cea_paged_status, sizeof(int)) != cudaSuccess) return cuda_check("cea_device_status");
+  if (v == 0) v = paged;
   if (clear) {
     const int zero = 0;
-    if (cudaMemcpyToSymbol(g_cea_status, &zero, sizeof(int)) != cudaSuccess) return cuda_check("cea_device_status");
+    if (cudaMemcpyToSymbol(g_cea_status, &zero, sizeof(int)) != cudaSuccess ||
+        cudaMemcpyToSymbol(g_cea_paged_status, &zero, sizeof(int)) != cudaSuccess)
+      return cuda_check("cea_device_status");
   }
   if (status_out) *status_out = v;
   return CEA_OK;
@@ -1275,3 +1282,5 @@ int cea_ipc_close(void* base) {
 }
 
 }  // extern "C"
+
+#include "paged_api.cuh"

@@ -1,0 +1,488 @@
+// Paged KV cache: the batch descriptor, the division of attention work over the CTAs, the write of new tokens into
+// pages and the copy of pages.
+//
+// Token p of sequence b lives in page table[b][p / ps], slot p % ps.  A batch is ragged: the new tokens of sequence
+// b are rows q_off[b] .. q_off[b + 1] of a flat token axis, at positions len_b - n_b + i of its len_b cached tokens
+// (the new ones included).  Lengths and tables live on the device, so one captured graph serves changing batches.
+// Whatever the device reads there is bounded before it is used: offsets to [0, T], lengths to [0, max_pages * ps],
+// and a page outside [0, num_pages) is neither read nor written but reported (CEA_DEV_BAD_PAGE).
+#pragma once
+
+#include "cea_common.cuh"
+
+// First bad page or batch descriptor seen by a paged kernel; unlike g_cea_status it stops no later kernel.
+__device__ int g_cea_paged_status;
+
+namespace cea {
+namespace paged {
+
+__device__ __forceinline__ void report(int code) { atomicCAS(&g_cea_paged_status, 0, code); }
+
+struct Batch {
+  const int32_t* q_off;
+  const int32_t* lens;
+  const int32_t* table;
+  int64_t table_sb;
+  int B, T, max_pages, num_pages, ps;
+};
+
+struct Seq {
+  int row0, n, len;
+};
+
+__device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
+  Seq s;
+  const int64_t cap = min(static_cast<int64_t>(bt.max_pages) * bt.ps, int64_t(0x7fffffff));
+  s.row0 = min(max(bt.q_off[b], 0), bt.T);
+  s.n = min(max(bt.q_off[b + 1], s.row0), bt.T) - s.row0;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(bt.lens[b], 0)), cap));
+  return s;
+}
+
+// ------------------------------------------------------------------ division of the attention work
+// A unit of work is one block of `tb` new tokens of one sequence for one KV head (or, in the generic kernel, for a
+// group of its query heads), over the keys its last token sees.  The units are laid end to end on one axis, each as
+// long as the keys it reads (at least 1), and CTA c of n takes the tiles that start in [W c / n, W (c + 1) / n):
+// every CTA gets the same number of tiles whatever the lengths are, with nothing known on the host.  A unit split
+// over CTAs leaves partial results, at most two a CTA (one that began before it, one that goes on behind it), which
+// combine_kernel joins; so the workspace depends on the grid alone.  A sequence's units form an arithmetic series
+// (block i of a causal chunk reads tb more keys than block i - 1), so its length and the block at a coordinate have
+// closed forms and no work list is written or read.
+struct Division {
+  int B, units_h, tb;   // units_h: units per block of tokens (KV heads x head groups)
+  int group;            // query rows per token and unit
+  int64_t max_rows, min_rows;  // sequences with n * group outside [min_rows, max_rows] belong to another kernel
+  int64_t served_min, served_max;  // range of n * group that this call's kernels serve between them
+  int causal;
+  int min_share;        // smallest share of the axis worth a CTA of its own
+};
+
+struct SeqUnits {
+  int n, len, row0, nb, n0, ctx;
+  int64_t S;  // length on the axis of one head's units
+};
+
+__device__ __forceinline__ int64_t units_before(const SeqUnits& s, int i, int tb, bool causal) {
+  if (!causal) return static_cast<int64_t>(i) * max(1, s.len);
+  if (i <= s.n0) return i;
+  const int64_t m = i - s.n0;
+  return s.n0 + m * s.ctx + static_cast<int64_t>(tb) * (m * (2ll * s.n0 + m + 1) / 2);
+}
+
+// keys that block i reads (its last token's view)
+__device__ __forceinline__ int unit_keys(const SeqUnits& s, int i, int tb, bool causal) {
+  if (!causal) return s.len;
+  const int64_t last = min(static_cast<int64_t>(i + 1) * tb, static_cast<int64_t>(s.n));
+  return static_cast<int>(min(max(s.ctx + last, int64_t(0)), static_cast<int64_t>(s.len)));
+}
+
+__device__ __forceinline__ SeqUnits seq_units(const Batch& bt, const Division& dv, int b) {
+  const Seq q = load_seq(bt, b);
+  SeqUnits s;
+  s.n = q.n;
+  s.len = q.len;
+  s.row0 = q.row0;
+  const int64_t rows = static_cast<int64_t>(q.n) * dv.group;
+  s.nb = q.n > 0 && rows >= dv.min_rows && rows <= dv.max_rows ? (q.n + dv.tb - 1) / dv.tb : 0;
+  s.ctx = q.len - q.n;  // may be negative: the first tokens then see nothing
+  s.n0 = s.ctx < 0 ? min(static_cast<int>((-static_cast<int64_t>(s.ctx)) / dv.tb), max(s.nb - 1, 0)) : 0;
+  s.S = s.nb == 0 ? 0 : units_before(s, s.nb - 1, dv.tb, dv.causal) + max(1, unit_keys(s, s.nb - 1, dv.tb, dv.causal));
+  return s;
+}
+
+struct Share {
+  int64_t W, lo, hi;
+  int n;       // CTAs that take part
+  int b;       // sequence at lo
+  int64_t at;  // where that sequence starts
+};
+
+// Called by every thread of the CTA (a multiple of 32 threads); `scratch` is 34 int64 in shared memory.
+__device__ __forceinline__ Share divide(const Batch& bt, const Division& dv, int64_t* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t sum = 0;
+  const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
+  for (int b = threadIdx.x; b < dv.B; b += blockDim.x) {
+    const SeqUnits s = seq_units(bt, dv, b);
+    sum += s.S * dv.units_h;
+    // a length that the table cannot hold, descending offsets, or a sequence that no launched kernel serves
+    const int64_t rows = static_cast<int64_t>(s.n) * dv.group;
+    if (bt.lens[b] < 0 || bt.lens[b] > cap || bt.q_off[b + 1] < bt.q_off[b] || bt.q_off[b] < 0 ||
+        bt.q_off[b + 1] > bt.T || (s.n > 0 && (rows < dv.served_min || rows > dv.served_max)))
+      report(CEA_DEV_BAD_BATCH);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) scratch[warp] = sum;
+  __syncthreads();
+  Share sh;
+  sh.W = 0;
+  for (int w = 0; w < nw; ++w) sh.W += scratch[w];
+  sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W / dv.min_share)));
+  const int c = blockIdx.x;
+  sh.lo = c < sh.n ? sh.W * c / sh.n : sh.W;
+  sh.hi = c < sh.n ? sh.W * (c + 1) / sh.n : sh.W;
+  if (warp == 0) {
+    int64_t before = 0;
+    int found = dv.B;
+    int64_t at = sh.W;
+    for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += 32) {
+      const int b = b0 + lane;
+      const int64_t w = b < dv.B ? seq_units(bt, dv, b).S * dv.units_h : 0;
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > sh.lo);
+      if (hit != 0u) {
+        const int l = __ffs(hit) - 1;
+        found = b0 + l;
+        at = before + __shfl_sync(0xffffffffu, incl - w, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      scratch[32] = found;
+      scratch[33] = at;
+    }
+  }
+  __syncthreads();
+  sh.b = static_cast<int>(scratch[32]);
+  sh.at = scratch[33];
+  return sh;
+}
+
+// The segments (a unit and a range of its key tiles) of one CTA's share, in order.
+template <int BK>
+struct Segments {
+  const Batch& bt;
+  const Division& dv;
+  const Share& sh;
+  SeqUnits s;
+  int b, hu, blk;       // the unit
+  int64_t base, pos;    // start of sequence b, start of the unit
+  int keys, t0, t1, nt; // keys the unit reads; its tiles [t0, t1) of nt belong to this CTA
+
+  __device__ __forceinline__ Segments(const Batch& bt_, const Division& dv_, const Share& sh_)
+      : bt(bt_), dv(dv_), sh(sh_), b(sh_.b), base(sh_.at) {
+    if (sh.lo >= sh.hi || b >= dv.B) {
+      b = dv.B;
+      return;
+    }
+    s = seq_units(bt, dv, b);
+    int64_t r = sh.lo - base;
+    hu = static_cast<int>(r / s.S);
+    r -= hu * s.S;
+    int lo = 0, hi = s.nb - 1;  // last block that starts at or before r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (units_before(s, mid, dv.tb, dv.causal) <= r) lo = mid; else hi = mid - 1;
+    }
+    blk = lo;
+    pos = base + hu * s.S + units_before(s, blk, dv.tb, dv.causal);
+    settle();
+  }
+
+  __device__ __forceinline__ bool done() const { return b >= dv.B; }
+
+  // the current unit's tiles, or those of the next unit that has some here
+  __device__ __forceinline__ void settle() {
+    while (true) {
+      if (pos >= sh.hi) {
+        b = dv.B;
+        return;
+      }
+      keys = unit_keys(s, blk, dv.tb, dv.causal);
+      nt = max(1, (keys + BK - 1) / BK);
+      t0 = static_cast<int>(max(int64_t(0), (sh.lo - pos + BK - 1) / BK));
+      t1 = static_cast<int>(min(static_cast<int64_t>(nt), (sh.hi - pos + BK - 1) / BK));
+      if (t0 < t1) return;
+      step();
+      if (b >= dv.B) return;
+    }
+  }
+
+  __device__ __forceinline__ void step() {
+    pos += max(1, unit_keys(s, blk, dv.tb, dv.causal));
+    if (++blk < s.nb) return;
+    blk = 0;
+    if (++hu < dv.units_h) return;
+    hu = 0;
+    do {
+      if (++b >= dv.B) return;
+      s = seq_units(bt, dv, b);
+    } while (s.S == 0);
+  }
+
+  __device__ __forceinline__ void next() {
+    step();
+    if (b < dv.B) settle();
+  }
+
+  // last CTA with a tile of this unit
+  __device__ __forceinline__ int last_cta() const {
+    const int64_t x = pos + static_cast<int64_t>(nt - 1) * BK;
+    return static_cast<int>(((x + 1) * sh.n + sh.W - 1) / sh.W - 1);
+  }
+};
+
+// Where a segment's result goes: -1 the output itself, else a slot of the partial results.
+template <int BK>
+__device__ __forceinline__ int segment_slot(const Segments<BK>& g) {
+  if (g.t0 > 0) return 2 * blockIdx.x;
+  if (g.t1 < g.nt) return 2 * blockIdx.x + 1;
+  return -1;
+}
+
+struct Meta {   // one per slot
+  int b, hu, blk;
+  int last;     // odd slots: last CTA that holds a part of the unit; even slots: 0 if the slot holds a part, else -1
+};
+
+// Every CTA writes both of its slots' descriptions, from one thread.
+template <int BK>
+__device__ __forceinline__ void write_meta(const Batch& bt, const Division& dv, const Share& sh, Meta* meta) {
+  Meta first = {0, 0, 0, -1}, behind = {0, 0, 0, -1};
+  for (Segments<BK> g(bt, dv, sh); !g.done(); g.next()) {
+    if (g.t0 > 0) first.last = 0;
+    if (g.t0 == 0 && g.t1 < g.nt) behind = Meta{g.b, g.hu, g.blk, g.last_cta()};
+  }
+  meta[2 * blockIdx.x] = first;
+  meta[2 * blockIdx.x + 1] = behind;
+}
+
+// Joins the parts of units that several CTAs worked on:
+//   lse = ln sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
+// in the partials' precision, parts in the order of the keys (the result does not depend on timing).
+// Block (c, y): the unit that goes on behind CTA c (if one does), rows y * RPB ...; 8 / RPB warps share a row's parts.
+// Bound by latency: a call's partials (at most 2 per SM) sit in L2.
+template <typename A>
+struct CombineArgs {
+  Batch bt;
+  Division dv;
+  const A* part_o;    // [slot][rows][D]
+  const A* part_lse;  // [slot][rows], natural log
+  const Meta* meta;
+  int rows;           // rows of a slot
+  void* out;
+  int64_t o_ss, o_sh;
+  A* lse;
+  int64_t l_sh, l_ss;
+  int D, out_dtype, heads_per_kv, head_groups;
+};
+
+template <typename A>
+__device__ __forceinline__ void store_out(void* out, int64_t at, A v, int dtype) {
+  if (dtype == CEA_BF16) reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(static_cast<float>(v));
+  else if (dtype == CEA_F16) reinterpret_cast<__half*>(out)[at] = __float2half_rn(static_cast<float>(v));
+  else reinterpret_cast<A*>(out)[at] = v;
+}
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float log_of(float x) { return logf(x); }
+__device__ __forceinline__ double log_of(double x) { return log(x); }
+
+constexpr int kCombineThreads = 256;
+constexpr int kMaxD = 256;
+
+template <typename A, int RPB>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineArgs<A> a) {
+  constexpr int WPR = 8 / RPB;  // warps per row
+  __shared__ A acc_s[WPR > 1 ? 8 : 1][WPR > 1 ? kMaxD : 1];
+  __shared__ A stat_s[8][2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (*reinterpret_cast<volatile int*>(&g_cea_status) != 0) return;  // the parts may be missing after a timeout
+  const int c = blockIdx.x;
+  const Meta m = a.meta[2 * c + 1];
+  if (m.last < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.y * RPB + warp / WPR, sub = warp % WPR;
+  const Seq q = load_seq(a.bt, m.b);
+  const int tok = m.blk * a.dv.tb + row / a.dv.group, g = row % a.dv.group;
+  const int head = (m.hu / a.head_groups) * a.heads_per_kv + (m.hu % a.head_groups) * a.dv.group + g;
+  const bool in = row < a.dv.tb * a.dv.group && tok < q.n &&
+                  (m.hu % a.head_groups) * a.dv.group + g < a.heads_per_kv;
+  const int parts = m.last - c + 1;
+  auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
+  auto lse_of = [&](int i) -> A {
+    if (i > 0 && a.meta[slot(i)].last < 0) return -INFINITY;  // a CTA whose share holds no tile start
+    return a.part_lse[static_cast<int64_t>(slot(i)) * a.rows + row];
+  };
+  A top = -INFINITY, sum = 0;
+  if (in) {
+    for (int i = lane; i < parts; i += 32) top = max(top, lse_of(i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // a row no part of which saw a key
+    const A ref = top == -INFINITY ? A(0) : top;
+    A acc[kMaxD / 32];
+#pragma unroll
+    for (int j = 0; j < kMaxD / 32; ++j) acc[j] = 0;
+    for (int i = sub; i < parts; i += WPR) {
+      const A w = exp_of(lse_of(i) - ref);
+      sum += w;
+      if (w == A(0)) continue;
+      const A* src = a.part_o + (static_cast<int64_t>(slot(i)) * a.rows + row) * a.D;
+#pragma unroll
+      for (int j = 0; j < kMaxD / 32; ++j)
+        if (j * 32 + lane < a.D) acc[j] += w * src[j * 32 + lane];
+    }
+    top = ref;
+    if constexpr (WPR == 1) {
+      const A inv = sum == A(0) ? A(0) : A(1) / sum;
+      const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.o_ss + head * a.o_sh;
+#pragma unroll
+      for (int j = 0; j < kMaxD / 32; ++j)
+        if (j * 32 + lane < a.D) store_out<A>(a.out, at + j * 32 + lane, acc[j] * inv, a.out_dtype);
+      if (lane == 0 && a.lse != nullptr)
+        a.lse[head * a.l_sh + static_cast<int64_t>(q.row0 + tok) * a.l_ss] =
+            sum == A(0) ? A(-INFINITY) : top + log_of(sum);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kMaxD / 32; ++j)
+        if (j * 32 + lane < a.D) acc_s[warp][j * 32 + lane] = acc[j];
+      if (lane == 0) stat_s[warp][0] = sum;
+    }
+  }
+  if constexpr (WPR > 1) {
+    __syncthreads();
+    if (!in) return;
+    const int w0 = warp / WPR * WPR;
+    A total = 0;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) total += stat_s[w0 + w][0];
+    const A inv = total == A(0) ? A(0) : A(1) / total;
+    const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.o_ss + head * a.o_sh;
+    for (int d = sub * 32 + lane; d < a.D; d += WPR * 32) {
+      A v = 0;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) v += acc_s[w0 + w][d];
+      store_out<A>(a.out, at + d, v * inv, a.out_dtype);
+    }
+    if (sub == 0 && lane == 0 && a.lse != nullptr)
+      a.lse[head * a.l_sh + static_cast<int64_t>(q.row0 + tok) * a.l_ss] =
+          total == A(0) ? A(-INFINITY) : top + log_of(total);
+  }
+}
+
+// ------------------------------------------------------------------ append
+// New token rows into their pages, bit for bit: one warp per token moves its K and its V rows.  Bound by HBM for
+// prompts and by latency for a decoding step, so the loads of the rows are issued before the walk from the token to
+// its page (sequence by a 32-way search of the offsets, then the table) and stored after it.
+struct AppendArgs {
+  Batch bt;
+  const uint8_t* src[2];   // k, v
+  uint8_t* dst[2];         // pages
+  int64_t src_ss[2], src_sh[2];           // bytes: token, head
+  int64_t dst_sp[2], dst_sh[2], dst_ss[2];  // bytes: page, head, slot
+  int H, units;            // units of U bytes per head row
+};
+
+// sequence of row t: the last b with q_off[b] <= t (offsets ascend; empty sequences are passed over), -1 if none
+__device__ __forceinline__ int find_seq(const Batch& bt, int t, int lane) {
+  int lo = 0, hi = bt.B + 1;  // q_off[lo - 1] <= t (or lo = 0), q_off[hi] > t (or hi = B + 1)
+  while (hi - lo > 0) {
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + lane * step;
+    const bool le = i < hi && bt.q_off[i] <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, le));  // offsets ascend: the first c probes hold
+    if (c == 0) return lo - 1;
+    const int first = lo + (c - 1) * step;  // q_off[first] <= t
+    hi = c < 32 ? min(hi, lo + c * step) : hi;
+    lo = first + 1;
+  }
+  return lo - 1;
+}
+
+constexpr int kAppendThreads = 128;
+constexpr int kAppendUnroll = 4;
+
+template <typename U>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int per = a.H * a.units;  // units of one token's K (or V)
+  const int stride = gridDim.x * (kAppendThreads / 32);
+  for (int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); t < a.bt.T; t += stride) {
+    U val[2][kAppendUnroll];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < kAppendUnroll; ++j) {
+        const int i = j * 32 + lane;
+        if (i < per)
+          val[x][j] = *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + (i / a.units) * a.src_sh[x] +
+                                                  static_cast<int64_t>(i % a.units) * sizeof(U));
+      }
+    const int b = find_seq(a.bt, t, lane);
+    if (b < 0 || b >= a.bt.B) continue;  // before the first or behind the last sequence
+    const Seq s = load_seq(a.bt, b);
+    const int64_t pos = static_cast<int64_t>(a.bt.lens[b]) - s.n + (t - s.row0);
+    const int64_t page_i = pos >= 0 ? pos / a.bt.ps : -1;
+    const int page = page_i >= 0 && page_i < a.bt.max_pages ? a.bt.table[b * a.bt.table_sb + page_i] : -1;
+    if (page < 0 || page >= a.bt.num_pages) {
+      if (lane == 0) report(CEA_DEV_BAD_PAGE);
+      continue;
+    }
+    const int64_t slot = pos - page_i * a.bt.ps;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint8_t* dst = a.dst[x] + page * a.dst_sp[x] + slot * a.dst_ss[x];
+#pragma unroll
+      for (int j = 0; j < kAppendUnroll; ++j) {
+        const int i = j * 32 + lane;
+        if (i < per)
+          *reinterpret_cast<U*>(dst + (i / a.units) * a.dst_sh[x] + static_cast<int64_t>(i % a.units) * sizeof(U)) =
+              val[x][j];
+      }
+      for (int i = kAppendUnroll * 32 + lane; i < per; i += 32)
+        *reinterpret_cast<U*>(dst + (i / a.units) * a.dst_sh[x] + static_cast<int64_t>(i % a.units) * sizeof(U)) =
+            *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + (i / a.units) * a.src_sh[x] +
+                                        static_cast<int64_t>(i % a.units) * sizeof(U));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ page copy
+// Pages src[i] -> dst[i] of every layer's K and V pool.  The pairs travel as kernel arguments (no copy of them to the
+// device, and a captured graph keeps its own).  No page is both read and written (checked on the host), so the order
+// of the copies does not matter.  Bound by HBM: 16-byte units, kCopyUnroll loads in flight per thread.
+constexpr int kCopyPairs = 480;  // a 4 KB argument block
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;
+
+struct CopyArgs {
+  uint8_t* pool[2];
+  int64_t page_stride[2], layer_stride[2];  // bytes
+  int64_t units;                            // units of U bytes per page
+  int n, layers;
+  int2 pair[kCopyPairs];
+};
+
+template <typename U>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+  // blockIdx.x walks the chunks of a page, then the pairs; y the layers, z K or V
+  constexpr int kChunk = kCopyThreads * kCopyUnroll;
+  const int chunks = static_cast<int>((a.units + kChunk - 1) / kChunk);
+  const int i = blockIdx.x / chunks;
+  const int64_t u0 = static_cast<int64_t>(blockIdx.x % chunks) * kChunk + threadIdx.x;
+  const int2 pr = a.pair[i];
+  for (int layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
+    uint8_t* base = (blockIdx.z ? a.pool[1] : a.pool[0]) + layer * a.layer_stride[blockIdx.z];
+    const U* src = reinterpret_cast<const U*>(base + pr.x * a.page_stride[blockIdx.z]);
+    U* dst = reinterpret_cast<U*>(base + pr.y * a.page_stride[blockIdx.z]);
+    U v[kCopyUnroll];
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; ++j)
+      if (u0 + j * kCopyThreads < a.units) v[j] = src[u0 + j * kCopyThreads];
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; ++j)
+      if (u0 + j * kCopyThreads < a.units) dst[u0 + j * kCopyThreads] = v[j];
+  }
+}
+
+}  // namespace paged
+}  // namespace cea

@@ -1,0 +1,419 @@
+// Entry points of the paged KV cache: argument checks, choice of kernels, launches.  Included by cea_api.cu, whose
+// helpers it uses.
+#pragma once
+
+#include <numeric>
+#include <vector>
+
+#include "paged.cuh"
+#include "paged_decode.cuh"
+#include "paged_simt.cuh"
+
+namespace {
+
+namespace pg = cea::paged;
+
+enum PagedKernel { kPagedTc = 1, kPagedDecode = 2, kPagedSimt = 4 };
+
+int paged_check_table(const char* what, int B, int T, int page_size, int num_pages, int max_pages, const void* off,
+                      const void* lens, const void* table) {
+  if (B < 0 || T < 0 || page_size < 1 || num_pages < 0 || max_pages < 0)
+    return fail(CEA_ERR_INVALID, "%s: sizes B=%d T=%d page_size=%d num_pages=%d max_pages=%d", what, B, T, page_size,
+                num_pages, max_pages);
+  if (B > 0 && T > 0 && (off == nullptr || lens == nullptr || (table == nullptr && max_pages > 0)))
+    return fail(CEA_ERR_INVALID, "%s: null offsets, lengths or page table", what);
+  return CEA_OK;
+}
+
+int paged_validate(const cea_paged_attn_params* p) {
+  const char* what = "cea_paged_attn";
+  if (p == nullptr) return fail(CEA_ERR_INVALID, "%s: null params", what);
+  if (int e = paged_check_table(what, p->B, p->T, p->page_size, p->num_pages, p->max_pages, p->q_offsets, p->seq_lens,
+                                p->page_table))
+    return e;
+  if (p->Hq < 0 || p->Hkv < 1 || p->D < 1) return fail(CEA_ERR_INVALID, "%s: Hq=%d Hkv=%d D=%d", what, p->Hq, p->Hkv, p->D);
+  if (p->Hq % p->Hkv != 0)
+    return fail(CEA_ERR_INVALID, "%s: %d query heads cannot share %d KV heads evenly", what, p->Hq, p->Hkv);
+  if (p->D > pg::kMaxD) return fail(CEA_ERR_UNSUPPORTED, "%s: head dim %d above %d", what, p->D, pg::kMaxD);
+  const int in = p->in_dtype, out = p->out_dtype;
+  if (in < CEA_F32 || in > CEA_F64) return fail(CEA_ERR_INVALID, "%s: unknown input dtype %d", what, in);
+  if (!(in == CEA_F64 ? out == CEA_F64 : (out == CEA_F32 || out == in)))
+    return fail(CEA_ERR_UNSUPPORTED, "%s: output dtype %d not available for input dtype %d", what, out, in);
+  if (p->min_q_len < 0 || p->max_q_len < 0 || p->min_q_len > p->max_q_len)
+    return fail(CEA_ERR_INVALID, "%s: new tokens per sequence between %d and %d", what, p->min_q_len, p->max_q_len);
+  if (!(p->scale == p->scale)) return fail(CEA_ERR_INVALID, "%s: scale is not a number", what);
+  if (p->B > 0 && p->T > 0 && p->Hq > 0 && p->max_q_len > 0) {
+    if (p->q == nullptr || p->out == nullptr) return fail(CEA_ERR_INVALID, "%s: null q or out", what);
+    if (p->num_pages > 0 && (p->k_pages == nullptr || p->v_pages == nullptr))
+      return fail(CEA_ERR_INVALID, "%s: null pages", what);
+  }
+  return CEA_OK;
+}
+
+// pages that TMA boxes of at least 8 slots can read: [num_pages, Hkv, page_size, D]
+bool paged_tma_ok(const cea_paged_attn_params* p, const void* ptr, const int64_t* st) {
+  if (!aligned16(ptr) || p->num_pages < 1) return false;
+  for (int i = 0; i < 3; ++i) {
+    if ((i == 0 && p->num_pages == 1) || (i == 1 && p->Hkv == 1)) continue;  // unused
+    if (st[i] <= 0 || st[i] % 8 != 0 || st[i] * 2 >= (int64_t(1) << 40)) return false;
+  }
+  return true;
+}
+
+bool paged_tensor_ok(const cea_paged_attn_params* p) {
+  if (p->in_dtype != CEA_BF16 && p->in_dtype != CEA_F16) return false;
+  if ((p->D != 64 && p->D != 128) || p->page_size % 8 != 0) return false;
+  return paged_tma_ok(p, p->k_pages, p->k_stride) && paged_tma_ok(p, p->v_pages, p->v_stride);
+}
+
+// the decode kernel reads query words of 4 bytes
+bool paged_decode_ok(const cea_paged_attn_params* p) {
+  return paged_tensor_ok(p) && p->Hq / p->Hkv <= pg::dec::ROWS && (reinterpret_cast<uintptr_t>(p->q) & 3u) == 0 &&
+         ((p->q_stride[0] | p->q_stride[1]) & 1) == 0;
+}
+
+int paged_kernels(const cea_paged_attn_params* p) {
+  if (p->B == 0 || p->T == 0 || p->Hq == 0 || p->max_q_len == 0) return 0;
+  const int64_t G = p->Hq / p->Hkv;
+  if (paged_decode_ok(p) && p->max_q_len * G <= pg::dec::ROWS) return kPagedDecode;
+  return kPagedSimt;
+}
+
+struct PagedPlan {
+  int grid, rows;       // CTAs, rows of a slot
+  size_t o, lse, meta, bytes;  // offsets into the workspace
+};
+
+PagedPlan paged_plan(int grid, int rows, int D, size_t elem, size_t at) {
+  PagedPlan pl;
+  pl.grid = grid;
+  pl.rows = rows;
+  pl.o = at;
+  pl.lse = pl.o + align256(elem * 2 * grid * rows * D);
+  pl.meta = pl.lse + align256(elem * 2 * grid * rows);
+  pl.bytes = pl.meta + align256(sizeof(pg::Meta) * 2 * grid);
+  return pl;
+}
+
+// CTAs of the CUDA-core kernel: as many as fit the shared memory of an SM, at most 8
+int paged_simt_grid(const cea_paged_attn_params* p) {
+  const size_t a = p->in_dtype == CEA_F64 ? 8 : 4;
+  const int dmax = p->D <= 32 ? 32 : p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
+  const size_t smem = a * (pg::simt::BQ * (dmax + 1) + 2 * pg::simt::BK * (dmax + 1) + pg::simt::BQ * (pg::simt::BK + 1));
+  return num_sms() * static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (smem + 1536))));
+}
+
+PagedPlan paged_simt_plan(const cea_paged_attn_params* p, size_t at) {
+  return paged_plan(paged_simt_grid(p), pg::simt::BQ, p->D, p->in_dtype == CEA_F64 ? 8 : 4, at);
+}
+
+PagedPlan paged_decode_plan(const cea_paged_attn_params* p, size_t at) {
+  return paged_plan(num_sms(), pg::dec::ROWS, p->D, 4, at);
+}
+
+pg::Batch paged_batch(const cea_paged_attn_params* p) {
+  return pg::Batch{p->q_offsets, p->seq_lens, p->page_table, p->table_stride, p->B, p->T, p->max_pages, p->num_pages,
+                   p->page_size};
+}
+
+// a launch whose start may overlap the end of the kernel before it on the stream (it waits for it on the device)
+template <typename K, typename... Args>
+cudaError_t launch_dependent(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename A, int RPB>
+int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const PagedPlan& pl, int head_groups,
+                   cudaStream_t s) {
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  pg::CombineArgs<A> c;
+  c.bt = paged_batch(p);
+  c.dv = dv;
+  c.part_o = reinterpret_cast<const A*>(ws + pl.o);
+  c.part_lse = reinterpret_cast<const A*>(ws + pl.lse);
+  c.meta = reinterpret_cast<const pg::Meta*>(ws + pl.meta);
+  c.rows = pl.rows;
+  c.out = p->out;
+  c.o_ss = p->o_stride[0];
+  c.o_sh = p->o_stride[1];
+  c.lse = static_cast<A*>(p->lse);
+  c.l_sh = p->lse_stride[0];
+  c.l_ss = p->lse_stride[1];
+  c.D = p->D;
+  c.out_dtype = p->out_dtype;
+  c.heads_per_kv = p->Hq / p->Hkv;
+  c.head_groups = head_groups;
+  const int rows = dv.tb * dv.group;
+  const cudaError_t e = launch_dependent(pg::combine_kernel<A, RPB>, dim3(pl.grid, (rows + RPB - 1) / RPB),
+                                         pg::kCombineThreads, 0, s, c);
+  return e == cudaSuccess ? CEA_OK : fail(CEA_ERR_CUDA, "combine_kernel: %s", cudaGetErrorString(e));
+}
+
+template <typename T, typename A, int DMAX>
+int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStream_t s) {
+  const int G = p->Hq / p->Hkv;
+  const int group = std::min(G, pg::simt::BQ), groups = (G + group - 1) / group;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  pg::simt::Params<A> a;
+  a.bt = paged_batch(p);
+  a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, 0, INT64_MAX, p->causal ? 1 : 0,
+                      pg::simt::BK};
+  a.q = p->q;
+  a.k = p->k_pages;
+  a.v = p->v_pages;
+  a.q_ss = p->q_stride[0];
+  a.q_sh = p->q_stride[1];
+  a.k_sp = p->k_stride[0];
+  a.k_sh = p->k_stride[1];
+  a.k_ss = p->k_stride[2];
+  a.v_sp = p->v_stride[0];
+  a.v_sh = p->v_stride[1];
+  a.v_ss = p->v_stride[2];
+  a.out = p->out;
+  a.o_ss = p->o_stride[0];
+  a.o_sh = p->o_stride[1];
+  a.lse = static_cast<A*>(p->lse);
+  a.l_sh = p->lse_stride[0];
+  a.l_ss = p->lse_stride[1];
+  a.part_o = reinterpret_cast<A*>(ws + pl.o);
+  a.part_lse = reinterpret_cast<A*>(ws + pl.lse);
+  a.meta = reinterpret_cast<pg::Meta*>(ws + pl.meta);
+  a.G = G;
+  a.head_groups = groups;
+  a.D = p->D;
+  a.out_dtype = p->out_dtype;
+  a.scale = p->scale;
+  auto k = pg::simt::attn_kernel<T, A, DMAX>;
+  constexpr size_t bytes = pg::simt::smem_bytes<A, DMAX>();
+  allow_smem(k, static_cast<int>(bytes));
+  k<<<pl.grid, pg::simt::NT, bytes, s>>>(a);
+  if (int e = cuda_check("paged attn_kernel")) return e;
+  return launch_combine<A, 8>(p, a.dv, pl, groups, s);
+}
+
+template <typename T, typename A>
+int launch_paged_simt_d(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStream_t s) {
+  if (p->D <= 32) return launch_paged_simt<T, A, 32>(p, pl, s);
+  if (p->D <= 64) return launch_paged_simt<T, A, 64>(p, pl, s);
+  if (p->D <= 128) return launch_paged_simt<T, A, 128>(p, pl, s);
+  return launch_paged_simt<T, A, 256>(p, pl, s);
+}
+
+// pages [num_pages, Hkv, page_size, D] as a 4-D tensor map (D, slot, head, page) with (64, rows, 1, 1) boxes
+bool paged_map(CUtensorMap* map, const cea_paged_attn_params* p, const void* ptr, const int64_t* st, int rows) {
+  return make_map(map, p->in_dtype, ptr, p->D, p->page_size, p->Hkv, p->num_pages, st[2], st[1], st[0], rows);
+}
+
+int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, int kernels, cudaStream_t s) {
+  const int G = p->Hq / p->Hkv;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  pg::dec::Params a;
+  a.bt = paged_batch(p);
+  a.dv = pg::Division{p->B, p->Hkv, pg::dec::ROWS / G, G, pg::dec::ROWS, 0, 0,
+                      (kernels & kPagedTc) ? INT64_MAX : int64_t(pg::dec::ROWS), p->causal ? 1 : 0, pg::dec::BK};
+  a.q = p->q;
+  a.q_ss = p->q_stride[0];
+  a.q_sh = p->q_stride[1];
+  a.out = p->out;
+  a.o_ss = p->o_stride[0];
+  a.o_sh = p->o_stride[1];
+  a.lse = static_cast<float*>(p->lse);
+  a.l_sh = p->lse_stride[0];
+  a.l_ss = p->lse_stride[1];
+  a.part_o = reinterpret_cast<float*>(ws + pl.o);
+  a.part_lse = reinterpret_cast<float*>(ws + pl.lse);
+  a.meta = reinterpret_cast<pg::Meta*>(ws + pl.meta);
+  a.box = std::gcd(p->page_size, pg::dec::BK);
+  a.out_dtype = p->out_dtype;
+  a.scale_log2 = static_cast<float>(p->scale * 1.4426950408889634);
+  CUtensorMap mk, mv;
+  if (!paged_map(&mk, p, p->k_pages, p->k_stride, a.box) || !paged_map(&mv, p, p->v_pages, p->v_stride, a.box))
+    return fail(CEA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pages");
+#define CEA_PDEC(DD, BF)                                                                  \
+  do {                                                                                    \
+    auto k = pg::dec::decode_kernel<DD, BF>;                                              \
+    allow_smem(k, pg::dec::Layout<DD>::SMEM_ALLOC);                                       \
+    k<<<pl.grid, pg::dec::NTHREADS, pg::dec::Layout<DD>::SMEM_ALLOC, s>>>(mk, mv, a);     \
+  } while (0)
+  const bool bf = p->in_dtype == CEA_BF16;
+  if (p->D == 128) {
+    if (bf) CEA_PDEC(128, true); else CEA_PDEC(128, false);
+  } else {
+    if (bf) CEA_PDEC(64, true); else CEA_PDEC(64, false);
+  }
+#undef CEA_PDEC
+  if (int e = cuda_check("paged decode_kernel")) return e;
+  return launch_combine<float, 1>(p, a.dv, pl, 1, s);
+}
+
+size_t paged_workspace(const cea_paged_attn_params* p, int kernels) {
+  size_t n = 0;
+  if (kernels & kPagedDecode) n = paged_decode_plan(p, n).bytes;
+  if (kernels & kPagedSimt) n = paged_simt_plan(p, n).bytes;
+  return n;
+}
+
+template <typename U>
+void launch_append(const pg::AppendArgs& a, cudaStream_t s) {
+  constexpr int per = pg::kAppendThreads / 32;
+  const int grid = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(a.bt.T) + per - 1) / per, 148 * 16));
+  pg::append_kernel<U><<<grid, pg::kAppendThreads, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int cea_paged_attn_kernels(const cea_paged_attn_params* p) {
+  if (paged_validate(p) != CEA_OK) return -1;
+  return paged_kernels(p);
+}
+
+size_t cea_paged_attn_workspace_size(const cea_paged_attn_params* p) {
+  if (paged_validate(p) != CEA_OK) return 0;
+  return paged_workspace(p, paged_kernels(p));
+}
+
+int cea_paged_attn(const cea_paged_attn_params* p, void* stream) {
+  if (int e = paged_validate(p)) return e;
+  const int kernels = paged_kernels(p);
+  if (kernels == 0) return CEA_OK;
+  const size_t need = paged_workspace(p, kernels);
+  if (p->workspace == nullptr || p->workspace_bytes < need || !aligned16(p->workspace))
+    return fail(CEA_ERR_WORKSPACE, "paged attention needs %zu 16-byte aligned workspace bytes, got %zu", need,
+                p->workspace_bytes);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  size_t at = 0;
+  if (kernels & kPagedDecode) {
+    const PagedPlan pl = paged_decode_plan(p, at);
+    if (int e = launch_paged_decode(p, pl, kernels, s)) return e;
+    at = pl.bytes;
+  }
+  if (kernels & kPagedSimt) {
+    const PagedPlan pl = paged_simt_plan(p, at);
+    switch (p->in_dtype) {
+      case CEA_F64: return launch_paged_simt_d<double, double>(p, pl, s);
+      case CEA_F32: return launch_paged_simt_d<float, float>(p, pl, s);
+      case CEA_BF16: return launch_paged_simt_d<__nv_bfloat16, float>(p, pl, s);
+      default: return launch_paged_simt_d<__half, float>(p, pl, s);
+    }
+  }
+  return CEA_OK;
+}
+
+int cea_paged_append(const cea_paged_append_params* p, void* stream) {
+  const char* what = "cea_paged_append";
+  if (p == nullptr) return fail(CEA_ERR_INVALID, "%s: null params", what);
+  if (int e = paged_check_table(what, p->B, p->T, p->page_size, p->num_pages, p->max_pages, p->q_offsets, p->seq_lens,
+                                p->page_table))
+    return e;
+  if (p->H < 1 || p->D < 1) return fail(CEA_ERR_INVALID, "%s: heads and head dim must be >= 1", what);
+  const int eb = p->elem_bytes;
+  if (eb != 1 && eb != 2 && eb != 4 && eb != 8) return fail(CEA_ERR_INVALID, "%s: element size %d", what, eb);
+  if (p->B == 0 || p->T == 0) return CEA_OK;
+  if (!p->k || !p->v || !p->k_pages || !p->v_pages) return fail(CEA_ERR_INVALID, "%s: null k, v or pages", what);
+  pg::AppendArgs a{};
+  a.bt = pg::Batch{p->q_offsets, p->seq_lens, p->page_table, p->table_stride, p->B, p->T, p->max_pages, p->num_pages,
+                   p->page_size};
+  const void* src[2] = {p->k, p->v};
+  void* dst[2] = {p->k_pages, p->v_pages};
+  const int64_t* ss[2] = {p->k_stride, p->v_stride};
+  const int64_t* ds[2] = {p->kp_stride, p->vp_stride};
+  // the widest unit that divides a row and every row start
+  uint64_t bits = static_cast<uint64_t>(p->D) * eb;
+  for (int i = 0; i < 2; ++i) {
+    a.src[i] = static_cast<const uint8_t*>(src[i]);
+    a.dst[i] = static_cast<uint8_t*>(dst[i]);
+    a.src_ss[i] = ss[i][0] * eb;
+    a.src_sh[i] = ss[i][1] * eb;
+    a.dst_sp[i] = ds[i][0] * eb;
+    a.dst_sh[i] = ds[i][1] * eb;
+    a.dst_ss[i] = ds[i][2] * eb;
+    for (int64_t x : {reinterpret_cast<int64_t>(src[i]), reinterpret_cast<int64_t>(dst[i]), a.src_ss[i], a.src_sh[i],
+                      a.dst_sp[i], a.dst_sh[i], a.dst_ss[i]})
+      bits |= static_cast<uint64_t>(x);
+  }
+  const int unit = static_cast<int>(std::min<uint64_t>(16, bits & (~bits + 1)));
+  a.H = p->H;
+  const int64_t units = static_cast<int64_t>(p->D) * eb / unit;
+  if (units * p->H > 0x7fffffff) return fail(CEA_ERR_UNSUPPORTED, "%s: %d heads of %d elements", what, p->H, p->D);
+  a.units = static_cast<int>(units);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  switch (unit) {
+    case 16: launch_append<uint4>(a, s); break;
+    case 8: launch_append<uint2>(a, s); break;
+    case 4: launch_append<uint32_t>(a, s); break;
+    case 2: launch_append<uint16_t>(a, s); break;
+    default: launch_append<uint8_t>(a, s); break;
+  }
+  return cuda_check(what);
+}
+
+int cea_copy_pages(const cea_copy_pages_params* p, void* stream) {
+  const char* what = "cea_copy_pages";
+  if (p == nullptr) return fail(CEA_ERR_INVALID, "%s: null params", what);
+  if (p->n < 0 || p->layers < 0 || p->num_pages < 0 || p->page_bytes < 0)
+    return fail(CEA_ERR_INVALID, "%s: negative size", what);
+  if (p->n == 0) return CEA_OK;
+  if (!p->src || !p->dst) return fail(CEA_ERR_INVALID, "%s: null indices", what);
+  // every destination once, and none that is also a source: the copies then commute
+  try {
+    std::vector<uint8_t> mark(p->num_pages, 0);
+    for (int i = 0; i < p->n; ++i) {
+      if (p->src[i] < 0 || p->src[i] >= p->num_pages || p->dst[i] < 0 || p->dst[i] >= p->num_pages)
+        return fail(CEA_ERR_INVALID, "%s: pair %d (%d -> %d) outside a pool of %d pages", what, i, p->src[i], p->dst[i],
+                    p->num_pages);
+      if (mark[p->dst[i]]) return fail(CEA_ERR_INVALID, "%s: page %d is written twice", what, p->dst[i]);
+      mark[p->dst[i]] = 1;
+    }
+    for (int i = 0; i < p->n; ++i)
+      if (mark[p->src[i]]) return fail(CEA_ERR_INVALID, "%s: page %d is both read and written", what, p->src[i]);
+  } catch (const std::exception& e) {
+    return fail(CEA_ERR_INVALID, "%s: %s", what, e.what());
+  }
+  if (p->layers == 0 || p->page_bytes == 0) return CEA_OK;
+  if (!p->k_pages || !p->v_pages) return fail(CEA_ERR_INVALID, "%s: null pages", what);
+  pg::CopyArgs a{};
+  a.pool[0] = static_cast<uint8_t*>(p->k_pages);
+  a.pool[1] = static_cast<uint8_t*>(p->v_pages);
+  uint64_t bits = static_cast<uint64_t>(p->page_bytes) | reinterpret_cast<uintptr_t>(p->k_pages) |
+                  reinterpret_cast<uintptr_t>(p->v_pages);
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* st = i ? p->v_stride : p->k_stride;
+    a.layer_stride[i] = st[0];
+    a.page_stride[i] = st[1];
+    bits |= static_cast<uint64_t>(st[1]) | (p->layers > 1 ? static_cast<uint64_t>(st[0]) : 0);
+  }
+  const int unit = static_cast<int>(std::min<uint64_t>(16, bits & (~bits + 1)));
+  a.units = p->page_bytes / unit;
+  a.layers = p->layers;
+  const int64_t chunks = (a.units + pg::kCopyThreads * pg::kCopyUnroll - 1) / (pg::kCopyThreads * pg::kCopyUnroll);
+  if (chunks * pg::kCopyPairs > 0x7fffffff) return fail(CEA_ERR_UNSUPPORTED, "%s: pages of %lld bytes", what, (long long)p->page_bytes);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  for (int i0 = 0; i0 < p->n; i0 += pg::kCopyPairs) {
+    a.n = std::min(pg::kCopyPairs, p->n - i0);
+    for (int i = 0; i < a.n; ++i) a.pair[i] = make_int2(p->src[i0 + i], p->dst[i0 + i]);
+    const dim3 grid(static_cast<unsigned>(chunks * a.n), std::min(p->layers, 65535), 2);
+    switch (unit) {
+      case 16: pg::copy_pages_kernel<uint4><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+      case 8: pg::copy_pages_kernel<uint2><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+      case 4: pg::copy_pages_kernel<uint32_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+      case 2: pg::copy_pages_kernel<uint16_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+      default: pg::copy_pages_kernel<uint8_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+    }
+    if (int e = cuda_check(what)) return e;
+  }
+  return CEA_OK;
+}
+
+}  // extern "C"

@@ -45,7 +45,9 @@ enum cea_device_error {
   CEA_DEV_TIMEOUT_MMA = 0x102,
   CEA_DEV_TIMEOUT_SOFTMAX = 0x103,
   CEA_DEV_TIMEOUT_DECODE = 0x104,
-  CEA_DEV_TIMEOUT_PEER = 0x105
+  CEA_DEV_TIMEOUT_PEER = 0x105,
+  CEA_DEV_BAD_PAGE = 0x106, /* a page table entry outside the pool, or a token behind the table */
+  CEA_DEV_BAD_BATCH = 0x107 /* offsets or lengths of a paged batch that do not fit the call */
 };
 
 typedef enum cea_dtype { CEA_F32 = 0, CEA_F16 = 1, CEA_BF16 = 2, CEA_F64 = 3 } cea_dtype;
@@ -326,6 +328,106 @@ typedef struct cea_kv_append_params {
 } cea_kv_append_params;
 
 int cea_kv_append(const cea_kv_append_params* p, void* stream);
+
+/*
+ * Paged KV cache.  Keys and values live in pages of page_size tokens:
+ * k_pages / v_pages [num_pages, Hkv, page_size, D] (element strides page,
+ * head, slot; D contiguous), token p of sequence b in page
+ * page_table[b, p / page_size], slot p % page_size.  A batch is ragged: its new
+ * tokens are the rows q_offsets[b] .. q_offsets[b + 1] of a flat token axis of
+ * T rows, and seq_lens[b] counts the sequence's cached tokens, the new ones
+ * included, so new token i of n_b is at position seq_lens[b] - n_b + i.
+ * q_offsets [B + 1], seq_lens [B] and page_table [B, max_pages] are int32 on the
+ * device: one captured graph serves batches that change in place.  Rows that
+ * belong to no sequence are left as they were.  What does not fit is bounded on the
+ * device and reported through cea_device_status (it stops no later kernel): a
+ * table entry outside [0, num_pages) reads as zeros and is not written
+ * (CEA_DEV_BAD_PAGE); descending offsets, a length that the table cannot hold or
+ * a sequence outside [min_q_len, max_q_len] whose kernel was not launched is
+ * CEA_DEV_BAD_BATCH.
+ *
+ * cea_paged_attn: attention of the new tokens (n_b from 0 on, single tokens
+ * included) over the cached ones; token i sees the keys at positions up to
+ * its own (causal) or all seq_lens[b].  q / out [T, Hq, D] (strides token, head),
+ * lse [Hq, T] natural log (strides head, token) or NULL.  A token that sees no key
+ * (position below 0, or an empty sequence) gives out = 0 and lse = -inf.  Slots
+ * behind a sequence's length are never used, whatever they hold.  out_dtype is
+ * the input dtype or F32 (F64 for F64); lse is F32 (F64 for F64).
+ * min_q_len / max_q_len bound the n_b > 0 of the batch and choose the kernels
+ * (0 and T are always right): sequences with n_b * Hq / Hkv <= 16 go through the
+ * split decode kernel, others through the tcgen05 kernel, each where it applies
+ * (bf16 / f16, D in {64, 128}, page_size a multiple of 8, 16-byte aligned rows);
+ * everything else through the CUDA-core kernel.  cea_paged_attn_kernels returns
+ * the kernels of a call as a mask: 1 tcgen05, 2 split decode, 4 CUDA cores.
+ */
+typedef struct cea_paged_attn_params {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  void* out;
+  void* lse;
+  const int32_t* q_offsets;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  int64_t q_stride[2];   /* token, head */
+  int64_t k_stride[3];   /* page, head, slot */
+  int64_t v_stride[3];
+  int64_t o_stride[2];
+  int64_t lse_stride[2]; /* head, token */
+  int64_t table_stride;  /* between sequences */
+  int32_t B, T, Hq, Hkv, D, page_size, num_pages, max_pages, min_q_len, max_q_len;
+  double scale;
+  int32_t causal, in_dtype, out_dtype;
+  void* workspace;
+  size_t workspace_bytes;
+} cea_paged_attn_params;
+
+int cea_paged_attn(const cea_paged_attn_params* p, void* stream);
+/* Bytes of workspace cea_paged_attn needs for these parameters on the current device (0 if none). */
+size_t cea_paged_attn_workspace_size(const cea_paged_attn_params* p);
+/* Mask of the kernels cea_paged_attn would run (0: nothing to do), -1 if the parameters are invalid. */
+int cea_paged_attn_kernels(const cea_paged_attn_params* p);
+
+/*
+ * cea_paged_append: the rows of k / v [T, H, D] (element strides token, head; D
+ * contiguous) into their pages, bit for bit (any dtype of 1, 2, 4 or 8 bytes), at
+ * the positions described above.
+ */
+typedef struct cea_paged_append_params {
+  const void* k;
+  const void* v;
+  void* k_pages;
+  void* v_pages;
+  const int32_t* q_offsets;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  int64_t k_stride[2];  /* token, head */
+  int64_t v_stride[2];
+  int64_t kp_stride[3]; /* page, head, slot */
+  int64_t vp_stride[3];
+  int64_t table_stride;
+  int32_t B, T, H, D, page_size, num_pages, max_pages, elem_bytes;
+} cea_paged_append_params;
+
+int cea_paged_append(const cea_paged_append_params* p, void* stream);
+
+/*
+ * cea_copy_pages: page src[i] to page dst[i] of both pools, in all layers.  A page is
+ * page_bytes contiguous bytes; strides are in bytes.  src and dst are host arrays of
+ * n indices: no destination may repeat or be a source (CEA_ERR_INVALID).
+ */
+typedef struct cea_copy_pages_params {
+  void* k_pages;
+  void* v_pages;
+  int64_t k_stride[2]; /* layer, page */
+  int64_t v_stride[2];
+  int64_t page_bytes;
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t n, layers, num_pages;
+} cea_copy_pages_params;
+
+int cea_copy_pages(const cea_copy_pages_params* p, void* stream);
 
 /*
  * NCCL transfers of the sequence-parallel path, for callers that hold no
