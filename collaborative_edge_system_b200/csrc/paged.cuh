@@ -242,17 +242,20 @@ struct Meta {   // one per slot
   int last;     // odd slots: last CTA that holds a part of the unit; even slots: 0 if the slot holds a part, else -1
 };
 
-// Every CTA writes both of its slots' descriptions, from one thread.
-template <int BK>
-__device__ __forceinline__ void write_meta(const Batch& bt, const Division& dv, const Share& sh, Meta* meta) {
+// Descriptions of a CTA's two slots, gathered by a warp that walks the segments anyway.
+struct MetaPair {
   Meta first = {0, 0, 0, -1}, behind = {0, 0, 0, -1};
-  for (Segments<BK> g(bt, dv, sh); !g.done(); g.next()) {
+
+  template <int BK>
+  __device__ __forceinline__ void note(const Segments<BK>& g) {
     if (g.t0 > 0) first.last = 0;
-    if (g.t0 == 0 && g.t1 < g.nt) behind = Meta{g.b, g.hu, g.blk, g.last_cta()};
+    else if (g.t1 < g.nt) behind = Meta{g.b, g.hu, g.blk, g.last_cta()};
   }
-  meta[2 * blockIdx.x] = first;
-  meta[2 * blockIdx.x + 1] = behind;
-}
+  __device__ __forceinline__ void store(Meta* meta) const {
+    meta[2 * blockIdx.x] = first;
+    meta[2 * blockIdx.x + 1] = behind;
+  }
+};
 
 // Joins the parts of units that several CTAs worked on:
 //   lse = ln sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i

@@ -8,6 +8,7 @@
 #include "paged.cuh"
 #include "paged_decode.cuh"
 #include "paged_simt.cuh"
+#include "paged_tc.cuh"
 
 namespace {
 
@@ -72,10 +73,29 @@ bool paged_decode_ok(const cea_paged_attn_params* p) {
          ((p->q_stride[0] | p->q_stride[1]) & 1) == 0;
 }
 
+// the chunk kernel reads Q by TMA and stores 16-byte vectors of a row
+bool paged_tc_ok(const cea_paged_attn_params* p) {
+  if (!paged_tensor_ok(p) || p->Hq / p->Hkv > pg::tc::BM) return false;
+  if (!aligned16(p->q) || !aligned16(p->out)) return false;
+  const int vec = p->out_dtype == CEA_F32 ? 4 : 8;
+  const int size[2] = {p->T, p->Hq};
+  for (int i = 0; i < 2; ++i) {
+    if (size[i] == 1) continue;
+    if (p->q_stride[i] <= 0 || p->q_stride[i] % 8 != 0 || p->q_stride[i] * 2 >= (int64_t(1) << 40)) return false;
+    if (p->o_stride[i] % vec != 0) return false;
+  }
+  return true;
+}
+
 int paged_kernels(const cea_paged_attn_params* p) {
   if (p->B == 0 || p->T == 0 || p->Hq == 0 || p->max_q_len == 0) return 0;
   const int64_t G = p->Hq / p->Hkv;
-  if (paged_decode_ok(p) && p->max_q_len * G <= pg::dec::ROWS) return kPagedDecode;
+  // rows n * G of a sequence: up to ROWS through the decode kernel, more through the chunk kernel (measured at 32/8
+  // heads of 128: see paged_tc.cuh), each launched only if the bounds allow such a sequence
+  const bool few = std::max<int64_t>(p->min_q_len, 1) * G <= pg::dec::ROWS;
+  const bool many = p->max_q_len * G > pg::dec::ROWS;
+  if ((!few || paged_decode_ok(p)) && (!many || paged_tc_ok(p)))
+    return (few ? kPagedDecode : 0) | (many ? kPagedTc : 0);
   return kPagedSimt;
 }
 
@@ -109,6 +129,10 @@ PagedPlan paged_simt_plan(const cea_paged_attn_params* p, size_t at) {
 
 PagedPlan paged_decode_plan(const cea_paged_attn_params* p, size_t at) {
   return paged_plan(num_sms(), pg::dec::ROWS, p->D, 4, at);
+}
+
+PagedPlan paged_tc_plan(const cea_paged_attn_params* p, size_t at) {
+  return paged_plan(num_sms(), 2 * pg::tc::BM, p->D, 4, at);
 }
 
 pg::Batch paged_batch(const cea_paged_attn_params* p) {
@@ -256,9 +280,66 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, int
   return launch_combine<float, 1>(p, a.dv, pl, 1, s);
 }
 
+// q [T, Hq, D] as a tensor map (D, head, token) with boxes of `tokens` x G heads x 64 columns
+bool paged_q_map(CUtensorMap* map, const cea_paged_attn_params* p, int G, int tokens) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return false;
+  // the stride of a dimension of size 1 is never used: give it a legal value
+  const int64_t sh = p->Hq == 1 ? p->D : p->q_stride[1], ss = p->T == 1 ? p->D * int64_t(p->Hq) : p->q_stride[0];
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->D), static_cast<cuuint64_t>(p->Hq),
+                              static_cast<cuuint64_t>(p->T), 1};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(ss) * 2,
+                                 static_cast<cuuint64_t>(ss) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(tokens), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t =
+      p->in_dtype == CEA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, t, 4, const_cast<void*>(p->q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, int kernels, cudaStream_t s) {
+  const int G = p->Hq / p->Hkv;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  pg::tc::Params a;
+  a.bt = paged_batch(p);
+  a.half = pg::tc::BM / G;
+  a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, pg::dec::ROWS + 1,
+                      (kernels & kPagedDecode) ? 0 : int64_t(pg::dec::ROWS + 1), INT64_MAX, p->causal ? 1 : 0,
+                      2 * pg::tc::BK};
+  a.box = std::gcd(p->page_size, pg::tc::BK);
+  a.out = p->out;
+  a.o_ss = p->o_stride[0];
+  a.o_sh = p->o_stride[1];
+  a.lse = static_cast<float*>(p->lse);
+  a.l_sh = p->lse_stride[0];
+  a.l_ss = p->lse_stride[1];
+  a.part_o = reinterpret_cast<float*>(ws + pl.o);
+  a.part_lse = reinterpret_cast<float*>(ws + pl.lse);
+  a.meta = reinterpret_cast<pg::Meta*>(ws + pl.meta);
+  a.out_dtype = p->out_dtype;
+  a.scale_log2 = static_cast<float>(p->scale * 1.4426950408889634);
+  CUtensorMap mq, mk, mv;
+  if (!paged_q_map(&mq, p, G, a.half) || !paged_map(&mk, p, p->k_pages, p->k_stride, a.box) ||
+      !paged_map(&mv, p, p->v_pages, p->v_stride, a.box))
+    return fail(CEA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the queries or the pages");
+#define CEA_PTC(DD, BF)                                                                                    do {                                                                                                       auto k = pg::tc::chunk_kernel<DD, BF>;                                                                   if (int e = check_launch_regs(reinterpret_cast<const void*>(k), pg::tc::kLaunchRegs)) return e;          allow_smem(k, pg::tc::Layout<DD>::SMEM_ALLOC);                                                           k<<<pl.grid, pg::tc::NUM_THREADS, pg::tc::Layout<DD>::SMEM_ALLOC, s>>>(mq, mk, mv, a);                 } while (0)
+  const bool bf = p->in_dtype == CEA_BF16;
+  if (p->D == 128) {
+    if (bf) CEA_PTC(128, true); else CEA_PTC(128, false);
+  } else {
+    if (bf) CEA_PTC(64, true); else CEA_PTC(64, false);
+  }
+#undef CEA_PTC
+  if (int e = cuda_check("paged chunk_kernel")) return e;
+  return launch_combine<float, 8>(p, a.dv, pl, 1, s);
+}
+
 size_t paged_workspace(const cea_paged_attn_params* p, int kernels) {
   size_t n = 0;
   if (kernels & kPagedDecode) n = paged_decode_plan(p, n).bytes;
+  if (kernels & kPagedTc) n = paged_tc_plan(p, n).bytes;
   if (kernels & kPagedSimt) n = paged_simt_plan(p, n).bytes;
   return n;
 }
@@ -297,6 +378,11 @@ int cea_paged_attn(const cea_paged_attn_params* p, void* stream) {
   if (kernels & kPagedDecode) {
     const PagedPlan pl = paged_decode_plan(p, at);
     if (int e = launch_paged_decode(p, pl, kernels, s)) return e;
+    at = pl.bytes;
+  }
+  if (kernels & kPagedTc) {
+    const PagedPlan pl = paged_tc_plan(p, at);
+    if (int e = launch_paged_tc(p, pl, kernels, s)) return e;
     at = pl.bytes;
   }
   if (kernels & kPagedSimt) {

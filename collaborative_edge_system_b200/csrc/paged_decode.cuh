@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(NTHREADS)
     if (lane == 0) {
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
-      write_meta<BK>(p.bt, p.dv, sh, p.meta);
     }
     __syncwarp();
     const int nbox = BK / p.box;  // boxes of 64 columns along a tile's keys
@@ -111,7 +110,9 @@ __global__ void __launch_bounds__(NTHREADS)
     const uint32_t dst0 = is_v * L::TILE + half * L::BOX + box * p.box * 128;
     int it = 0;
     bool ok = !dead;
+    MetaPair meta;
     for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+      meta.note(g);
       const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
       for (int t = g.t0; t < g.t1; ++t, ++it) {
         const int st = it % L::NSTAGE;
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(NTHREADS)
         if (load) tma_load_4d(sbase + st * L::STAGE + dst0, map, full_bar(st), half * 64, slot, g.hu, page);
       }
     }
+    if (lane == 0) meta.store(p.meta);
     return;
   }
 

@@ -62,7 +62,9 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
   const Share sh = divide(p.bt, p.dv, scratch);
   asm volatile("griddepcontrol.launch_dependents;");
 
+  MetaPair meta;
   for (Segments<BK> g(p.bt, p.dv, sh); !g.done(); g.next()) {
+    meta.note(g);
     const int kvh = g.hu / p.head_groups, g0 = (g.hu % p.head_groups) * p.dv.group;
     const int tok = g.blk * p.dv.tb + r / p.dv.group, gg = g0 + r % p.dv.group;
     const bool in = r < p.dv.tb * p.dv.group && tok < g.s.n && gg < p.G;
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
       if (sub == 0) p.part_lse[at] = lse;
     }
   }
-  if (threadIdx.x == 0) write_meta<BK>(p.bt, p.dv, sh, p.meta);
+  if (threadIdx.x == 0) meta.store(p.meta);
 }
 
 }  // namespace simt

@@ -1,0 +1,441 @@
+// Attention over a paged cache for chunks of new tokens (n_b * G > 16 query rows per KV head): tcgen05 products.
+//
+// Tensor-bound on long chunks.  One persistent CTA per SM takes an equal share of all key tiles of the batch
+// (paged.cuh).  A unit is 2 x (128 / G) new tokens of one KV head: the G query heads of a group are packed with the
+// tokens into the 128 rows of each of two MMA tiles ("halves"), so short chunks fill the rows and every K/V tile
+// is read once for all heads that share it.  Q rows (token, head) come from one TMA box of (64, G, 128 / G).
+//   warps 0-3 / 4-7   softmax and epilogue of half 0 / 1: one thread per query row (= TMEM lane)
+//   warp 8 / 10       the K / V ring: 128-key tiles, one TMA box per page (or part of one), one box per lane
+//   warp 9 / 11       MMA issuer of half 0 / 1 (one thread), which also loads its half's Q
+// The issuers take turns, each pushing PV_h(u - 1), S_h(u) for the running tile number u, as in the dense prefill
+// kernel (attn_tc2.cuh): one half's products run during the other's softmax.  The tile numbers and rings run on across
+// segments.  A new segment needs no drain: its Q_h is loaded once the last S_h of the old one is complete, during that
+// tile's softmax; its first PV_h, which overwrites O_h, waits for a P_h that the softmax warps write after their
+// epilogue has read O_h.
+// A row sees keys 0 .. limit; only tiles that reach behind the first token's limit are masked, with one compare per key.
+// Slots behind the unit's last key are not loaded or hold anything: their scores are masked, and their V rows are zeroed
+// in shared memory before the tile is released to the MMA (a probability of 0 does not silence a NaN).
+// P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16, independent per key), the sum is of the
+// unrounded fp32 values; S, statistics and O are fp32.
+#pragma once
+
+#include "attn_tc2.cuh"
+#include "paged.cuh"
+
+namespace cea {
+namespace paged {
+namespace tc {
+
+using cea::tc2::umma_ts;
+using cea::tc2::warp_wait;
+
+constexpr int BM = 128;
+constexpr int BK = 128;
+constexpr int NUM_THREADS = 384;
+constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 10, kMmaWarp1 = 11;
+constexpr int kLaunchRegs = 168, kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kLaunchRegs * NUM_THREADS, "register split");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kPCol = 64;
+constexpr float kRescaleThreshold = 8.0f;
+
+template <int D>
+struct Layout {
+  static constexpr int KBOX = D / 64;
+  static constexpr int BOX = 128 * 128;  // 64 columns of 128 rows
+  static constexpr int TILE = KBOX * BOX;
+  static constexpr int KST = D == 128 ? 3 : 5;
+  static constexpr int VST = D == 128 ? 2 : 5;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_V = OFF_K + KST * TILE;
+  static constexpr int OFF_BAR = OFF_V + VST * TILE;
+  static constexpr int B_QFULL = 0;  // x2
+  static constexpr int B_KFULL = B_QFULL + 2;
+  static constexpr int B_KEMPTY = B_KFULL + KST;
+  static constexpr int B_VFULL = B_KEMPTY + KST;
+  static constexpr int B_VEMPTY = B_VFULL + VST;
+  static constexpr int B_VTAIL = B_VEMPTY + VST;  // a V tile that is zeroed behind its last key before it counts as full
+  static constexpr int B_SFULL = B_VTAIL + 1;     // x2
+  static constexpr int B_PFULL = B_SFULL + 2;     // x2
+  static constexpr int B_PVDONE = B_PFULL + 2;    // x2
+  static constexpr int B_TURN = B_PVDONE + 2;     // x2
+  static constexpr int NBAR = B_TURN + 2;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int OFF_SCRATCH = OFF_MISC + 16;  // 34 int64 of the division
+  static constexpr int BYTES = OFF_SCRATCH + 34 * 8;
+  static constexpr int SMEM_ALLOC = BYTES + 1024;
+  static_assert(OFF_SCRATCH % 8 == 0 && SMEM_ALLOC <= 232448, "shared memory");
+};
+
+struct Params {
+  Batch bt;
+  Division dv;  // tb = 2 * half
+  int half;     // tokens of a half: 128 / G
+  int box;      // slots of a TMA box: divides the page and the tile
+  void* out;
+  int64_t o_ss, o_sh;
+  float* lse;
+  int64_t l_sh, l_ss;
+  float* part_o;
+  float* part_lse;
+  Meta* meta;
+  int out_dtype;
+  float scale_log2;
+};
+
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  auto bar = [&](int i) -> uint32_t { return sbase + L::OFF_BAR + 8 * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(bar(L::B_QFULL + h), 1);
+      mbar_init(bar(L::B_SFULL + h), 1);
+      mbar_init(bar(L::B_PFULL + h), 4);  // one arrival per softmax warp
+      mbar_init(bar(L::B_PVDONE + h), 1);
+      mbar_init(bar(L::B_TURN + h), 1);
+    }
+    for (int s = 0; s < L::KST; ++s) {
+      mbar_init(bar(L::B_KFULL + s), 1);
+      mbar_init(bar(L::B_KEMPTY + s), 2);  // released by each half, with or without a product
+    }
+    for (int s = 0; s < L::VST; ++s) {
+      mbar_init(bar(L::B_VFULL + s), 1);
+      mbar_init(bar(L::B_VEMPTY + s), 2);
+    }
+    mbar_init(bar(L::B_VTAIL), 1);
+    // after a device-side timeout nothing is computed
+    *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kKWarp && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  const Share sh = divide(p.bt, p.dv, reinterpret_cast<int64_t*>(smem + L::OFF_SCRATCH));
+  asm volatile("griddepcontrol.launch_dependents;");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool dead = *abort_flag != 0;
+
+  if (warp >= kKWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kKWarp || warp == kVWarp) {
+      // ---------------------------------------------------------- TMA producers, one box per lane
+      const bool is_k = warp == kKWarp;
+      const CUtensorMap* map = is_k ? &tmK : &tmV;
+      const int nst = is_k ? L::KST : L::VST;
+      const uint32_t off = sbase + (is_k ? L::OFF_K : L::OFF_V);
+      const int b_full = is_k ? L::B_KFULL : L::B_VFULL, b_empty = is_k ? L::B_KEMPTY : L::B_VEMPTY;
+      const int nbox = BK / p.box;
+      const int box = lane % nbox, col = lane / nbox;
+      const bool mine = col < L::KBOX;
+      int u = 0;
+      uint32_t tails = 0;
+      bool ok = !dead;
+      MetaPair meta;
+      for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+        meta.note(g);
+        const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
+        for (int t = g.t0; t < g.t1; ++t, ++u) {
+          const int st = u % nst;
+          const uint32_t n = u / nst;
+          const int key = t * BK + box * p.box;
+          const bool load = mine && key < g.keys;
+          int page = 0, slot = 0;
+          if (load) {
+            const int page_i = key / p.bt.ps;
+            slot = key - page_i * p.bt.ps;
+            page = table[page_i];
+            if (page < 0 || page >= p.bt.num_pages) {
+              report(CEA_DEV_BAD_PAGE);
+              page = p.bt.num_pages;  // outside the tensor map: reads as zeros
+            }
+          }
+          if (n > 0) ok = mbar_wait(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int boxes = __popc(__ballot_sync(0xffffffffu, load));
+          const int left = g.keys - t * BK;
+          const bool tail = !is_k && left < BK;
+          const uint32_t to = off + st * L::TILE;
+          const uint32_t fb = tail ? bar(L::B_VTAIL) : bar(b_full + st);
+          if (lane == 0) mbar_arrive_expect_tx(fb, boxes * p.box * 128);
+          __syncwarp();
+          if (load) tma_load_4d(to + col * L::BOX + box * p.box * 128, map, fb, col * 64, slot, g.hu, page);
+          if (tail) {
+            ok = mbar_wait(bar(L::B_VTAIL), tails & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++tails;
+            uint8_t* tile = smem + L::OFF_V + st * L::TILE;
+            for (int i = max(left, 0) * 8 + lane; i < BK * 8; i += 32)
+#pragma unroll
+              for (int c = 0; c < L::KBOX; ++c)
+                *reinterpret_cast<uint4*>(tile + c * L::BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(b_full + st));
+          }
+        }
+      }
+      if (is_k && lane == 0) meta.store(p.meta);
+    } else if (lane == 0 && !dead) {
+      // ---------------------------------------------------------- MMA issuer of half h (one thread)
+      const int h = warp == kMmaWarp ? 0 : 1;
+      constexpr uint32_t kIdescQK = idesc_f16(kBF16, false, BM, BK);
+      constexpr uint32_t kIdescPV = idesc_f16(kBF16, true, BM, D);
+      const uint32_t tS = tmem + 256 * h;
+      const uint32_t tP = tS + kPCol;
+      const uint32_t tO = tS + 128;
+      const uint64_t qdesc = sw128_desc(sbase + L::OFF_Q + h * L::TILE, 16, 1024);
+      const uint64_t kdesc0 = sw128_desc(sbase + L::OFF_K, 16, 1024);
+      const uint64_t vdesc0 = sw128_desc(sbase + L::OFF_V, L::BOX, 1024);
+      int u = 0;        // tile number, both halves alike
+      int cnt = 0;      // tiles this half computed
+      uint32_t nq = 0;  // segments this half loaded Q for
+      bool pend = false, pend_first = false;  // PV of tile u - 1 is to be issued; it begins its segment
+      bool ok = true;
+      // pair u: PV_h(u - 1), then S_h(u) if there is a tile u
+      auto pair = [&](bool has_s, bool act, bool first) -> bool {
+        if (has_s && !mbar_wait(bar(L::B_KFULL + u % L::KST), (u / L::KST) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA))
+          return false;
+        const int vs = (u - 1) % L::VST;
+        if (u > 0) {
+          if (pend && !mbar_spin(bar(L::B_PFULL + h), (cnt - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
+          if (!mbar_wait(bar(L::B_VFULL + vs), ((u - 1) / L::VST) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
+        }
+        const bool turn = h == 0 ? (u == 0 || mbar_spin(bar(L::B_TURN + 1), (u - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA))
+                                 : mbar_spin(bar(L::B_TURN + 0), u & 1, abort_flag, CEA_DEV_TIMEOUT_MMA);
+        if (!turn) return false;
+        tc_fence_after();
+        if (pend) {
+          const uint64_t vdesc = vdesc0 + static_cast<uint64_t>((vs * L::TILE) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            umma_ts(tO, tP + kk * 8, vdesc + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
+                    (!pend_first || kk > 0) ? 1u : 0u);
+          umma_commit(bar(L::B_PVDONE + h));
+          umma_commit(bar(L::B_VEMPTY + vs));
+        } else if (u > 0) {
+          mbar_arrive(bar(L::B_VEMPTY + vs));
+        }
+        if (has_s) {
+          const int ks = u % L::KST;
+          if (act) {
+            if (first && !mbar_wait(bar(L::B_QFULL + h), (nq - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
+            const uint64_t kdesc = kdesc0 + static_cast<uint64_t>((ks * L::TILE) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * L::BOX + (kk & 3) * 32) >> 4;
+              umma_ss(tS, qdesc + o, kdesc + o, kIdescQK, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(bar(L::B_SFULL + h));
+            umma_commit(bar(L::B_KEMPTY + ks));
+            ++cnt;
+          } else {
+            mbar_arrive(bar(L::B_KEMPTY + ks));
+          }
+        }
+        mbar_arrive(bar(L::B_TURN + h));
+        pend = has_s && act;
+        pend_first = first;
+        return true;
+      };
+      for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+        const int tok = g.blk * p.dv.tb + h * p.half;
+        const bool act = tok < g.s.n || h == 0;
+        if (act) {
+          // Q_h is free once this half's last S is complete
+          if (cnt > 0 && !mbar_spin(bar(L::B_SFULL + h), (cnt - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(bar(L::B_QFULL + h), L::KBOX * 128 * p.half * p.dv.group);
+#pragma unroll
+          for (int kb = 0; kb < L::KBOX; ++kb)
+            tma_load_4d(sbase + L::OFF_Q + h * L::TILE + kb * L::BOX, &tmQ, bar(L::B_QFULL + h), kb * 64,
+                        g.hu * p.dv.group, g.s.row0 + tok, 0);
+          ++nq;
+        }
+        for (int t = g.t0; ok && t < g.t1; ++t) {
+          ok = pair(true, act, t == g.t0);
+          ++u;
+        }
+      }
+      if (ok && u > 0) pair(false, false, false);
+    }
+  } else {
+    // ================================================================ softmax + epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int h = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 256 * h + lane_base;
+    const uint32_t tO = tmem + 256 * h + 128 + lane_base;
+    const int G = p.dv.group;
+    const int row_tok = row / G, row_head = row - row_tok * G;
+    int it = 0;  // tiles this half computed
+    bool ok = !dead;
+    for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+      const int tok0 = g.blk * p.dv.tb + h * p.half;
+      if (tok0 >= g.s.n && h == 1) continue;
+      const int tok = tok0 + row_tok;
+      const bool row_in = row_tok < p.half && tok < g.s.n;
+      const int seen = g.s.len - 1;
+      const int limit = !row_in ? -1 : (p.dv.causal ? min(g.s.ctx + tok, seen) : seen);
+      const int first_limit = p.dv.causal ? min(g.s.ctx + tok0, seen) : seen;  // of the half's first token
+      float m = -INFINITY, l = 0.f;
+      for (int t = g.t0; t < g.t1; ++t) {
+        if (!warp_wait(bar(L::B_SFULL + h), it & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[BK];
+#pragma unroll
+        for (int c = 0; c < BK / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        tmem_wait_ld();
+        float mx[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) mx[a] = -INFINITY;
+        if (t * BK + BK - 1 > first_limit) {
+          const int vis = limit - t * BK;  // keys 0 .. vis of the tile
+#pragma unroll
+          for (int j = 0; j < BK; ++j) {
+            if (j > vis) s[j] = __float_as_uint(-INFINITY);
+            mx[j & 7] = fmaxf(mx[j & 7], __uint_as_float(s[j]));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < BK; ++j) mx[j & 7] = fmaxf(mx[j & 7], __uint_as_float(s[j]));
+        }
+        const float tmax =
+            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) *
+            p.scale_log2;
+        const float m_new = fmaxf(m, tmax);
+        const bool rescale = (m != -INFINITY) && (m_new > m + kRescaleThreshold);
+        float alpha = 1.f;
+        if (m == -INFINITY) {
+          m = m_new;
+        } else if (rescale) {
+          alpha = fast_exp2(m - m_new);
+          l *= alpha;
+          m = m_new;
+        }
+        const float neg_m = (m == -INFINITY) ? 0.f : -m;
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        uint64_t rs2[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) rs2[a] = 0ull;
+        const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+        const uint64_t negm2 = f2_pack(neg_m, neg_m);
+#pragma unroll
+        for (int c = 0; c < BK / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])),
+                             scale2, negm2),
+                      x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            rs2[e & 3] = f2_add(rs2[e & 3], f2_pack(p0, p1));
+            pk[e] = pack2(p0, p1, kBF16);
+          }
+          tmem_st16(tS + kPCol + c * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_PFULL + h));
+        {
+          const uint64_t r = f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3]));
+          float r0, r1;
+          f2_unpack(r, r0, r1);
+          l += r0 + r1;
+        }
+        ++it;
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------------- epilogue of the segment
+      // S_h(it - 1) completed, hence PV_h(it - 2) did: the parity wait for PV_h(it - 1) is unambiguous
+      ok = warp_wait(bar(L::B_PVDONE + h), (it - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX);
+      if (!ok) break;
+      tc_fence_after();
+      const float inv_l = l == 0.f ? 0.f : 1.f / l;
+      const float lse_row = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      const int slot = segment_slot(g);
+      const int head = g.hu * G + row_head;
+      const int64_t trow = static_cast<int64_t>(g.s.row0) + tok;
+      const int64_t obase = trow * p.o_ss + head * p.o_sh;
+      const int64_t prow = static_cast<int64_t>(slot) * (2 * BM) + h * p.half * G + row;
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld16(tO + c * 16, o);
+        tmem_wait_ld();
+        if (!row_in) continue;
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv_l;
+        if (slot >= 0 || p.out_dtype == CEA_F32) {
+          float* dst = slot >= 0 ? p.part_o + prow * D + c * 16 : reinterpret_cast<float*>(p.out) + obase + c * 16;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(dst + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        } else {
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + obase + c * 16;
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack2(f[e], f[e + 1], kBF16), pack2(f[e + 2], f[e + 3], kBF16),
+                                                            pack2(f[e + 4], f[e + 5], kBF16),
+                                                            pack2(f[e + 6], f[e + 7], kBF16));
+        }
+      }
+      tc_fence_before();
+      if (row_in) {
+        if (slot >= 0) p.part_lse[prow] = lse_row;
+        else if (p.lse != nullptr) p.lse[head * p.l_sh + trow * p.l_ss] = lse_row;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+}  // namespace tc
+}  // namespace paged
+}  // namespace cea

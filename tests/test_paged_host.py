@@ -267,7 +267,10 @@ def test_choice_of_kernels():
             setattr(p, n, v)
         return lib.cea_paged_attn_kernels(ctypes.byref(p))
 
-    assert mask() == _lib.PAGED_DECODE and mask(max_q_len=4) == _lib.PAGED_DECODE
+    assert mask() == _lib.PAGED_DECODE and mask(max_q_len=4) == _lib.PAGED_DECODE  # 4 query heads share a KV head
+    assert mask(max_q_len=5) == _lib.PAGED_DECODE | _lib.PAGED_TC and mask(min_q_len=5, max_q_len=5) == _lib.PAGED_TC
+    assert mask(q=FAKE + 8, max_q_len=5) == _lib.PAGED_SIMT and mask(q=FAKE + 8) == _lib.PAGED_DECODE
+    assert mask(Hq=2 * 64, out=FAKE + 2) == _lib.PAGED_SIMT and mask(Hq=2 * 64) == _lib.PAGED_TC
     for kw in ({"in_dtype": _lib.F32, "out_dtype": _lib.F32}, {"D": 80}, {"page_size": 12}, {"k_pages": FAKE + 2},
                {"v_stride": (2 * 16 * 128, 16 * 128, 132)}, {"num_pages": 0}):
         assert mask(**kw) == _lib.PAGED_SIMT, kw
