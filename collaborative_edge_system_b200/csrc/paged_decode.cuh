@@ -2,15 +2,18 @@
 // a decoding step and of a few proposed tokens.
 //
 // HBM-bound: K and V are read once, about 4 FLOP per byte at a group of 4 query heads.  One CTA per SM takes an
-// equal share of all key tiles of the batch (paged.cuh), so lengths may differ at will and no CTA idles; a warp
-// streams 64-key K and V tiles into a ring of 192 KB with TMA, one box per page (or part of one), its lanes looking
-// the pages up and issuing the boxes side by side; the ring runs on across the segments of a share, so the loads do not
-// pause while four consumer warps join their results.  Consumer warp w takes keys 16w .. 16w + 15 of a tile for the 16
-// (padded) query rows on mma.sync m16n8k16: S = Q K^T, online softmax in the log2 domain, O += P V.  P is carried as
-// the sum of two 16-bit numbers (the value's rounding and the rounding of what that leaves, 2^-17 of the value for
-// bf16), which doubles the PV products and makes the result as exact as fp32 probabilities; the products are far from
-// the bound.  TMA boxes behind the last key are not loaded, and the V fragments of keys behind it are zeroed in
-// registers, so slots that hold no token never count, whatever they hold.
+// equal share of all key tiles of the batch (paged.cuh), so lengths may differ at will and no CTA idles; four
+// warps stream 64-key K and V tiles into a ring of 192 KB with TMA, one box per page (or part of one) and 64 columns,
+// each lane looking its box's page up a tile ahead (issuing a box takes a warp about 60 ns whichever lane does it, so
+// one warp could not keep up with pages of 16: 4470 GB/s); the ring runs on across the segments of a share, so the loads do not
+// pause while the consumer warps join their results.  Two groups of four consumer warps take the tiles in turn, each
+// warp 16 keys, transposed on mma.sync m16n8k16 so that the keys (and then the columns of V) fill the 16 rows and the few
+// query rows the 8 columns: S^T = K Q^T, online softmax in the log2 domain down the columns, O^T += V^T P^T.  With
+// the query rows on the 16-row side instead, half of each product was padding at 4 or 8 rows.  P is carried as the
+// sum of two 16-bit numbers (the value's rounding and the rounding of what that leaves, 2^-17 of the value for bf16),
+// which doubles the PV products and makes the result as exact as fp32 probabilities.  TMA boxes behind the last
+// key are not loaded, and the V fragments of keys behind it are zeroed in registers, so slots that hold no token never
+// count, whatever they hold.
 #pragma once
 
 #include "decode.cuh"
@@ -26,8 +29,9 @@ using cea::dec::mma16816;
 using cea::dec::swz;
 
 constexpr int BK = 64;
-constexpr int NCW = 4;
-constexpr int NTHREADS = (NCW + 1) * 32;
+constexpr int NCW = 8;  // consumer warps: two groups of four
+constexpr int NPW = 4;  // producer warps
+constexpr int NTHREADS = (NCW + NPW) * 32;
 constexpr int ROWS = 16;
 
 template <int D>
@@ -37,9 +41,10 @@ struct Layout {
   static constexpr int TILE = KBOX * BOX;
   static constexpr int STAGE = 2 * TILE;
   static constexpr int NSTAGE = 196608 / STAGE;
-  static constexpr int LDO = D + 4;
-  static constexpr int OFF_MERGE = NSTAGE * STAGE;  // [NCW][16] max, sum, then [NCW][16][LDO]
-  static constexpr int OFF_BAR = OFF_MERGE + NCW * ROWS * (LDO + 2) * 4;
+  static constexpr int DT = D / 16;
+  static constexpr int OFF_MERGE = NSTAGE * STAGE;          // [NCW][DT][32] float4: fragments of 8 query rows
+  static constexpr int OFF_STAT = OFF_MERGE + NCW * DT * 32 * 16;  // [NCW][16] max, then sum
+  static constexpr int OFF_BAR = OFF_STAT + 2 * NCW * ROWS * 4;
   static constexpr int OFF_MISC = OFF_BAR + 2 * NSTAGE * 8;
   static constexpr int BYTES = OFF_MISC + 16;
   static constexpr int SMEM_ALLOC = BYTES + 1024;
@@ -69,6 +74,222 @@ __device__ __forceinline__ float round16(float x) {
   return __half2float(__float2half_rn(x));
 }
 
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// One segment of a consumer warp, for NT x 8 query rows; `it` is the running number of the segment's first tile.
+// Once a wait has expired (`ok` false) a warp reads no more tiles, but it still meets the others at every join.
+template <int D, bool kBF16, int NT>
+__device__ __forceinline__ bool consume(const Params& p, const Segments<BK>& g, int it, bool ok, uint8_t* smem,
+                                        uint32_t sbase, volatile int* abort_flag, int warp, int lane) {
+  using L = Layout<D>;
+  const int grp = warp >> 2, key0 = (warp & 3) * 16;  // this warp's keys within a tile
+  const int G = p.dv.group, R = g.s.n * G;
+  const int mi = lane >> 3, ri = lane & 7, kr = lane >> 2, c2 = 2 * (lane & 3);
+
+  // Q^T fragments: rows nt * 8 + kr
+  uint32_t qb[NT][D / 16][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + kr;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
+                          (static_cast<int64_t>(g.s.row0) + r / G) * p.q_ss + (g.hu * G + r % G) * p.q_sh + c2;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qb[nt][kk][0] = r < R ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+      qb[nt][kk][1] = r < R ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+    }
+  }
+  // last key that rows nt * 8 + c2, + 1 see, -1 for none
+  int lim[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + c2 + e, seen = g.s.len - 1;
+      lim[nt][e] = r >= R ? -1 : (p.dv.causal ? min(g.s.ctx + r / G, seen) : seen);
+    }
+
+  float o[NT][D / 16][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
+
+  for (int t = g.t0; ok && t < g.t1; ++t, ++it) {
+    if ((it & 1) != grp) continue;
+    const int st = it % L::NSTAGE;
+    const bool got = mbar_wait(sbase + L::OFF_BAR + 8 * st, (it / L::NSTAGE) & 1, abort_flag, CEA_DEV_TIMEOUT_DECODE);
+    ok = __all_sync(0xffffffffu, got);
+    if (!ok) break;
+    const uint32_t kt = sbase + st * L::STAGE;
+    const uint32_t vt = kt + L::TILE;
+    const int left = g.keys - t * BK;  // keys of the unit in this tile
+    if (left > key0) {                 // warp-uniform: else none of this warp's keys exists
+      float s[NT][2][4];               // two chains of products, added below
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        ldsm_x4(swz(kt, key0 + ((mi & 1) << 3) + ri, 2 * kk + (mi >> 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(s[nt][kk & 1], a, qb[nt][kk][0], qb[nt][kk][1]);
+      }
+      const int kA = t * BK + key0 + kr, kB = kA + 8;
+      uint32_t pb[NT][2], pl[NT][2];  // P^T = pb + pl
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = (s[nt][0][e] + s[nt][1][e]) * p.scale_log2;
+          x[e] = (e < 2 ? kA : kB) <= lim[nt][e & 1] ? v : -INFINITY;
+        }
+        float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+        }
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float nm = fmaxf(m[nt][e], top[e]);
+          const float u = nm == -INFINITY ? 0.f : nm;
+          alpha[e] = fast_exp2(m[nt][e] - u);
+          m[nt][e] = nm;
+          x[e] = fast_exp2(x[e] - u);
+          x[2 + e] = fast_exp2(x[2 + e] - u);
+          l[nt][e] = l[nt][e] * alpha[e] + x[e] + x[2 + e];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float y0 = x[2 * i], y1 = x[2 * i + 1];
+          pb[nt][i] = transpose8x8(pack2(y0, y1, kBF16));
+          pl[nt][i] = transpose8x8(pack2(y0 - round16<kBF16>(y0), y1 - round16<kBF16>(y1), kBF16));
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[nt][i][0] *= alpha[0];
+            o[nt][i][1] *= alpha[1];
+            o[nt][i][2] *= alpha[0];
+            o[nt][i][3] *= alpha[1];
+          }
+        }
+      }
+      // V^T fragment words hold keys c2, c2 + 1 of the first or second 8 keys
+      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+      if (left < key0 + 16) {
+        const int k0 = key0 + c2;
+        keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
+        keep1 = (k0 + 8 < left ? 0xffffu : 0u) | (k0 + 9 < left ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t a[4];
+        ldsm_x4_t(swz(vt, key0 + ((mi >> 1) << 3) + ri, 2 * i + (mi & 1)), a[0], a[1], a[2], a[3]);
+        a[0] &= keep0;
+        a[1] &= keep0;
+        a[2] &= keep1;
+        a[3] &= keep1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<kBF16>(o[nt][i], a, pb[nt][0], pb[nt][1]);
+          mma16816<kBF16>(o[nt][i], a, pl[nt][0], pl[nt][1]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sbase + L::OFF_BAR + 8 * (L::NSTAGE + st));
+  }
+
+  // ------------------------------------------------- join the warps' results, in the order of the warps
+  float4* os = reinterpret_cast<float4*>(smem + L::OFF_MERGE);
+  float* ms = reinterpret_cast<float*>(smem + L::OFF_STAT);
+  float* ls = ms + NCW * ROWS;
+  const int slot = segment_slot(g);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+    asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32));  // the previous reads of the scratch
+    if (kr == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ms[warp * ROWS + nt * 8 + c2 + e] = m[nt][e];
+        ls[warp * ROWS + nt * 8 + c2 + e] = l[nt][e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      os[(warp * L::DT + i) * 32 + lane] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+    asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32));
+    // warp i of the eight: columns 16 i .. 16 i + 15 of all rows (D = 64: the first four)
+    if (warp < L::DT) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f}, sum[2], lse[2];
+      float wt[2][NCW];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + c2 + e;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NCW; ++w) mx = fmaxf(mx, ms[w * ROWS + r]);
+        const float u = mx == -INFINITY ? 0.f : mx;
+        sum[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < NCW; ++w) {
+          wt[e][w] = fast_exp2(ms[w * ROWS + r] - u);
+          sum[e] += wt[e][w] * ls[w * ROWS + r];
+        }
+        lse[e] = sum[e] == 0.f ? -INFINITY : (u + log2f(sum[e])) * kLn2;
+        sum[e] = sum[e] == 0.f ? 0.f : 1.f / sum[e];
+      }
+#pragma unroll
+      for (int w = 0; w < NCW; ++w) {
+        const float4 f = os[(w * L::DT + warp) * 32 + lane];
+        v[0] += wt[0][w] * f.x;
+        v[1] += wt[1][w] * f.y;
+        v[2] += wt[0][w] * f.z;
+        v[3] += wt[1][w] * f.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + c2 + e;
+        if (r >= R) continue;
+        const int64_t trow = static_cast<int64_t>(g.s.row0) + r / G;
+        const int head = g.hu * G + r % G;
+        const int d = warp * 16 + kr;
+        const float x = v[e] * sum[e], y = v[2 + e] * sum[e];
+        if (slot >= 0) {
+          float* po = p.part_o + (static_cast<int64_t>(slot) * ROWS + r) * D;
+          po[d] = x;
+          po[d + 8] = y;
+          if (warp == 0 && kr == 0) p.part_lse[static_cast<int64_t>(slot) * ROWS + r] = lse[e];
+        } else {
+          const int64_t at = trow * p.o_ss + head * p.o_sh + d;
+          store_out<float>(p.out, at, x, p.out_dtype);
+          store_out<float>(p.out, at + 8, y, p.out_dtype);
+          if (warp == 0 && kr == 0 && p.lse != nullptr) p.lse[head * p.l_sh + trow * p.l_ss] = lse[e];
+        }
+      }
+    }
+  }
+  return ok;
+}
+
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(NTHREADS)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -85,7 +306,7 @@ __global__ void __launch_bounds__(NTHREADS)
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::NSTAGE; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), NCW);
+      mbar_init(empty_bar(s), NCW / 2);
     }
     // after a device-side timeout nothing is computed (the shares below are walked without waiting for data)
     *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
@@ -96,15 +317,17 @@ __global__ void __launch_bounds__(NTHREADS)
   __syncthreads();
   const bool dead = *abort_flag != 0;
 
-  if (warp == NCW) {
-    // ---------------------------------------------------------------- producer: one TMA box per lane
-    if (lane == 0) {
+  if (warp >= NCW) {
+    // ---------------------------------------------------------------- producers: one TMA box per lane
+    const int pw = warp - NCW;
+    if (pw == 0 && lane == 0) {
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
-    __syncwarp();
     const int nbox = BK / p.box;  // boxes of 64 columns along a tile's keys
-    const int box = lane % nbox, half = (lane / nbox) % L::KBOX, is_v = lane / (nbox * L::KBOX);
+    // this lane's box of the tile's 2 x KBOX x nbox: dealt to the warps in turn
+    const int id = lane * NPW + pw;
+    const int box = id % nbox, half = (id / nbox) % L::KBOX, is_v = id / (nbox * L::KBOX);
     const bool mine = is_v < 2;
     const CUtensorMap* map = is_v == 1 ? &tmV : &tmK;
     const uint32_t dst0 = is_v * L::TILE + half * L::BOX + box * p.box * 128;
@@ -114,236 +337,50 @@ __global__ void __launch_bounds__(NTHREADS)
     for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
       meta.note(g);
       const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
+      // place of this lane's box in tile t: page (num_pages, outside the tensor map, reads as zeros), -1 for no load
+      auto place = [&](int t, int& slot) -> int {
+        const int key = t * BK + box * p.box;
+        if (!mine || t >= g.t1 || key >= g.keys) return -1;
+        const int page_i = key / p.bt.ps;
+        slot = key - page_i * p.bt.ps;
+        return table[page_i];
+      };
+      int slot = 0, slot_next = 0;
+      const int none = p.bt.num_pages;
+      int page_next = place(g.t0, slot_next);
       for (int t = g.t0; t < g.t1; ++t, ++it) {
         const int st = it % L::NSTAGE;
         const uint32_t n = it / L::NSTAGE;
-        const int key = t * BK + box * p.box;
-        const bool load = mine && key < g.keys;
-        int page = 0, slot = 0;
-        if (load) {
-          const int page_i = key / p.bt.ps;
-          slot = key - page_i * p.bt.ps;
-          page = table[page_i];
-          if (page < 0 || page >= p.bt.num_pages) {
-            report(CEA_DEV_BAD_PAGE);
-            page = p.bt.num_pages;  // outside the tensor map: reads as zeros
-          }
+        const bool load = mine && t * BK + box * p.box < g.keys;
+        int page = page_next;
+        slot = slot_next;
+        page_next = place(t + 1, slot_next);  // looked up a tile ahead
+        if (load && (page < 0 || page >= none)) {
+          report(CEA_DEV_BAD_PAGE);
+          page = none;
         }
         if (n > 0) ok = mbar_wait(empty_bar(st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_DECODE);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int boxes = __popc(__ballot_sync(0xffffffffu, load));
-        if (lane == 0) mbar_arrive_expect_tx(full_bar(st), boxes * p.box * 128);
-        __syncwarp();
+        if (pw == 0 && lane == 0) {
+          const int rows = min(nbox, (g.keys - t * BK + p.box - 1) / p.box) * p.box;
+          mbar_arrive_expect_tx(full_bar(st), max(rows, 0) * 2 * L::KBOX * 128);
+        }
+        // a box may land before the byte count is set: the phase waits for that one arrival
         if (load) tma_load_4d(sbase + st * L::STAGE + dst0, map, full_bar(st), half * 64, slot, g.hu, page);
       }
     }
-    if (lane == 0) meta.store(p.meta);
+    if (pw == 0 && lane == 0) meta.store(p.meta);
     return;
   }
 
   // ------------------------------------------------------------------ consumers
-  float* ms = reinterpret_cast<float*>(smem + L::OFF_MERGE);  // [NCW][16] max (log2 domain)
-  float* ls = ms + NCW * ROWS;                                // [NCW][16] sum
-  float* os = ls + NCW * ROWS;                                // [NCW][16][LDO]
-  const int G = p.dv.group;
-  const int rA = lane >> 2, rB = rA + 8;
-  const uint16_t* qg = reinterpret_cast<const uint16_t*>(p.q);
   int it = 0;
-  bool ok = !dead;
-  for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
-    const int R = g.s.n * G;
-    uint32_t qa[D / 16][4];
-    {
-      auto qrow = [&](int r) -> const uint16_t* {
-        return r < R ? qg + (static_cast<int64_t>(g.s.row0) + r / G) * p.q_ss + (g.hu * G + r % G) * p.q_sh : nullptr;
-      };
-      const uint16_t *qA = qrow(rA), *qB = qrow(rB);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const int d0 = kk * 16 + 2 * (lane & 3);
-        qa[kk][0] = qA ? *reinterpret_cast<const uint32_t*>(qA + d0) : 0u;
-        qa[kk][1] = qB ? *reinterpret_cast<const uint32_t*>(qB + d0) : 0u;
-        qa[kk][2] = qA ? *reinterpret_cast<const uint32_t*>(qA + d0 + 8) : 0u;
-        qa[kk][3] = qB ? *reinterpret_cast<const uint32_t*>(qB + d0 + 8) : 0u;
-      }
-    }
-    // last key each row sees, -1 for none
-    auto limit_of = [&](int r) -> int {
-      if (r >= R) return -1;
-      return p.dv.causal ? min(g.s.ctx + r / G, g.s.len - 1) : g.s.len - 1;
-    };
-    const int limA = limit_of(rA), limB = limit_of(rB);
-
-    float o[D / 8][4];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
-
-    for (int t = g.t0; t < g.t1; ++t, ++it) {
-      const int st = it % L::NSTAGE;
-      const bool got = mbar_wait(full_bar(st), (it / L::NSTAGE) & 1, abort_flag, CEA_DEV_TIMEOUT_DECODE);
-      ok = __all_sync(0xffffffffu, got);
-      if (!ok) break;
-      const uint32_t kt = sbase + st * L::STAGE;
-      const uint32_t vt = kt + L::TILE;
-      const int key0 = warp * 16;        // this warp's keys within the tile
-      const int left = g.keys - t * BK;  // keys of the unit in this tile
-      if (left > key0) {                 // warp-uniform: else none of this warp's keys exists
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        {
-          const int mi = lane >> 3, ri = lane & 7;
-          const int key = key0 + ((mi >> 1) << 3) + ri;
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t b0, b1, b2, b3;
-            ldsm_x4(swz(kt, key, 2 * kk + (mi & 1)), b0, b1, b2, b3);
-            mma16816<kBF16>(s[0], qa[kk], b0, b1);
-            mma16816<kBF16>(s[1], qa[kk], b2, b3);
-          }
-        }
-        float tA = -INFINITY, tB = -INFINITY;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = t * BK + key0 + nt * 8 + 2 * (lane & 3) + e;
-            s[nt][e] = key <= limA ? s[nt][e] * p.scale_log2 : -INFINITY;
-            s[nt][2 + e] = key <= limB ? s[nt][2 + e] * p.scale_log2 : -INFINITY;
-            tA = fmaxf(tA, s[nt][e]);
-            tB = fmaxf(tB, s[nt][2 + e]);
-          }
-        }
-#pragma unroll
-        for (int off = 1; off < 4; off <<= 1) {
-          tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, off));
-          tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, off));
-        }
-        const float nA = fmaxf(mA, tA), nB = fmaxf(mB, tB);
-        const float uA = nA == -INFINITY ? 0.f : nA, uB = nB == -INFINITY ? 0.f : nB;
-        const float aA = fast_exp2(mA - uA), aB = fast_exp2(mB - uB);
-        mA = nA;
-        mB = nB;
-        uint32_t pa[4], pl[4];  // P = pa + pl
-        {
-          float pv[2][4];
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            pv[nt][0] = fast_exp2(s[nt][0] - uA);
-            pv[nt][1] = fast_exp2(s[nt][1] - uA);
-            pv[nt][2] = fast_exp2(s[nt][2] - uB);
-            pv[nt][3] = fast_exp2(s[nt][3] - uB);
-          }
-          lA = lA * aA + pv[0][0] + pv[0][1] + pv[1][0] + pv[1][1];
-          lB = lB * aB + pv[0][2] + pv[0][3] + pv[1][2] + pv[1][3];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = pv[i >> 1][(i & 1) * 2], y = pv[i >> 1][(i & 1) * 2 + 1];
-            pa[i] = pack2(x, y, kBF16);
-            pl[i] = pack2(x - round16<kBF16>(x), y - round16<kBF16>(y), kBF16);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= aA;
-          o[i][1] *= aA;
-          o[i][2] *= aB;
-          o[i][3] *= aB;
-        }
-        // V fragment words hold keys 2 (lane & 3), + 1 of the first (b0, b2) or second (b1, b3) 8 keys
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if (left < key0 + 16) {
-          const int k0 = key0 + 2 * (lane & 3);
-          keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-          keep1 = (k0 + 8 < left ? 0xffffu : 0u) | (k0 + 9 < left ? 0xffff0000u : 0u);
-        }
-        {
-          const int mi = lane >> 3, ri = lane & 7;
-          const int key = key0 + ((mi & 1) << 3) + ri;
-#pragma unroll
-          for (int dn = 0; dn < D / 8; dn += 2) {
-            uint32_t b0, b1, b2, b3;
-            ldsm_x4_t(swz(vt, key, dn + (mi >> 1)), b0, b1, b2, b3);
-            b0 &= keep0;
-            b1 &= keep1;
-            b2 &= keep0;
-            b3 &= keep1;
-            mma16816<kBF16>(o[dn], pa, b0, b1);
-            mma16816<kBF16>(o[dn + 1], pa, b2, b3);
-            mma16816<kBF16>(o[dn], pl, b0, b1);
-            mma16816<kBF16>(o[dn + 1], pl, b2, b3);
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty_bar(st));
-    }
-    if (!ok) break;
-
-    // ------------------------------------------------- join the four warps' results, in the order of the warps
-    lA += __shfl_xor_sync(0xffffffffu, lA, 1);
-    lA += __shfl_xor_sync(0xffffffffu, lA, 2);
-    lB += __shfl_xor_sync(0xffffffffu, lB, 1);
-    lB += __shfl_xor_sync(0xffffffffu, lB, 2);
-    asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32));  // the previous segment's reads of the scratch
-    if ((lane & 3) == 0) {
-      ms[warp * ROWS + rA] = mA;
-      ms[warp * ROWS + rB] = mB;
-      ls[warp * ROWS + rA] = lA;
-      ls[warp * ROWS + rB] = lB;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const int d = i * 8 + 2 * (lane & 3);
-      *reinterpret_cast<float2*>(os + (warp * ROWS + rA) * L::LDO + d) = make_float2(o[i][0], o[i][1]);
-      *reinterpret_cast<float2*>(os + (warp * ROWS + rB) * L::LDO + d) = make_float2(o[i][2], o[i][3]);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32));
-    const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
-    if (row < R) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < NCW; ++w) mx = fmaxf(mx, ms[w * ROWS + row]);
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      float wsum = 0.f, wt[NCW];
-#pragma unroll
-      for (int w = 0; w < NCW; ++w) {
-        wt[w] = fast_exp2(ms[w * ROWS + row] - mu);
-        wsum += wt[w] * ls[w * ROWS + row];
-      }
-      const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
-      const float lse = wsum == 0.f ? -INFINITY : (mu + log2f(wsum)) * kLn2;
-      const int tok = row / G, head = g.hu * G + row % G;
-      const int64_t trow = static_cast<int64_t>(g.s.row0) + tok;
-      const int slot = segment_slot(g);
-      float* po = p.part_o + (static_cast<int64_t>(slot) * ROWS + row) * D;
-      const int64_t at = trow * p.o_ss + head * p.o_sh;
-      for (int d = 2 * part; d < D; d += 16) {
-        float x = 0.f, y = 0.f;
-#pragma unroll
-        for (int w = 0; w < NCW; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(os + (w * ROWS + row) * L::LDO + d);
-          x += wt[w] * v.x;
-          y += wt[w] * v.y;
-        }
-        x *= inv;
-        y *= inv;
-        if (slot >= 0) {
-          *reinterpret_cast<float2*>(po + d) = make_float2(x, y);
-        } else if (p.out_dtype == CEA_F32) {
-          reinterpret_cast<float*>(p.out)[at + d] = x;
-          reinterpret_cast<float*>(p.out)[at + d + 1] = y;
-        } else {
-          const uint32_t w = pack2(x, y, kBF16);
-          reinterpret_cast<uint16_t*>(p.out)[at + d] = static_cast<uint16_t>(w);
-          reinterpret_cast<uint16_t*>(p.out)[at + d + 1] = static_cast<uint16_t>(w >> 16);
-        }
-      }
-      if (part == 0) {
-        if (slot >= 0) p.part_lse[static_cast<int64_t>(slot) * ROWS + row] = lse;
-        else if (p.lse != nullptr) p.lse[head * p.l_sh + trow * p.l_ss] = lse;
-      }
-    }
+  bool ok = true;
+  for (Segments<BK> g(p.bt, p.dv, sh); !dead && !g.done(); g.next()) {
+    ok = g.s.n * p.dv.group <= 8 ? consume<D, kBF16, 1>(p, g, it, ok, smem, sbase, abort_flag, warp, lane)
+                                 : consume<D, kBF16, 2>(p, g, it, ok, smem, sbase, abort_flag, warp, lane);
+    it += g.t1 - g.t0;
   }
 }
 
