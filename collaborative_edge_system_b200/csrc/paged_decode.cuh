@@ -4,8 +4,10 @@
 // HBM-bound: K and V are read once, about 4 FLOP per byte at a group of 4 query heads.  One CTA per SM takes an
 // equal share of all key tiles of the batch (paged.cuh), so lengths may differ at will and no CTA idles; four
 // warps stream 64-key K and V tiles into a ring of 192 KB with TMA, one box per page (or part of one) and 64 columns,
-// each lane looking its box's page up a tile ahead (issuing a box takes a warp about 60 ns whichever lane does it, so
-// one warp could not keep up with pages of 16: 4470 GB/s); the ring runs on across the segments of a share, so the loads do not
+// each lane looking its box's page up; a warp takes about 60 ns a box and 0.5 us a tile, so four take the tiles in turn
+// (one warp for all of them: 2.8 TB/s at pages of 8 and 4.5 at 16; the boxes of each tile dealt to four warps: 5.3 and
+// 6.1, and 3.8 at D = 64; the tiles in turn: 6.5 and 6.5, and 6.0 at D = 64; 32 sequences of 16384, 8 KV heads);
+// the ring runs on across the segments of a share, so the loads do not
 // pause while the consumer warps join their results.  Two groups of four consumer warps take the tiles in turn, each
 // warp 16 keys, transposed on mma.sync m16n8k16 so that the keys (and then the columns of V) fill the 16 rows and the few
 // query rows the 8 columns: S^T = K Q^T, online softmax in the log2 domain down the columns, O^T += V^T P^T.  With
@@ -30,7 +32,7 @@ using cea::dec::swz;
 
 constexpr int BK = 64;
 constexpr int NCW = 8;  // consumer warps: two groups of four
-constexpr int NPW = 4;  // producer warps
+constexpr int NPW = 4;  // producer warps, which take the tiles in turn
 constexpr int NTHREADS = (NCW + NPW) * 32;
 constexpr int ROWS = 16;
 
@@ -319,15 +321,12 @@ __global__ void __launch_bounds__(NTHREADS)
 
   if (warp >= NCW) {
     // ---------------------------------------------------------------- producers: one TMA box per lane
-    const int pw = warp - NCW;
-    if (pw == 0 && lane == 0) {
+    if (warp == NCW && lane == 0) {
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
     const int nbox = BK / p.box;  // boxes of 64 columns along a tile's keys
-    // this lane's box of the tile's 2 x KBOX x nbox: dealt to the warps in turn
-    const int id = lane * NPW + pw;
-    const int box = id % nbox, half = (id / nbox) % L::KBOX, is_v = id / (nbox * L::KBOX);
+    const int box = lane % nbox, half = (lane / nbox) % L::KBOX, is_v = lane / (nbox * L::KBOX);
     const bool mine = is_v < 2;
     const CUtensorMap* map = is_v == 1 ? &tmV : &tmK;
     const uint32_t dst0 = is_v * L::TILE + half * L::BOX + box * p.box * 128;
@@ -347,14 +346,16 @@ __global__ void __launch_bounds__(NTHREADS)
       };
       int slot = 0, slot_next = 0;
       const int none = p.bt.num_pages;
-      int page_next = place(g.t0, slot_next);
-      for (int t = g.t0; t < g.t1; ++t, ++it) {
-        const int st = it % L::NSTAGE;
-        const uint32_t n = it / L::NSTAGE;
+      const int skip = (warp - NCW - it) & (NPW - 1);  // tiles to this warp's first one
+      int page_next = place(g.t0 + skip, slot_next);
+      for (int t = g.t0 + skip; t < g.t1; t += NPW) {
+        const int i = it + (t - g.t0);
+        const int st = i % L::NSTAGE;
+        const uint32_t n = i / L::NSTAGE;
         const bool load = mine && t * BK + box * p.box < g.keys;
         int page = page_next;
         slot = slot_next;
-        page_next = place(t + 1, slot_next);  // looked up a tile ahead
+        page_next = place(t + NPW, slot_next);  // looked up before this tile is waited for
         if (load && (page < 0 || page >= none)) {
           report(CEA_DEV_BAD_PAGE);
           page = none;
@@ -362,15 +363,14 @@ __global__ void __launch_bounds__(NTHREADS)
         if (n > 0) ok = mbar_wait(empty_bar(st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_DECODE);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (pw == 0 && lane == 0) {
-          const int rows = min(nbox, (g.keys - t * BK + p.box - 1) / p.box) * p.box;
-          mbar_arrive_expect_tx(full_bar(st), max(rows, 0) * 2 * L::KBOX * 128);
-        }
-        // a box may land before the byte count is set: the phase waits for that one arrival
+        const int boxes = __popc(__ballot_sync(0xffffffffu, load));
+        if (lane == 0) mbar_arrive_expect_tx(full_bar(st), boxes * p.box * 128);
+        __syncwarp();
         if (load) tma_load_4d(sbase + st * L::STAGE + dst0, map, full_bar(st), half * 64, slot, g.hu, page);
       }
+      it += g.t1 - g.t0;
     }
-    if (pw == 0 && lane == 0) meta.store(p.meta);
+    if (warp == NCW && lane == 0) meta.store(p.meta);
     return;
   }
 
