@@ -52,9 +52,9 @@ struct Division {
   int B, units_h, tb;   // units_h: units per block of tokens (KV heads x head groups)
   int group;            // query rows per token and unit
   int64_t max_rows, min_rows;  // sequences with n * group outside [min_rows, max_rows] belong to another kernel
-  int64_t served_min, served_max;  // range of n * group that this call's kernels serve between them
+  int min_n, max_n;  // what the caller promised of sequences with n > 0
   int causal;
-  int min_share;        // smallest share of the axis worth a CTA of its own
+  int min_share_log2;   // smallest share of the axis worth a CTA of its own; at least a tile
 };
 
 struct SeqUnits {
@@ -90,64 +90,98 @@ __device__ __forceinline__ SeqUnits seq_units(const Batch& bt, const Division& d
   return s;
 }
 
+// CTA c's share of an axis of length W: [base c + min(c, rem), base (c + 1) + min(c + 1, rem)), W = base n + rem.
 struct Share {
-  int64_t W, lo, hi;
-  int n;       // CTAs that take part
+  int64_t W, lo, hi, base;
+  int n, rem;  // CTAs that take part
   int b;       // sequence at lo
   int64_t at;  // where that sequence starts
+
+  __device__ __forceinline__ int64_t start(int c) const { return base * c + min(c, rem); }
+  // the CTA whose share holds x
+  __device__ __forceinline__ int cta_of(int64_t x) const {
+    const int64_t wide = (base + 1) * rem;  // the first rem shares are one longer
+    return x < wide ? static_cast<int>(div64(x, base + 1)) : rem + static_cast<int>(div64(x - wide, base));
+  }
+  // 64-bit division costs several hundred cycles, most axes fit 32 bits
+  __device__ __forceinline__ static int64_t div64(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+  }
 };
 
-// Called by every thread of the CTA (a multiple of 32 threads); `scratch` is 34 int64 in shared memory.
+// Called by every thread of the CTA (a multiple of 32 threads); `scratch` is 36 int64 in shared memory.
 __device__ __forceinline__ Share divide(const Batch& bt, const Division& dv, int64_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  int64_t sum = 0;
   const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
-  for (int b = threadIdx.x; b < dv.B; b += blockDim.x) {
+  // length on the axis of sequence b, 0 behind the last
+  auto weigh = [&](int b, bool check) -> int64_t {
+    if (b >= dv.B) return 0;
     const SeqUnits s = seq_units(bt, dv, b);
-    sum += s.S * dv.units_h;
-    // a length that the table cannot hold, descending offsets, or a sequence that no launched kernel serves
-    const int64_t rows = static_cast<int64_t>(s.n) * dv.group;
-    if (bt.lens[b] < 0 || bt.lens[b] > cap || bt.q_off[b + 1] < bt.q_off[b] || bt.q_off[b] < 0 ||
-        bt.q_off[b + 1] > bt.T || (s.n > 0 && (rows < dv.served_min || rows > dv.served_max)))
-      report(CEA_DEV_BAD_BATCH);
-  }
+    if (check) {
+      // a length that the table cannot hold, descending offsets, or a broken promise
+      const int raw = bt.lens[b], o0 = bt.q_off[b], o1 = bt.q_off[b + 1];
+      if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T ||
+          (s.n > 0 && (s.n < dv.min_n || s.n > dv.max_n)))
+        report(CEA_DEV_BAD_BATCH);
+    }
+    return s.S * dv.units_h;
+  };
+  auto scan = [&](int64_t w) -> int64_t {  // inclusive sum over the warp
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) scratch[warp] = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += up;
+    }
+    return w;
+  };
+  // a round of blockDim.x sequences: this thread's weight, and where its sequence starts within the round
+  int64_t w = weigh(threadIdx.x, true);
+  int64_t incl = scan(w);
+  int64_t more = 0;  // behind the first round
+  for (int b = threadIdx.x + blockDim.x; b < dv.B; b += blockDim.x) more += weigh(b, true);
+  if (dv.B > static_cast<int>(blockDim.x)) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+  }
+  if (lane == 31) scratch[warp] = incl + more;
+  if (threadIdx.x == 0) {
+    scratch[32] = dv.B;
+    scratch[33] = 0;
+  }
   __syncthreads();
   Share sh;
   sh.W = 0;
-  for (int w = 0; w < nw; ++w) sh.W += scratch[w];
-  sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W / dv.min_share)));
-  const int c = blockIdx.x;
-  sh.lo = c < sh.n ? sh.W * c / sh.n : sh.W;
-  sh.hi = c < sh.n ? sh.W * (c + 1) / sh.n : sh.W;
-  if (warp == 0) {
-    int64_t before = 0;
-    int found = dv.B;
-    int64_t at = sh.W;
-    for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += 32) {
-      const int b = b0 + lane;
-      const int64_t w = b < dv.B ? seq_units(bt, dv, b).S * dv.units_h : 0;
-      int64_t incl = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > sh.lo);
-      if (hit != 0u) {
-        const int l = __ffs(hit) - 1;
-        found = b0 + l;
-        at = before + __shfl_sync(0xffffffffu, incl - w, l);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
+  for (int i = 0; i < nw; ++i) sh.W += scratch[i];
+  sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W >> dv.min_share_log2)));
+  sh.base = Share::div64(sh.W, sh.n);
+  sh.rem = static_cast<int>(sh.W - sh.base * sh.n);
+  const int c = min(static_cast<int>(blockIdx.x), sh.n);
+  sh.lo = sh.start(c);
+  sh.hi = sh.start(min(c + 1, sh.n));
+  // the sequence that holds lo, round by round
+  int64_t before = 0;
+  for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += blockDim.x) {
+    if (b0 > 0) {
+      w = weigh(b0 + threadIdx.x, false);
+      incl = scan(w);
     }
-    if (lane == 0) {
-      scratch[32] = found;
-      scratch[33] = at;
+    if (dv.B > static_cast<int>(blockDim.x)) {
+      __syncthreads();
+      if (lane == 31) scratch[warp] = incl;
+      __syncthreads();
     }
+    int64_t round = 0;
+    for (int i = 0; i < nw; ++i) {
+      if (i == warp) incl += before + round;
+      round += scratch[i];
+    }
+    if (incl > sh.lo && incl - w <= sh.lo) {  // one thread of one round
+      scratch[32] = b0 + threadIdx.x;
+      scratch[33] = incl - w;
+    }
+    before += round;
+    if (before > sh.lo) break;
   }
   __syncthreads();
   sh.b = static_cast<int>(scratch[32]);
@@ -174,7 +208,7 @@ struct Segments {
     }
     s = seq_units(bt, dv, b);
     int64_t r = sh.lo - base;
-    hu = static_cast<int>(r / s.S);
+    hu = static_cast<int>(Share::div64(r, s.S));
     r -= hu * s.S;
     int lo = 0, hi = s.nb - 1;  // last block that starts at or before r
     while (lo < hi) {
@@ -224,8 +258,7 @@ struct Segments {
 
   // last CTA with a tile of this unit
   __device__ __forceinline__ int last_cta() const {
-    const int64_t x = pos + static_cast<int64_t>(nt - 1) * BK;
-    return static_cast<int>(((x + 1) * sh.n + sh.W - 1) / sh.W - 1);
+    return sh.cta_of(pos + static_cast<int64_t>(nt - 1) * BK);
   }
 };
 
@@ -237,38 +270,23 @@ __device__ __forceinline__ int segment_slot(const Segments<BK>& g) {
   return -1;
 }
 
-struct Meta {   // one per slot
-  int b, hu, blk;
-  int last;     // odd slots: last CTA that holds a part of the unit; even slots: 0 if the slot holds a part, else -1
-};
-
-// Descriptions of a CTA's two slots, gathered by a warp that walks the segments anyway.
-struct MetaPair {
-  Meta first = {0, 0, 0, -1}, behind = {0, 0, 0, -1};
+// The unit that goes on behind a CTA's share, gathered by a warp that walks the segments anyway.
+struct Meta {
+  int last;  // last CTA that holds a part of it; -1: no such unit
+  int hu, blk, row0, n;
 
   template <int BK>
   __device__ __forceinline__ void note(const Segments<BK>& g) {
-    if (g.t0 > 0) first.last = 0;
-    else if (g.t1 < g.nt) behind = Meta{g.b, g.hu, g.blk, g.last_cta()};
-  }
-  __device__ __forceinline__ void store(Meta* meta) const {
-    meta[2 * blockIdx.x] = first;
-    meta[2 * blockIdx.x + 1] = behind;
+    if (g.t0 == 0 && g.t1 < g.nt) *this = Meta{g.last_cta(), g.hu, g.blk, g.s.row0, g.s.n};
   }
 };
 
-// Joins the parts of units that several CTAs worked on:
-//   lse = ln sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
-// in the partials' precision, parts in the order of the keys (the result does not depend on timing).
-// Block (c, y): the unit that goes on behind CTA c (if one does), rows y * RPB ...; 8 / RPB warps share a row's parts.
-// Bound by latency: a call's partials (at most 2 per SM) sit in L2.
 template <typename A>
 struct CombineArgs {
-  Batch bt;
   Division dv;
   const A* part_o;    // [slot][rows][D]
   const A* part_lse;  // [slot][rows], natural log
-  const Meta* meta;
+  const Meta* meta;   // [CTA]
   int rows;           // rows of a slot
   void* out;
   int64_t o_ss, o_sh;
@@ -292,83 +310,118 @@ __device__ __forceinline__ double log_of(double x) { return log(x); }
 constexpr int kCombineThreads = 256;
 constexpr int kMaxD = 256;
 
+// 4 columns of a part; `vec`: rows are 16-byte aligned (D a multiple of 4)
+__device__ __forceinline__ void load4(const float* p, int left, bool vec, float (&v)[4]) {
+  if (vec) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? p[e] : 0.f;
+  }
+}
+__device__ __forceinline__ void load4(const double* p, int left, bool, double (&v)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < left ? p[e] : 0.0;
+}
+
+// Joins the parts of units that several CTAs worked on:
+//   lse = ln sum_i exp(lse_i),  out = sum_i exp(lse_i - lse) out_i
+// in the partials' precision, parts in the order of the keys (the result does not depend on timing).  The unit that
+// goes on behind CTA c has its first part in slot 2 c + 1 and the others in the slots 2 (c + 1), 2 (c + 2), ...: a share
+// is at least a tile long, so every CTA up to the unit's last one holds a part.
+// Block (c, y): rows y * RPB ...; 8 / RPB warps share a row's parts, a lane has 4 columns.  Bound by latency and L2: a
+// call's partials (at most 2 slots per CTA) are just written, so the weights of 32 parts are formed at once, one a lane,
+// and the parts are read four at a time.
 template <typename A, int RPB>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineArgs<A> a) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineArgs<A> a) {
   constexpr int WPR = 8 / RPB;  // warps per row
+  constexpr int C = kMaxD / 128;
   __shared__ A acc_s[WPR > 1 ? 8 : 1][WPR > 1 ? kMaxD : 1];
-  __shared__ A stat_s[8][2];
+  __shared__ A sum_s[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (*reinterpret_cast<volatile int*>(&g_cea_status) != 0) return;  // the parts may be missing after a timeout
   const int c = blockIdx.x;
-  const Meta m = a.meta[2 * c + 1];
+  const Meta m = a.meta[c];
   if (m.last < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.y * RPB + warp / WPR, sub = warp % WPR;
-  const Seq q = load_seq(a.bt, m.b);
-  const int tok = m.blk * a.dv.tb + row / a.dv.group, g = row % a.dv.group;
-  const int head = (m.hu / a.head_groups) * a.heads_per_kv + (m.hu % a.head_groups) * a.dv.group + g;
-  const bool in = row < a.dv.tb * a.dv.group && tok < q.n &&
-                  (m.hu % a.head_groups) * a.dv.group + g < a.heads_per_kv;
+  const int tok = m.blk * a.dv.tb + row / a.dv.group, g = (m.hu % a.head_groups) * a.dv.group + row % a.dv.group;
+  const int head = (m.hu / a.head_groups) * a.heads_per_kv + g;
+  const bool in = row < a.dv.tb * a.dv.group && tok < m.n && g < a.heads_per_kv;
   const int parts = m.last - c + 1;
-  auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
-  auto lse_of = [&](int i) -> A {
-    if (i > 0 && a.meta[slot(i)].last < 0) return -INFINITY;  // a CTA whose share holds no tile start
-    return a.part_lse[static_cast<int64_t>(slot(i)) * a.rows + row];
-  };
+  const bool vec = a.D % 4 == 0;
+  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
+  const int64_t orow = (static_cast<int64_t>(m.row0) + tok) * a.o_ss + head * a.o_sh;
+  const int64_t lrow = head * a.l_sh + (static_cast<int64_t>(m.row0) + tok) * a.l_ss;
   A top = -INFINITY, sum = 0;
+  A acc[C][4];
+#pragma unroll
+  for (int j = 0; j < C; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0;
   if (in) {
-    for (int i = lane; i < parts; i += 32) top = max(top, lse_of(i));
+    for (int i = lane; i < parts; i += 32) top = max(top, a.part_lse[slot(i) * a.rows + row]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // a row no part of which saw a key
-    const A ref = top == -INFINITY ? A(0) : top;
-    A acc[kMaxD / 32];
-#pragma unroll
-    for (int j = 0; j < kMaxD / 32; ++j) acc[j] = 0;
-    for (int i = sub; i < parts; i += WPR) {
-      const A w = exp_of(lse_of(i) - ref);
+    top = top == -INFINITY ? A(0) : top;  // a row no part of which saw a key
+    // this warp's parts: sub, sub + WPR, ...
+    for (int i0 = 0; i0 * WPR + sub < parts; i0 += 32) {
+      const int mine = (i0 + lane) * WPR + sub, here = min(32, (parts - sub - i0 * WPR + WPR - 1) / WPR);
+      const A w = mine < parts ? exp_of(a.part_lse[slot(mine) * a.rows + row] - top) : A(0);
       sum += w;
-      if (w == A(0)) continue;
-      const A* src = a.part_o + (static_cast<int64_t>(slot(i)) * a.rows + row) * a.D;
+      for (int i = 0; i < here; i += 4) {
+        A wi[4], v[4][C][4];
 #pragma unroll
-      for (int j = 0; j < kMaxD / 32; ++j)
-        if (j * 32 + lane < a.D) acc[j] += w * src[j * 32 + lane];
+        for (int k = 0; k < 4; ++k) {
+          wi[k] = __shfl_sync(0xffffffffu, w, (i + k) & 31);
+          if (i + k >= here) wi[k] = 0;
+          const A* src = a.part_o + (slot((i0 + min(i + k, here - 1)) * WPR + sub) * a.rows + row) * a.D;
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            v[k][j][0] = v[k][j][1] = v[k][j][2] = v[k][j][3] = 0;
+            if (j * 128 + lane * 4 < a.D) load4(src + j * 128 + lane * 4, a.D - j * 128 - lane * 4, vec, v[k][j]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + k < here) acc[j][e] += wi[k] * v[k][j][e];
+      }
     }
-    top = ref;
-    if constexpr (WPR == 1) {
-      const A inv = sum == A(0) ? A(0) : A(1) / sum;
-      const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.o_ss + head * a.o_sh;
 #pragma unroll
-      for (int j = 0; j < kMaxD / 32; ++j)
-        if (j * 32 + lane < a.D) store_out<A>(a.out, at + j * 32 + lane, acc[j] * inv, a.out_dtype);
-      if (lane == 0 && a.lse != nullptr)
-        a.lse[head * a.l_sh + static_cast<int64_t>(q.row0 + tok) * a.l_ss] =
-            sum == A(0) ? A(-INFINITY) : top + log_of(sum);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kMaxD / 32; ++j)
-        if (j * 32 + lane < a.D) acc_s[warp][j * 32 + lane] = acc[j];
-      if (lane == 0) stat_s[warp][0] = sum;
-    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if constexpr (WPR > 1) {
+  if constexpr (WPR == 1) {
+    if (!in) return;
+    const A inv = sum == A(0) ? A(0) : A(1) / sum;
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j * 128 + lane * 4 + e < a.D) store_out<A>(a.out, orow + j * 128 + lane * 4 + e, acc[j][e] * inv, a.out_dtype);
+    if (lane == 0 && a.lse != nullptr) a.lse[lrow] = sum == A(0) ? A(-INFINITY) : top + log_of(sum);
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc_s[warp][j * 128 + lane * 4 + e] = acc[j][e];
+    if (lane == 0) sum_s[warp] = sum;
     __syncthreads();
     if (!in) return;
     const int w0 = warp / WPR * WPR;
     A total = 0;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) total += stat_s[w0 + w][0];
+    for (int w = 0; w < WPR; ++w) total += sum_s[w0 + w];
     const A inv = total == A(0) ? A(0) : A(1) / total;
-    const int64_t at = static_cast<int64_t>(q.row0 + tok) * a.o_ss + head * a.o_sh;
     for (int d = sub * 32 + lane; d < a.D; d += WPR * 32) {
       A v = 0;
 #pragma unroll
       for (int w = 0; w < WPR; ++w) v += acc_s[w0 + w][d];
-      store_out<A>(a.out, at + d, v * inv, a.out_dtype);
+      store_out<A>(a.out, orow + d, v * inv, a.out_dtype);
     }
-    if (sub == 0 && lane == 0 && a.lse != nullptr)
-      a.lse[head * a.l_sh + static_cast<int64_t>(q.row0 + tok) * a.l_ss] =
-          total == A(0) ? A(-INFINITY) : top + log_of(total);
+    if (sub == 0 && lane == 0 && a.lse != nullptr) a.lse[lrow] = total == A(0) ? A(-INFINITY) : top + log_of(total);
   }
 }
 
@@ -408,6 +461,7 @@ template <typename U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int per = a.H * a.units;  // units of one token's K (or V)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int stride = gridDim.x * (kAppendThreads / 32);
   for (int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); t < a.bt.T; t += stride) {
     U val[2][kAppendUnroll];
@@ -469,6 +523,7 @@ template <typename U>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
   // blockIdx.x walks the chunks of a page, then the pairs; y the layers, z K or V
   constexpr int kChunk = kCopyThreads * kCopyUnroll;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int chunks = static_cast<int>((a.units + kChunk - 1) / kChunk);
   const int i = blockIdx.x / chunks;
   const int64_t u0 = static_cast<int64_t>(blockIdx.x % chunks) * kChunk + threadIdx.x;

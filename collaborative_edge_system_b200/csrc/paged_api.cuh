@@ -111,7 +111,7 @@ PagedPlan paged_plan(int grid, int rows, int D, size_t elem, size_t at) {
   pl.o = at;
   pl.lse = pl.o + align256(elem * 2 * grid * rows * D);
   pl.meta = pl.lse + align256(elem * 2 * grid * rows);
-  pl.bytes = pl.meta + align256(sizeof(pg::Meta) * 2 * grid);
+  pl.bytes = pl.meta + align256(sizeof(pg::Meta) * grid);
   return pl;
 }
 
@@ -161,7 +161,6 @@ int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const
                    cudaStream_t s) {
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::CombineArgs<A> c;
-  c.bt = paged_batch(p);
   c.dv = dv;
   c.part_o = reinterpret_cast<const A*>(ws + pl.o);
   c.part_lse = reinterpret_cast<const A*>(ws + pl.lse);
@@ -177,7 +176,8 @@ int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const
   c.out_dtype = p->out_dtype;
   c.heads_per_kv = p->Hq / p->Hkv;
   c.head_groups = head_groups;
-  const int rows = dv.tb * dv.group;
+  // no unit has more rows than a sequence of the batch
+  const int rows = static_cast<int>(std::min<int64_t>(dv.tb, p->max_q_len) * dv.group);
   const cudaError_t e = launch_dependent(pg::combine_kernel<A, RPB>, dim3(pl.grid, (rows + RPB - 1) / RPB),
                                          pg::kCombineThreads, 0, s, c);
   return e == cudaSuccess ? CEA_OK : fail(CEA_ERR_CUDA, "combine_kernel: %s", cudaGetErrorString(e));
@@ -190,8 +190,8 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::simt::Params<A> a;
   a.bt = paged_batch(p);
-  a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, 0, INT64_MAX, p->causal ? 1 : 0,
-                      pg::simt::BK};
+  a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, p->min_q_len, p->max_q_len, p->causal ? 1 : 0,
+                      5};
   a.q = p->q;
   a.k = p->k_pages;
   a.v = p->v_pages;
@@ -220,8 +220,8 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   auto k = pg::simt::attn_kernel<T, A, DMAX>;
   constexpr size_t bytes = pg::simt::smem_bytes<A, DMAX>();
   allow_smem(k, static_cast<int>(bytes));
-  k<<<pl.grid, pg::simt::NT, bytes, s>>>(a);
-  if (int e = cuda_check("paged attn_kernel")) return e;
+  if (const cudaError_t e = launch_dependent(k, dim3(pl.grid), pg::simt::NT, bytes, s, a))
+    return fail(CEA_ERR_CUDA, "paged attn_kernel: %s", cudaGetErrorString(e));
   return launch_combine<A, 8>(p, a.dv, pl, groups, s);
 }
 
@@ -238,13 +238,13 @@ bool paged_map(CUtensorMap* map, const cea_paged_attn_params* p, const void* ptr
   return make_map(map, p->in_dtype, ptr, p->D, p->page_size, p->Hkv, p->num_pages, st[2], st[1], st[0], rows);
 }
 
-int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, int kernels, cudaStream_t s) {
+int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStream_t s) {
   const int G = p->Hq / p->Hkv;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::dec::Params a;
   a.bt = paged_batch(p);
-  a.dv = pg::Division{p->B, p->Hkv, pg::dec::ROWS / G, G, pg::dec::ROWS, 0, 0,
-                      (kernels & kPagedTc) ? INT64_MAX : int64_t(pg::dec::ROWS), p->causal ? 1 : 0, pg::dec::BK};
+  a.dv = pg::Division{p->B, p->Hkv, pg::dec::ROWS / G, G, pg::dec::ROWS, 0, p->min_q_len, p->max_q_len,
+                      p->causal ? 1 : 0, 7};
   a.q = p->q;
   a.q_ss = p->q_stride[0];
   a.q_sh = p->q_stride[1];
@@ -263,11 +263,12 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, int
   CUtensorMap mk, mv;
   if (!paged_map(&mk, p, p->k_pages, p->k_stride, a.box) || !paged_map(&mv, p, p->v_pages, p->v_stride, a.box))
     return fail(CEA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the pages");
+  cudaError_t err = cudaSuccess;
 #define CEA_PDEC(DD, BF)                                                                  \
   do {                                                                                    \
     auto k = pg::dec::decode_kernel<DD, BF>;                                              \
     allow_smem(k, pg::dec::Layout<DD>::SMEM_ALLOC);                                       \
-    k<<<pl.grid, pg::dec::NTHREADS, pg::dec::Layout<DD>::SMEM_ALLOC, s>>>(mk, mv, a);     \
+    err = launch_dependent(k, dim3(pl.grid), pg::dec::NTHREADS, pg::dec::Layout<DD>::SMEM_ALLOC, s, mk, mv, a); \
   } while (0)
   const bool bf = p->in_dtype == CEA_BF16;
   if (p->D == 128) {
@@ -276,7 +277,7 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, int
     if (bf) CEA_PDEC(64, true); else CEA_PDEC(64, false);
   }
 #undef CEA_PDEC
-  if (int e = cuda_check("paged decode_kernel")) return e;
+  if (err != cudaSuccess) return fail(CEA_ERR_CUDA, "paged decode_kernel: %s", cudaGetErrorString(err));
   return launch_combine<float, 1>(p, a.dv, pl, 1, s);
 }
 
@@ -299,15 +300,14 @@ bool paged_q_map(CUtensorMap* map, const cea_paged_attn_params* p, int G, int to
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, int kernels, cudaStream_t s) {
+int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStream_t s) {
   const int G = p->Hq / p->Hkv;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::tc::Params a;
   a.bt = paged_batch(p);
   a.half = pg::tc::BM / G;
   a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, pg::dec::ROWS + 1,
-                      (kernels & kPagedDecode) ? 0 : int64_t(pg::dec::ROWS + 1), INT64_MAX, p->causal ? 1 : 0,
-                      2 * pg::tc::BK};
+                      p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 8};
   a.box = std::gcd(p->page_size, pg::tc::BK);
   a.out = p->out;
   a.o_ss = p->o_stride[0];
@@ -324,6 +324,7 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, int ker
   if (!paged_q_map(&mq, p, G, a.half) || !paged_map(&mk, p, p->k_pages, p->k_stride, a.box) ||
       !paged_map(&mv, p, p->v_pages, p->v_stride, a.box))
     return fail(CEA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the queries or the pages");
+  cudaError_t err = cudaSuccess;
 #define CEA_PTC(DD, BF)                                                                                    do {                                                                                                       auto k = pg::tc::chunk_kernel<DD, BF>;                                                                   if (int e = check_launch_regs(reinterpret_cast<const void*>(k), pg::tc::kLaunchRegs)) return e;          allow_smem(k, pg::tc::Layout<DD>::SMEM_ALLOC);                                                           k<<<pl.grid, pg::tc::NUM_THREADS, pg::tc::Layout<DD>::SMEM_ALLOC, s>>>(mq, mk, mv, a);                 } while (0)
   const bool bf = p->in_dtype == CEA_BF16;
   if (p->D == 128) {
@@ -332,7 +333,7 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, int ker
     if (bf) CEA_PTC(64, true); else CEA_PTC(64, false);
   }
 #undef CEA_PTC
-  if (int e = cuda_check("paged chunk_kernel")) return e;
+  if (err != cudaSuccess) return fail(CEA_ERR_CUDA, "paged chunk_kernel: %s", cudaGetErrorString(err));
   return launch_combine<float, 8>(p, a.dv, pl, 1, s);
 }
 
@@ -345,10 +346,10 @@ size_t paged_workspace(const cea_paged_attn_params* p, int kernels) {
 }
 
 template <typename U>
-void launch_append(const pg::AppendArgs& a, cudaStream_t s) {
+cudaError_t launch_append(const pg::AppendArgs& a, cudaStream_t s) {
   constexpr int per = pg::kAppendThreads / 32;
   const int grid = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(a.bt.T) + per - 1) / per, 148 * 16));
-  pg::append_kernel<U><<<grid, pg::kAppendThreads, 0, s>>>(a);
+  return launch_dependent(pg::append_kernel<U>, dim3(grid), pg::kAppendThreads, 0, s, a);
 }
 
 }  // namespace
@@ -377,12 +378,12 @@ int cea_paged_attn(const cea_paged_attn_params* p, void* stream) {
   size_t at = 0;
   if (kernels & kPagedDecode) {
     const PagedPlan pl = paged_decode_plan(p, at);
-    if (int e = launch_paged_decode(p, pl, kernels, s)) return e;
+    if (int e = launch_paged_decode(p, pl, s)) return e;
     at = pl.bytes;
   }
   if (kernels & kPagedTc) {
     const PagedPlan pl = paged_tc_plan(p, at);
-    if (int e = launch_paged_tc(p, pl, kernels, s)) return e;
+    if (int e = launch_paged_tc(p, pl, s)) return e;
     at = pl.bytes;
   }
   if (kernels & kPagedSimt) {
@@ -435,14 +436,15 @@ int cea_paged_append(const cea_paged_append_params* p, void* stream) {
   if (units * p->H > 0x7fffffff) return fail(CEA_ERR_UNSUPPORTED, "%s: %d heads of %d elements", what, p->H, p->D);
   a.units = static_cast<int>(units);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
   switch (unit) {
-    case 16: launch_append<uint4>(a, s); break;
-    case 8: launch_append<uint2>(a, s); break;
-    case 4: launch_append<uint32_t>(a, s); break;
-    case 2: launch_append<uint16_t>(a, s); break;
-    default: launch_append<uint8_t>(a, s); break;
+    case 16: e = launch_append<uint4>(a, s); break;
+    case 8: e = launch_append<uint2>(a, s); break;
+    case 4: e = launch_append<uint32_t>(a, s); break;
+    case 2: e = launch_append<uint16_t>(a, s); break;
+    default: e = launch_append<uint8_t>(a, s); break;
   }
-  return cuda_check(what);
+  return e == cudaSuccess ? CEA_OK : fail(CEA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 int cea_copy_pages(const cea_copy_pages_params* p, void* stream) {
@@ -490,14 +492,15 @@ int cea_copy_pages(const cea_copy_pages_params* p, void* stream) {
     a.n = std::min(pg::kCopyPairs, p->n - i0);
     for (int i = 0; i < a.n; ++i) a.pair[i] = make_int2(p->src[i0 + i], p->dst[i0 + i]);
     const dim3 grid(static_cast<unsigned>(chunks * a.n), std::min(p->layers, 65535), 2);
+    cudaError_t e;
     switch (unit) {
-      case 16: pg::copy_pages_kernel<uint4><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
-      case 8: pg::copy_pages_kernel<uint2><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
-      case 4: pg::copy_pages_kernel<uint32_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
-      case 2: pg::copy_pages_kernel<uint16_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
-      default: pg::copy_pages_kernel<uint8_t><<<grid, pg::kCopyThreads, 0, s>>>(a); break;
+      case 16: e = launch_dependent(pg::copy_pages_kernel<uint4>, grid, pg::kCopyThreads, 0, s, a); break;
+      case 8: e = launch_dependent(pg::copy_pages_kernel<uint2>, grid, pg::kCopyThreads, 0, s, a); break;
+      case 4: e = launch_dependent(pg::copy_pages_kernel<uint32_t>, grid, pg::kCopyThreads, 0, s, a); break;
+      case 2: e = launch_dependent(pg::copy_pages_kernel<uint16_t>, grid, pg::kCopyThreads, 0, s, a); break;
+      default: e = launch_dependent(pg::copy_pages_kernel<uint8_t>, grid, pg::kCopyThreads, 0, s, a); break;
     }
-    if (int e = cuda_check(what)) return e;
+    if (e != cudaSuccess) return fail(CEA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   }
   return CEA_OK;
 }

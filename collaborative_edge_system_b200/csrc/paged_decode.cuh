@@ -310,10 +310,13 @@ __global__ void __launch_bounds__(NTHREADS)
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), NCW / 2);
     }
-    // after a device-side timeout nothing is computed (the shares below are walked without waiting for data)
-    *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // after a device-side timeout nothing is computed
+  if (threadIdx.x == 0) *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
   const Share sh = divide(p.bt, p.dv, reinterpret_cast<int64_t*>(smem + L::OFF_MERGE));
   asm volatile("griddepcontrol.launch_dependents;");
   __syncthreads();
@@ -321,10 +324,6 @@ __global__ void __launch_bounds__(NTHREADS)
 
   if (warp >= NCW) {
     // ---------------------------------------------------------------- producers: one TMA box per lane
-    if (warp == NCW && lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
     const int nbox = BK / p.box;  // boxes of 64 columns along a tile's keys
     const int box = lane % nbox, half = (lane / nbox) % L::KBOX, is_v = lane / (nbox * L::KBOX);
     const bool mine = is_v < 2;
@@ -332,7 +331,7 @@ __global__ void __launch_bounds__(NTHREADS)
     const uint32_t dst0 = is_v * L::TILE + half * L::BOX + box * p.box * 128;
     int it = 0;
     bool ok = !dead;
-    MetaPair meta;
+    Meta meta{-1, 0, 0, 0, 0};
     for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
       meta.note(g);
       const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
@@ -370,7 +369,7 @@ __global__ void __launch_bounds__(NTHREADS)
       }
       it += g.t1 - g.t0;
     }
-    if (warp == NCW && lane == 0) meta.store(p.meta);
+    if (warp == NCW && lane == 0) p.meta[blockIdx.x] = meta;
     return;
   }
 

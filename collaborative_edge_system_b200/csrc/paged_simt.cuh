@@ -49,7 +49,7 @@ template <typename T> __device__ __forceinline__ float widen(T x, float) { retur
 template <typename T, typename A, int DMAX>
 __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ int64_t scratch[34];
+  __shared__ int64_t scratch[36];
   constexpr int LD = DMAX + 1;
   A* qs = reinterpret_cast<A*>(smem_raw);
   A* ks = qs + BQ * LD;
@@ -59,10 +59,11 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
   const T* kp = reinterpret_cast<const T*>(p.k);
   const T* vp = reinterpret_cast<const T*>(p.v);
   const int r = threadIdx.x / TPR, sub = threadIdx.x % TPR;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share sh = divide(p.bt, p.dv, scratch);
   asm volatile("griddepcontrol.launch_dependents;");
 
-  MetaPair meta;
+  Meta meta{-1, 0, 0, 0, 0};
   for (Segments<BK> g(p.bt, p.dv, sh); !g.done(); g.next()) {
     meta.note(g);
     const int kvh = g.hu / p.head_groups, g0 = (g.hu % p.head_groups) * p.dv.group;
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
       if (sub == 0) p.part_lse[at] = lse;
     }
   }
-  if (threadIdx.x == 0) meta.store(p.meta);
+  if (threadIdx.x == 0) p.meta[blockIdx.x] = meta;
 }
 
 }  // namespace simt

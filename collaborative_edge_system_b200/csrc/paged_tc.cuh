@@ -62,8 +62,8 @@ struct Layout {
   static constexpr int B_TURN = B_PVDONE + 2;     // x2
   static constexpr int NBAR = B_TURN + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int OFF_SCRATCH = OFF_MISC + 16;  // 34 int64 of the division
-  static constexpr int BYTES = OFF_SCRATCH + 34 * 8;
+  static constexpr int OFF_SCRATCH = OFF_MISC + 16;  // 36 int64 of the division
+  static constexpr int BYTES = OFF_SCRATCH + 36 * 8;
   static constexpr int SMEM_ALLOC = BYTES + 1024;
   static_assert(OFF_SCRATCH % 8 == 0 && SMEM_ALLOC <= 232448, "shared memory");
 };
@@ -114,8 +114,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(bar(L::B_VEMPTY + s), 2);
     }
     mbar_init(bar(L::B_VTAIL), 1);
-    // after a device-side timeout nothing is computed
-    *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -127,6 +125,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // after a device-side timeout nothing is computed
+  if (threadIdx.x == 0) *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
   const Share sh = divide(p.bt, p.dv, reinterpret_cast<int64_t*>(smem + L::OFF_SCRATCH));
   asm volatile("griddepcontrol.launch_dependents;");
   tc_fence_before();
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int u = 0;
       uint32_t tails = 0;
       bool ok = !dead;
-      MetaPair meta;
+      Meta meta{-1, 0, 0, 0, 0};
       for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
         meta.note(g);
         const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
       }
-      if (is_k && lane == 0) meta.store(p.meta);
+      if (is_k && lane == 0) p.meta[blockIdx.x] = meta;
     } else if (lane == 0 && !dead) {
       // ---------------------------------------------------------- MMA issuer of half h (one thread)
       const int h = warp == kMmaWarp ? 0 : 1;

@@ -342,9 +342,9 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * belong to no sequence are left as they were.  What does not fit is bounded on the
  * device and reported through cea_device_status (it stops no later kernel): a
  * table entry outside [0, num_pages) reads as zeros and is not written
- * (CEA_DEV_BAD_PAGE); descending offsets, a length that the table cannot hold or
- * a sequence outside [min_q_len, max_q_len] whose kernel was not launched is
- * CEA_DEV_BAD_BATCH.
+ * (CEA_DEV_BAD_PAGE); descending offsets, a length that the table cannot hold
+ * (it is cut) or a sequence with a number of new tokens outside [min_q_len,
+ * max_q_len] (its rows are undefined) is CEA_DEV_BAD_BATCH.
  *
  * cea_paged_attn: attention of the new tokens (n_b from 0 on, single tokens
  * included) over the cached ones; token i sees the keys at positions up to

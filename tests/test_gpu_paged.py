@@ -150,6 +150,28 @@ def test_batches_that_do_not_fit_the_call_are_reported(dtype):
         assert _lib.device_status(clear=True) == _lib.DEV_BAD_BATCH
 
 
+def test_broken_promises_are_reported():
+    assert _lib.device_status(clear=True) == 0
+    for dtype in (torch.bfloat16, torch.float32):
+        x = R.batch([60, 40], [2, 20], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype, device=DEV, seed=8)
+        for kw in ({"max_q_len": 19}, {"min_q_len": 3}, {"max_q_len": 1}):
+            cea.paged_attention(**x, **kw)
+            assert _lib.device_status(clear=True) == _lib.DEV_BAD_BATCH
+        cea.paged_attention(**x, min_q_len=2, max_q_len=20)
+        assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 16)])
+def test_more_sequences_than_threads(dtype, dim):
+    lens = [(i * 37) % 90 for i in range(1500)]
+    counts = [min(n, (0, 1, 1, 2, 17, 1, 30)[i % 7]) for i, n in enumerate(lens)]
+    x = R.batch(lens, counts, heads=4, kv_heads=2, dim=dim, page=8, dtype=TYPES[dtype], device=DEV, seed=15)
+    _check(x)
+    x = R.batch(lens, [min(c, 2) for c in counts], heads=4, kv_heads=2, dim=dim, page=8, dtype=TYPES[dtype], device=DEV,
+                seed=16)
+    _check(x, max_q_len=2)
+
+
 def test_long_contexts_split_over_the_gpu_and_are_deterministic():
     x = R.batch([60001, 7, 1500], [1, 1, 1], heads=8, kv_heads=1, dim=128, page=16, dtype=torch.bfloat16, device=DEV,
                 seed=9)
