@@ -76,12 +76,21 @@ __device__ __forceinline__ int unit_keys(const SeqUnits& s, int i, int tb, bool 
   return static_cast<int>(min(max(s.ctx + last, int64_t(0)), static_cast<int64_t>(s.len)));
 }
 
+// kOne: every sequence served is one block of tokens (tb >= its n), whose last token sees all its keys
+template <bool kOne>
 __device__ __forceinline__ SeqUnits seq_units(const Batch& bt, const Division& dv, int b) {
   const Seq q = load_seq(bt, b);
   SeqUnits s;
   s.n = q.n;
   s.len = q.len;
   s.row0 = q.row0;
+  if constexpr (kOne) {
+    s.nb = q.n > 0 && q.n <= dv.tb ? 1 : 0;
+    s.n0 = 0;
+    s.ctx = q.len - q.n;
+    s.S = s.nb * max(1, q.len);
+    return s;
+  }
   const int64_t rows = static_cast<int64_t>(q.n) * dv.group;
   s.nb = q.n > 0 && rows >= dv.min_rows && rows <= dv.max_rows ? (q.n + dv.tb - 1) / dv.tb : 0;
   s.ctx = q.len - q.n;  // may be negative: the first tokens then see nothing
@@ -110,87 +119,58 @@ struct Share {
   }
 };
 
-// Called by every thread of the CTA (a multiple of 32 threads); `scratch` is 36 int64 in shared memory.
-__device__ __forceinline__ Share divide(const Batch& bt, const Division& dv, int64_t* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+// Called by one whole warp.
+template <bool kOne>
+__device__ __forceinline__ Share divide(const Batch& bt, const Division& dv) {
+  const int lane = threadIdx.x & 31;
   const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
-  // length on the axis of sequence b, 0 behind the last
-  auto weigh = [&](int b, bool check) -> int64_t {
-    if (b >= dv.B) return 0;
-    const SeqUnits s = seq_units(bt, dv, b);
-    if (check) {
-      // a length that the table cannot hold, descending offsets, or a broken promise
-      const int raw = bt.lens[b], o0 = bt.q_off[b], o1 = bt.q_off[b + 1];
-      if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T ||
-          (s.n > 0 && (s.n < dv.min_n || s.n > dv.max_n)))
-        report(CEA_DEV_BAD_BATCH);
-    }
-    return s.S * dv.units_h;
-  };
-  auto scan = [&](int64_t w) -> int64_t {  // inclusive sum over the warp
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += up;
-    }
-    return w;
-  };
-  // a round of blockDim.x sequences: this thread's weight, and where its sequence starts within the round
-  int64_t w = weigh(threadIdx.x, true);
-  int64_t incl = scan(w);
-  int64_t more = 0;  // behind the first round
-  for (int b = threadIdx.x + blockDim.x; b < dv.B; b += blockDim.x) more += weigh(b, true);
-  if (dv.B > static_cast<int>(blockDim.x)) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+  int64_t mine = 0, first = 0;  // this lane's sequences; the first of them
+  for (int b = lane; b < dv.B; b += 32) {
+    const SeqUnits s = seq_units<kOne>(bt, dv, b);
+    const int64_t w = s.S * dv.units_h;
+    mine += w;
+    if (b == lane) first = w;
+    // a length that the table cannot hold, descending offsets, or a broken promise
+    const int raw = bt.lens[b], o0 = bt.q_off[b], o1 = bt.q_off[b + 1];
+    if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T || (s.n > 0 && (s.n < dv.min_n || s.n > dv.max_n)))
+      report(CEA_DEV_BAD_BATCH);
   }
-  if (lane == 31) scratch[warp] = incl + more;
-  if (threadIdx.x == 0) {
-    scratch[32] = dv.B;
-    scratch[33] = 0;
-  }
-  __syncthreads();
   Share sh;
-  sh.W = 0;
-  for (int i = 0; i < nw; ++i) sh.W += scratch[i];
+  sh.W = mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sh.W += __shfl_xor_sync(0xffffffffu, sh.W, o);
   sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W >> dv.min_share_log2)));
   sh.base = Share::div64(sh.W, sh.n);
   sh.rem = static_cast<int>(sh.W - sh.base * sh.n);
   const int c = min(static_cast<int>(blockIdx.x), sh.n);
   sh.lo = sh.start(c);
   sh.hi = sh.start(min(c + 1, sh.n));
-  // the sequence that holds lo, round by round
+  // the sequence that holds lo, 32 at a time
+  sh.b = dv.B;
+  sh.at = sh.W;
   int64_t before = 0;
-  for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += blockDim.x) {
-    if (b0 > 0) {
-      w = weigh(b0 + threadIdx.x, false);
-      incl = scan(w);
+  for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += 32) {
+    const int64_t w = b0 == 0 ? first : (b0 + lane < dv.B ? seq_units<kOne>(bt, dv, b0 + lane).S * dv.units_h : 0);
+    int64_t incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
     }
-    if (dv.B > static_cast<int>(blockDim.x)) {
-      __syncthreads();
-      if (lane == 31) scratch[warp] = incl;
-      __syncthreads();
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > sh.lo);
+    if (hit != 0u) {
+      const int l = __ffs(hit) - 1;
+      sh.b = b0 + l;
+      sh.at = before + __shfl_sync(0xffffffffu, incl - w, l);
+      break;
     }
-    int64_t round = 0;
-    for (int i = 0; i < nw; ++i) {
-      if (i == warp) incl += before + round;
-      round += scratch[i];
-    }
-    if (incl > sh.lo && incl - w <= sh.lo) {  // one thread of one round
-      scratch[32] = b0 + threadIdx.x;
-      scratch[33] = incl - w;
-    }
-    before += round;
-    if (before > sh.lo) break;
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  __syncthreads();
-  sh.b = static_cast<int>(scratch[32]);
-  sh.at = scratch[33];
   return sh;
 }
 
 // The segments (a unit and a range of its key tiles) of one CTA's share, in order.
-template <int BK>
+template <int BK, bool kOne>
 struct Segments {
   const Batch& bt;
   const Division& dv;
@@ -206,17 +186,17 @@ struct Segments {
       b = dv.B;
       return;
     }
-    s = seq_units(bt, dv, b);
+    s = seq_units<kOne>(bt, dv, b);
     int64_t r = sh.lo - base;
     hu = static_cast<int>(Share::div64(r, s.S));
     r -= hu * s.S;
     int lo = 0, hi = s.nb - 1;  // last block that starts at or before r
-    while (lo < hi) {
+    while (!kOne && lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (units_before(s, mid, dv.tb, dv.causal) <= r) lo = mid; else hi = mid - 1;
     }
     blk = lo;
-    pos = base + hu * s.S + units_before(s, blk, dv.tb, dv.causal);
+    pos = base + hu * s.S + (kOne ? 0 : units_before(s, blk, dv.tb, dv.causal));
     settle();
   }
 
@@ -229,7 +209,7 @@ struct Segments {
         b = dv.B;
         return;
       }
-      keys = unit_keys(s, blk, dv.tb, dv.causal);
+      keys = kOne ? s.len : unit_keys(s, blk, dv.tb, dv.causal);
       nt = max(1, (keys + BK - 1) / BK);
       t0 = static_cast<int>(max(int64_t(0), (sh.lo - pos + BK - 1) / BK));
       t1 = static_cast<int>(min(static_cast<int64_t>(nt), (sh.hi - pos + BK - 1) / BK));
@@ -240,14 +220,16 @@ struct Segments {
   }
 
   __device__ __forceinline__ void step() {
-    pos += max(1, unit_keys(s, blk, dv.tb, dv.causal));
-    if (++blk < s.nb) return;
-    blk = 0;
+    pos += max(1, keys);
+    if (!kOne) {
+      if (++blk < s.nb) return;
+      blk = 0;
+    }
     if (++hu < dv.units_h) return;
     hu = 0;
     do {
       if (++b >= dv.B) return;
-      s = seq_units(bt, dv, b);
+      s = seq_units<kOne>(bt, dv, b);
     } while (s.S == 0);
   }
 
@@ -262,24 +244,97 @@ struct Segments {
   }
 };
 
-// Where a segment's result goes: -1 the output itself, else a slot of the partial results.
-template <int BK>
-__device__ __forceinline__ int segment_slot(const Segments<BK>& g) {
-  if (g.t0 > 0) return 2 * blockIdx.x;
-  if (g.t1 < g.nt) return 2 * blockIdx.x + 1;
-  return -1;
-}
+// What the warps of a CTA need of a segment.
+struct alignas(16) Seg {
+  int b;         // sequence; -1: the share ends
+  int hu, blk;   // unit
+  int row0, n;   // the sequence's new tokens
+  int ctx, len;
+  int keys, t0, t1;
+  int slot;      // of the partial result; -1: the output itself
+  int it;        // running number of tile t0 in the share
+};
+static_assert(sizeof(Seg) == 48, "three 16-byte words");
 
-// The unit that goes on behind a CTA's share, gathered by a warp that walks the segments anyway.
+// The unit that goes on behind a CTA's share.
 struct Meta {
   int last;  // last CTA that holds a part of it; -1: no such unit
   int hu, blk, row0, n;
+};
 
-  template <int BK>
-  __device__ __forceinline__ void note(const Segments<BK>& g) {
-    if (g.t0 == 0 && g.t1 < g.nt) *this = Meta{g.last_cta(), g.hu, g.blk, g.s.row0, g.s.n};
+// The segments of a share pass from the one warp that walks them to the others through a short queue in shared
+// memory, so that the walk (64-bit positions) is done once and ahead of its use.
+constexpr int kQueue = 8;
+
+struct SegQueue {
+  uint8_t* seg;   // kQueue x Seg
+  uint32_t full;  // kQueue barriers, one arrival
+  uint32_t empty; // kQueue barriers, one arrival per reading warp
+  volatile int* abort;
+  int code;
+
+  static constexpr int kBytes = kQueue * sizeof(Seg);
+  static constexpr int kBars = 2 * kQueue;
+
+  __device__ __forceinline__ void init(int readers) const {
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, readers);
+    }
+  }
+  // by a whole warp
+  __device__ __forceinline__ bool put(int i, const Seg& g, int lane) const {
+    const uint32_t st = i % kQueue, n = i / kQueue;
+    if (n > 0 && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, (n - 1) & 1, abort, code))) return false;
+    if (lane != 0) return true;
+    int4* to = reinterpret_cast<int4*>(seg + st * sizeof(Seg));
+    to[0] = make_int4(g.b, g.hu, g.blk, g.row0);
+    to[1] = make_int4(g.n, g.ctx, g.len, g.keys);
+    to[2] = make_int4(g.t0, g.t1, g.slot, g.it);
+    mbar_arrive(full + 8 * st);
+    return true;
+  }
+  __device__ __forceinline__ bool read(int i, Seg& g) const {
+    const uint32_t st = i % kQueue, n = i / kQueue;
+    if (!mbar_wait(full + 8 * st, n & 1, abort, code)) return false;
+    const int4* from = reinterpret_cast<const int4*>(seg + st * sizeof(Seg));
+    const int4 x = from[0], y = from[1], z = from[2];
+    g = Seg{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+    return true;
+  }
+  // segment i, by a whole warp; false at the end of the share or after a timeout
+  __device__ __forceinline__ bool get(int i, Seg& g, int lane) const {
+    const bool ok = __all_sync(0xffffffffu, read(i, g));
+    if (ok && lane == 0) mbar_arrive(empty + 8 * (i % kQueue));
+    return ok && g.b >= 0;
+  }
+  // the same by one thread
+  __device__ __forceinline__ bool get1(int i, Seg& g) const {
+    if (!read(i, g)) return false;
+    mbar_arrive(empty + 8 * (i % kQueue));
+    return g.b >= 0;
   }
 };
+
+// Walks this CTA's share: one whole warp, which hands every segment to `take` (and a Seg with b = -1 at the end); the
+// unit that goes on behind the share is described in `meta`.
+template <int BK, bool kOne, typename Take>
+__device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool dead, Meta* meta, const Take& take) {
+  const Share sh = divide<kOne>(bt, dv);
+  Meta behind = {-1, 0, 0, 0, 0};
+  int it = 0;
+  bool ok = true;
+  if (!dead) {
+    for (Segments<BK, kOne> g(bt, dv, sh); ok && !g.done(); g.next()) {
+      const int cta = blockIdx.x, slot = g.t0 > 0 ? 2 * cta : g.t1 < g.nt ? 2 * cta + 1 : -1;
+      if (g.t0 == 0 && g.t1 < g.nt) behind = Meta{g.last_cta(), g.hu, g.blk, g.s.row0, g.s.n};
+      ok = take(Seg{g.b, g.hu, g.blk, g.s.row0, g.s.n, g.s.ctx, g.s.len, g.keys, g.t0, g.t1, slot, it});
+      it += g.t1 - g.t0;
+    }
+  }
+  if (ok) take(Seg{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
+  if ((threadIdx.x & 31) == 0) meta[blockIdx.x] = behind;
+}
 
 template <typename A>
 struct CombineArgs {
@@ -340,10 +395,10 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
   __shared__ A acc_s[WPR > 1 ? 8 : 1][WPR > 1 ? kMaxD : 1];
   __shared__ A sum_s[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (*reinterpret_cast<volatile int*>(&g_cea_status) != 0) return;  // the parts may be missing after a timeout
   const int c = blockIdx.x;
+  const int status = *reinterpret_cast<volatile int*>(&g_cea_status);
   const Meta m = a.meta[c];
-  if (m.last < 0) return;
+  if (status != 0 || m.last < 0) return;  // after a timeout parts may be missing
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.y * RPB + warp / WPR, sub = warp % WPR;
   const int tok = m.blk * a.dv.tb + row / a.dv.group, g = (m.hu % a.head_groups) * a.dv.group + row % a.dv.group;

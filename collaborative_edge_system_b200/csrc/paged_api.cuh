@@ -87,17 +87,31 @@ bool paged_tc_ok(const cea_paged_attn_params* p) {
   return true;
 }
 
-int paged_kernels(const cea_paged_attn_params* p) {
-  if (p->B == 0 || p->T == 0 || p->Hq == 0 || p->max_q_len == 0) return 0;
-  const int64_t G = p->Hq / p->Hkv;
-  // rows n * G of a sequence: up to ROWS through the decode kernel, more through the chunk kernel (measured at 32/8
-  // heads of 128: see paged_tc.cuh), each launched only if the bounds allow such a sequence
-  const bool few = std::max<int64_t>(p->min_q_len, 1) * G <= pg::dec::ROWS;
-  const bool many = p->max_q_len * G > pg::dec::ROWS;
+// Which kernels serve a call.  Sequences of up to `few` new tokens go through the decode kernel, which is compiled for 8
+// or 16 query rows per KV head; the others through the chunk kernel.  A kernel is launched only if the promised
+// numbers of new tokens allow a sequence for it.  16 rows serve a call whose sequences all fit them; where chunks come
+// too, sequences of 9 to 16 rows join those, as the 16-row form costs every single token of the batch.
+struct PagedChoice {
+  int kernels;
+  int rows;  // query rows of the decode kernel: 8 or 16
+  int few;   // tokens those hold
+};
+
+PagedChoice paged_choice(const cea_paged_attn_params* p) {
+  PagedChoice c = {0, 8, 0};
+  if (p->B == 0 || p->T == 0 || p->Hq == 0 || p->max_q_len == 0) return c;
+  const int64_t G = p->Hq / p->Hkv, most = p->max_q_len * G;
+  c.rows = most <= 8 || (most > pg::dec::ROWS && G <= 8) ? 8 : pg::dec::ROWS;
+  c.few = static_cast<int>(c.rows / G);
+  const bool few = std::max(p->min_q_len, 1) <= c.few, many = p->max_q_len > c.few;
   if ((!few || paged_decode_ok(p)) && (!many || paged_tc_ok(p)))
-    return (few ? kPagedDecode : 0) | (many ? kPagedTc : 0);
-  return kPagedSimt;
+    c.kernels = (few ? kPagedDecode : 0) | (many ? kPagedTc : 0);
+  else
+    c.kernels = kPagedSimt;
+  return c;
 }
+
+int paged_kernels(const cea_paged_attn_params* p) { return paged_choice(p).kernels; }
 
 struct PagedPlan {
   int grid, rows;       // CTAs, rows of a slot
@@ -243,7 +257,8 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, cud
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::dec::Params a;
   a.bt = paged_batch(p);
-  a.dv = pg::Division{p->B, p->Hkv, pg::dec::ROWS / G, G, pg::dec::ROWS, 0, p->min_q_len, p->max_q_len,
+  const PagedChoice choice = paged_choice(p);
+  a.dv = pg::Division{p->B, p->Hkv, choice.few, G, choice.rows, 0, p->min_q_len, p->max_q_len,
                       p->causal ? 1 : 0, 7};
   a.q = p->q;
   a.q_ss = p->q_stride[0];
@@ -266,7 +281,7 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, cud
   cudaError_t err = cudaSuccess;
 #define CEA_PDEC(DD, BF)                                                                  \
   do {                                                                                    \
-    auto k = pg::dec::decode_kernel<DD, BF>;                                              \
+    auto k = choice.rows == 8 ? pg::dec::decode_kernel<DD, BF, 1> : pg::dec::decode_kernel<DD, BF, 2>; \
     allow_smem(k, pg::dec::Layout<DD>::SMEM_ALLOC);                                       \
     err = launch_dependent(k, dim3(pl.grid), pg::dec::NTHREADS, pg::dec::Layout<DD>::SMEM_ALLOC, s, mk, mv, a); \
   } while (0)
@@ -306,7 +321,7 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStr
   pg::tc::Params a;
   a.bt = paged_batch(p);
   a.half = pg::tc::BM / G;
-  a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, pg::dec::ROWS + 1,
+  a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, int64_t(paged_choice(p).few) * G + 1,
                       p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 8};
   a.box = std::gcd(p->page_size, pg::tc::BK);
   a.out = p->out;

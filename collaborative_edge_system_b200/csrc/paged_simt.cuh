@@ -49,7 +49,6 @@ template <typename T> __device__ __forceinline__ float widen(T x, float) { retur
 template <typename T, typename A, int DMAX>
 __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ int64_t scratch[36];
   constexpr int LD = DMAX + 1;
   A* qs = reinterpret_cast<A*>(smem_raw);
   A* ks = qs + BQ * LD;
@@ -60,19 +59,17 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
   const T* vp = reinterpret_cast<const T*>(p.v);
   const int r = threadIdx.x / TPR, sub = threadIdx.x % TPR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Share sh = divide(p.bt, p.dv, scratch);
   asm volatile("griddepcontrol.launch_dependents;");
 
-  Meta meta{-1, 0, 0, 0, 0};
-  for (Segments<BK> g(p.bt, p.dv, sh); !g.done(); g.next()) {
-    meta.note(g);
+  walk<BK, false>(p.bt, p.dv, false, p.meta, [&](const Seg& g) -> bool {  // every warp alike
+    if (g.b < 0) return true;
     const int kvh = g.hu / p.head_groups, g0 = (g.hu % p.head_groups) * p.dv.group;
     const int tok = g.blk * p.dv.tb + r / p.dv.group, gg = g0 + r % p.dv.group;
-    const bool in = r < p.dv.tb * p.dv.group && tok < g.s.n && gg < p.G;
+    const bool in = r < p.dv.tb * p.dv.group && tok < g.n && gg < p.G;
     const int head = kvh * p.G + gg;
-    const int64_t row = static_cast<int64_t>(g.s.row0) + tok;
+    const int64_t row = static_cast<int64_t>(g.row0) + tok;
     // keys 0 .. limit are visible to this row
-    const int64_t limit = !in ? -1 : (p.dv.causal ? min(int64_t(g.s.ctx) + tok, int64_t(g.s.len) - 1) : g.s.len - 1);
+    const int64_t limit = !in ? -1 : (p.dv.causal ? min(int64_t(g.ctx) + tok, int64_t(g.len) - 1) : g.len - 1);
     __syncthreads();  // the previous segment's reads of qs
     if (in)
       for (int d = sub; d < p.D; d += TPR) qs[r * LD + d] = widen(q[row * p.q_ss + head * p.q_sh + d], A(0));
@@ -142,7 +139,7 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
     for (int o2 = 1; o2 < TPR; o2 <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
     const A inv = l == A(0) ? A(0) : A(1) / l;  // no visible key: zeros and -inf
     const A lse = l == A(0) ? A(-INFINITY) : m + log_of(l);
-    const int slot = segment_slot(g);
+    const int slot = g.slot;
     if (slot < 0) {
       if (in) {
         const int64_t at = row * p.o_ss + head * p.o_sh;
@@ -158,8 +155,8 @@ __global__ void __launch_bounds__(NT) attn_kernel(const Params<A> p) {
         if (sub + TPR * c < p.D) p.part_o[at * p.D + sub + TPR * c] = o[c] * inv;
       if (sub == 0) p.part_lse[at] = lse;
     }
-  }
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = meta;
+    return true;
+  });
 }
 
 }  // namespace simt

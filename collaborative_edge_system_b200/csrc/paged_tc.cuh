@@ -60,12 +60,13 @@ struct Layout {
   static constexpr int B_PFULL = B_SFULL + 2;     // x2
   static constexpr int B_PVDONE = B_PFULL + 2;    // x2
   static constexpr int B_TURN = B_PVDONE + 2;     // x2
-  static constexpr int NBAR = B_TURN + 2;
-  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int OFF_SCRATCH = OFF_MISC + 16;  // 36 int64 of the division
-  static constexpr int BYTES = OFF_SCRATCH + 36 * 8;
+  static constexpr int B_QUEUE = B_TURN + 2;
+  static constexpr int NBAR = B_QUEUE + SegQueue::kBars;
+  static constexpr int OFF_QUEUE = (OFF_BAR + NBAR * 8 + 15) / 16 * 16;
+  static constexpr int OFF_MISC = OFF_QUEUE + SegQueue::kBytes;
+  static constexpr int BYTES = OFF_MISC + 16;
   static constexpr int SMEM_ALLOC = BYTES + 1024;
-  static_assert(OFF_SCRATCH % 8 == 0 && SMEM_ALLOC <= 232448, "shared memory");
+  static_assert(SMEM_ALLOC <= 232448, "shared memory");
 };
 
 struct Params {
@@ -95,6 +96,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   auto bar = [&](int i) -> uint32_t { return sbase + L::OFF_BAR + 8 * i; };
+  const SegQueue queue{smem + L::OFF_QUEUE, bar(L::B_QUEUE), bar(L::B_QUEUE + kQueue), abort_flag,
+                       CEA_DEV_TIMEOUT_PRODUCER};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -114,6 +117,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(bar(L::B_VEMPTY + s), 2);
     }
     mbar_init(bar(L::B_VTAIL), 1);
+    queue.init(8 + 3);  // the softmax warps, the V producer and the issuers
+    *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -125,16 +130,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // after a device-side timeout nothing is computed
-  if (threadIdx.x == 0) *abort_flag = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
-  const Share sh = divide(p.bt, p.dv, reinterpret_cast<int64_t*>(smem + L::OFF_SCRATCH));
-  asm volatile("griddepcontrol.launch_dependents;");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const bool dead = *abort_flag != 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
 
   if (warp >= kKWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -148,14 +149,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int nbox = BK / p.box;
       const int box = lane % nbox, col = lane / nbox;
       const bool mine = col < L::KBOX;
-      int u = 0;
       uint32_t tails = 0;
-      bool ok = !dead;
-      Meta meta{-1, 0, 0, 0, 0};
-      for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
-        meta.note(g);
+      auto load_tiles = [&](const Seg& g) -> bool {
         const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
-        for (int t = g.t0; t < g.t1; ++t, ++u) {
+        for (int t = g.t0; t < g.t1; ++t) {
+          const int u = g.it + (t - g.t0);
           const int st = u % nst;
           const uint32_t n = u / nst;
           const int key = t * BK + box * p.box;
@@ -170,9 +168,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               page = p.bt.num_pages;  // outside the tensor map: reads as zeros
             }
           }
-          if (n > 0) ok = mbar_wait(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          bool ok = n == 0 || mbar_wait(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
+          if (!__all_sync(0xffffffffu, ok)) return false;
           const int boxes = __popc(__ballot_sync(0xffffffffu, load));
           const int left = g.keys - t * BK;
           const bool tail = !is_k && left < BK;
@@ -183,8 +180,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           if (load) tma_load_4d(to + col * L::BOX + box * p.box * 128, map, fb, col * 64, slot, g.hu, page);
           if (tail) {
             ok = mbar_wait(bar(L::B_VTAIL), tails & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu, ok)) return false;
             ++tails;
             uint8_t* tile = smem + L::OFF_V + st * L::TILE;
             for (int i = max(left, 0) * 8 + lane; i < BK * 8; i += 32)
@@ -196,9 +192,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (lane == 0) mbar_arrive(bar(b_full + st));
           }
         }
+        return true;
+      };
+      int i = 0;
+      if (is_k) {
+        // this warp also walks the share, ahead of the others; after a device-side timeout nothing is computed
+        const bool dead = *reinterpret_cast<volatile int*>(&g_cea_status) != 0;
+        walk<BK, false>(p.bt, p.dv, dead, p.meta, [&](const Seg& g) -> bool {
+          return queue.put(i++, g, lane) && (g.b < 0 || load_tiles(g));
+        });
+      } else {
+        Seg g;
+        while (queue.get(i++, g, lane))
+          if (!load_tiles(g)) break;
       }
-      if (is_k && lane == 0) p.meta[blockIdx.x] = meta;
-    } else if (lane == 0 && !dead) {
+    } else if (lane == 0) {
       // ---------------------------------------------------------- MMA issuer of half h (one thread)
       const int h = warp == kMmaWarp ? 0 : 1;
       constexpr uint32_t kIdescQK = idesc_f16(kBF16, false, BM, BK);
@@ -260,9 +268,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         pend_first = first;
         return true;
       };
-      for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+      Seg g;
+      for (int i = 0; ok && queue.get1(i, g); ++i) {
         const int tok = g.blk * p.dv.tb + h * p.half;
-        const bool act = tok < g.s.n || h == 0;
+        const bool act = tok < g.n || h == 0;
         if (act) {
           // Q_h is free once this half's last S is complete
           if (cnt > 0 && !mbar_spin(bar(L::B_SFULL + h), (cnt - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) {
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
           for (int kb = 0; kb < L::KBOX; ++kb)
             tma_load_4d(sbase + L::OFF_Q + h * L::TILE + kb * L::BOX, &tmQ, bar(L::B_QFULL + h), kb * 64,
-                        g.hu * p.dv.group, g.s.row0 + tok, 0);
+                        g.hu * p.dv.group, g.row0 + tok, 0);
           ++nq;
         }
         for (int t = g.t0; ok && t < g.t1; ++t) {
@@ -294,15 +303,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int G = p.dv.group;
     const int row_tok = row / G, row_head = row - row_tok * G;
     int it = 0;  // tiles this half computed
-    bool ok = !dead;
-    for (Segments<BK> g(p.bt, p.dv, sh); ok && !g.done(); g.next()) {
+    bool ok = true;
+    Seg g;
+    for (int i = 0; ok && queue.get(i, g, lane); ++i) {
       const int tok0 = g.blk * p.dv.tb + h * p.half;
-      if (tok0 >= g.s.n && h == 1) continue;
+      if (tok0 >= g.n && h == 1) continue;
       const int tok = tok0 + row_tok;
-      const bool row_in = row_tok < p.half && tok < g.s.n;
-      const int seen = g.s.len - 1;
-      const int limit = !row_in ? -1 : (p.dv.causal ? min(g.s.ctx + tok, seen) : seen);
-      const int first_limit = p.dv.causal ? min(g.s.ctx + tok0, seen) : seen;  // of the half's first token
+      const bool row_in = row_tok < p.half && tok < g.n;
+      const int seen = g.len - 1;
+      const int limit = !row_in ? -1 : (p.dv.causal ? min(g.ctx + tok, seen) : seen);
+      const int first_limit = p.dv.causal ? min(g.ctx + tok0, seen) : seen;  // of the half's first token
       float m = -INFINITY, l = 0.f;
       for (int t = g.t0; t < g.t1; ++t) {
         if (!warp_wait(bar(L::B_SFULL + h), it & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
@@ -393,9 +403,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_after();
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
       const float lse_row = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-      const int slot = segment_slot(g);
+      const int slot = g.slot;
       const int head = g.hu * G + row_head;
-      const int64_t trow = static_cast<int64_t>(g.s.row0) + tok;
+      const int64_t trow = static_cast<int64_t>(g.row0) + tok;
       const int64_t obase = trow * p.o_ss + head * p.o_sh;
       const int64_t prow = static_cast<int64_t>(slot) * (2 * BM) + h * p.half * G + row;
 #pragma unroll 1

@@ -5,7 +5,7 @@ import math
 import torch
 
 
-def attention(q, k_pages, v_pages, table, lens, offsets, causal=True, scale=None):
+def attention(q, k_pages, v_pages, table, lens, offsets, causal=True, scale=None, where="cpu"):
     """``(out, lse, spread, size)`` in float64 of a ragged batch, sequence by sequence; rows of no sequence are NaN.
 
     ``spread`` is ``sum_j p_ij |v_j|`` (what a relative error of the probabilities is multiplied by) and ``size`` is
@@ -14,33 +14,33 @@ def attention(q, k_pages, v_pages, table, lens, offsets, causal=True, scale=None
     H, ps = k_pages.shape[1], k_pages.shape[2]
     G = Hq // H
     scale = 1.0 / math.sqrt(D) if scale is None else scale
-    out = torch.full((T, Hq, D), math.nan, dtype=torch.float64)
-    lse = torch.full((Hq, T), math.nan, dtype=torch.float64)
-    spread, size = out.clone(), torch.zeros(Hq, T, dtype=torch.float64)
-    q, table = q.double().cpu(), table.cpu()
+    out = torch.full((T, Hq, D), math.nan, dtype=torch.float64, device=where)
+    lse = torch.full((Hq, T), math.nan, dtype=torch.float64, device=where)
+    spread, size = out.clone(), torch.zeros(Hq, T, dtype=torch.float64, device=where)
+    q, table = q.double().to(where), table.cpu()
     for b, n_all in enumerate(lens.tolist()):
         r0, r1 = int(offsets[b]), int(offsets[b + 1])
         n = r1 - r0
         if n == 0:
             continue
         pages = table[b, : -(-n_all // ps)].long()
-        k = k_pages[pages.to(k_pages.device)].double().cpu().transpose(1, 2).reshape(-1, H, D)[:n_all]
-        v = v_pages[pages.to(v_pages.device)].double().cpu().transpose(1, 2).reshape(-1, H, D)[:n_all]
+        k = k_pages[pages.to(k_pages.device)].to(where).double().transpose(1, 2).reshape(-1, H, D)[:n_all]
+        v = v_pages[pages.to(v_pages.device)].to(where).double().transpose(1, 2).reshape(-1, H, D)[:n_all]
         k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
         s = torch.einsum("ihd,jhd->hij", q[r0:r1], k) * scale
         big = torch.einsum("ihd,jhd->hij", q[r0:r1].abs(), k.abs()) * scale
         if causal:
-            at = torch.arange(n_all - n, n_all)
-            hidden = torch.arange(n_all)[None, :] > at[:, None]
+            at = torch.arange(n_all - n, n_all, device=where)
+            hidden = torch.arange(n_all, device=where)[None, :] > at[:, None]
             s = s.masked_fill(hidden, -math.inf)
             big = big.masked_fill(hidden, 0.0)
-        stat = torch.logsumexp(s, -1) if n_all else torch.full((Hq, n), -math.inf, dtype=torch.float64)
+        stat = torch.logsumexp(s, -1) if n_all else torch.full((Hq, n), -math.inf, dtype=torch.float64, device=where)
         p = torch.exp(s - stat.clamp(min=-1e300)[..., None])
         out[r0:r1] = torch.einsum("hij,jhd->ihd", p, v)
         spread[r0:r1] = torch.einsum("hij,jhd->ihd", p, v.abs())
         lse[:, r0:r1] = stat
         size[:, r0:r1] = big.amax(-1) if n_all else 0.0
-    return out, lse, spread, size
+    return out.cpu(), lse.cpu(), spread.cpu(), size.cpu()
 
 
 def check(got, got_lse, ref, *, dtype, out_dtype, single_p):

@@ -182,6 +182,23 @@ def test_long_contexts_split_over_the_gpu_and_are_deterministic():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [("bf16", 32, 8, 128, 16), ("f16", 32, 8, 64, 16),
+                                                           ("bf16", 16, 16, 128, 8), ("bf16", 16, 8, 64, 256)])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_long_shares(dtype, heads, kv_heads, dim, page, n):
+    """Hundreds of tiles for every CTA: each stage of the rings is reused many times, across many segments."""
+    lens = [30011, 700, 12345, 64, 25000, 1, 3333, 9000]
+    x = R.batch(lens, [min(n, v) for v in lens], heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=TYPES[dtype],
+                device=DEV, seed=dim + page)
+    out = torch.empty_like(x["q"])
+    lse = torch.empty(heads, x["q"].shape[0], device=DEV)
+    for _ in range(3):
+        cea.paged_attend_into(**x, out=out, lse=lse, max_q_len=n)
+    ref = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"], where=DEV)
+    R.check(out, lse, ref, dtype=TYPES[dtype], out_dtype=TYPES[dtype], single_p=bool(_kernels(x, max_q_len=n) & _lib.PAGED_TC))
+    assert _lib.device_status(clear=True) == 0
+
+
 def test_page_offsets_behind_32_bits():
     P, H, ps, D = 70000, 8, 64, 64  # 2.3e9 elements per pool
     k, v = (torch.zeros(P, H, ps, D, dtype=torch.float16, device=DEV) for _ in range(2))
