@@ -78,8 +78,7 @@ __device__ __forceinline__ int unit_keys(const SeqUnits& s, int i, int tb, bool 
 
 // kOne: every sequence served is one block of tokens (tb >= its n), whose last token sees all its keys
 template <bool kOne>
-__device__ __forceinline__ SeqUnits seq_units(const Batch& bt, const Division& dv, int b) {
-  const Seq q = load_seq(bt, b);
+__device__ __forceinline__ SeqUnits seq_units(const Division& dv, const Seq& q) {
   SeqUnits s;
   s.n = q.n;
   s.len = q.len;
@@ -105,6 +104,7 @@ struct Share {
   int n, rem;  // CTAs that take part
   int b;       // sequence at lo
   int64_t at;  // where that sequence starts
+  SeqUnits s;  // its units
 
   __device__ __forceinline__ int64_t start(int c) const { return base * c + min(c, rem); }
   // the CTA whose share holds x
@@ -124,21 +124,38 @@ template <bool kOne>
 __device__ __forceinline__ Share divide(const Batch& bt, const Division& dv) {
   const int lane = threadIdx.x & 31;
   const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
-  int64_t mine = 0, first = 0;  // this lane's sequences; the first of them
+  // 32 sequences: this lane's, its units' length together, and the end of that on an axis of the 32
+  Seq q;
+  int64_t w, end;
+  auto round = [&](int b0) {
+    const int b = b0 + lane;
+    q = Seq{0, 0, 0};
+    if (b < dv.B) q = load_seq(bt, b);
+    w = seq_units<kOne>(dv, q).S * dv.units_h;
+    end = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += up;
+    }
+  };
+  int64_t more = 0;  // behind the first 32
   for (int b = lane; b < dv.B; b += 32) {
-    const SeqUnits s = seq_units<kOne>(bt, dv, b);
-    const int64_t w = s.S * dv.units_h;
-    mine += w;
-    if (b == lane) first = w;
+    const Seq x = load_seq(bt, b);
+    if (b >= 32) more += seq_units<kOne>(dv, x).S * dv.units_h;
     // a length that the table cannot hold, descending offsets, or a broken promise
     const int raw = bt.lens[b], o0 = bt.q_off[b], o1 = bt.q_off[b + 1];
-    if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T || (s.n > 0 && (s.n < dv.min_n || s.n > dv.max_n)))
+    if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T || (x.n > 0 && (x.n < dv.min_n || x.n > dv.max_n)))
       report(CEA_DEV_BAD_BATCH);
   }
+  round(0);
   Share sh;
-  sh.W = mine;
+  sh.W = __shfl_sync(0xffffffffu, end, 31);
+  if (dv.B > 32) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sh.W += __shfl_xor_sync(0xffffffffu, sh.W, o);
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    sh.W += more;
+  }
   sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W >> dv.min_share_log2)));
   sh.base = Share::div64(sh.W, sh.n);
   sh.rem = static_cast<int>(sh.W - sh.base * sh.n);
@@ -150,23 +167,37 @@ __device__ __forceinline__ Share divide(const Batch& bt, const Division& dv) {
   sh.at = sh.W;
   int64_t before = 0;
   for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += 32) {
-    const int64_t w = b0 == 0 ? first : (b0 + lane < dv.B ? seq_units<kOne>(bt, dv, b0 + lane).S * dv.units_h : 0);
-    int64_t incl = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > sh.lo);
+    if (b0 > 0) round(b0);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + end > sh.lo);
     if (hit != 0u) {
       const int l = __ffs(hit) - 1;
       sh.b = b0 + l;
-      sh.at = before + __shfl_sync(0xffffffffu, incl - w, l);
+      sh.at = before + __shfl_sync(0xffffffffu, end - w, l);
+      sh.s = seq_units<kOne>(dv, Seq{__shfl_sync(0xffffffffu, q.row0, l), __shfl_sync(0xffffffffu, q.n, l),
+                                     __shfl_sync(0xffffffffu, q.len, l)});
       break;
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    before += __shfl_sync(0xffffffffu, end, 31);
   }
   return sh;
+}
+
+// The last block that starts at or before r on a head's part of the axis: r = n0 + m ctx + tb m (m + 1) / 2 solved for
+// m (in the form without a difference of large numbers), then put right where the float was off.
+__device__ __forceinline__ int block_at(const SeqUnits& s, int64_t r, int tb, bool causal) {
+  if (!causal) return static_cast<int>(Share::div64(r, max(1, s.len)));
+  int i;
+  if (r < s.n0) {
+    i = static_cast<int>(r);
+  } else {
+    const float a = 2.f * s.ctx + tb, x = static_cast<float>(r - s.n0);
+    const float m = s.n0 == 0 ? 4.f * x / (a + sqrtf(a * a + 8.f * tb * x)) : (sqrtf(a * a + 8.f * tb * x) - a) / (2.f * tb);
+    i = s.n0 + static_cast<int>(m);
+  }
+  i = min(max(i, 0), s.nb - 1);
+  while (i + 1 < s.nb && units_before(s, i + 1, tb, true) <= r) ++i;
+  while (i > 0 && units_before(s, i, tb, true) > r) --i;
+  return i;
 }
 
 // The segments (a unit and a range of its key tiles) of one CTA's share, in order.
@@ -177,30 +208,27 @@ struct Segments {
   const Share& sh;
   SeqUnits s;
   int b, hu, blk;       // the unit
-  int64_t base, pos;    // start of sequence b, start of the unit
+  int64_t pos;          // its start
   int keys, t0, t1, nt; // keys the unit reads; its tiles [t0, t1) of nt belong to this CTA
 
   __device__ __forceinline__ Segments(const Batch& bt_, const Division& dv_, const Share& sh_)
-      : bt(bt_), dv(dv_), sh(sh_), b(sh_.b), base(sh_.at) {
+      : bt(bt_), dv(dv_), sh(sh_), s(sh_.s), b(sh_.b) {
     if (sh.lo >= sh.hi || b >= dv.B) {
       b = dv.B;
       return;
     }
-    s = seq_units<kOne>(bt, dv, b);
-    int64_t r = sh.lo - base;
+    int64_t r = sh.lo - sh.at;
     hu = static_cast<int>(Share::div64(r, s.S));
     r -= hu * s.S;
-    int lo = 0, hi = s.nb - 1;  // last block that starts at or before r
-    while (!kOne && lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (units_before(s, mid, dv.tb, dv.causal) <= r) lo = mid; else hi = mid - 1;
-    }
-    blk = lo;
-    pos = base + hu * s.S + (kOne ? 0 : units_before(s, blk, dv.tb, dv.causal));
+    blk = kOne ? 0 : block_at(s, r, dv.tb, dv.causal);
+    pos = sh.at + hu * s.S + (kOne ? 0 : units_before(s, blk, dv.tb, dv.causal));
     settle();
   }
 
   __device__ __forceinline__ bool done() const { return b >= dv.B; }
+
+  // tiles that start before x, of those whose first one starts at 0
+  __device__ __forceinline__ static int tiles(int64_t x) { return static_cast<int>((max(x, int64_t(0)) + BK - 1) / BK); }
 
   // the current unit's tiles, or those of the next unit that has some here
   __device__ __forceinline__ void settle() {
@@ -211,8 +239,8 @@ struct Segments {
       }
       keys = kOne ? s.len : unit_keys(s, blk, dv.tb, dv.causal);
       nt = max(1, (keys + BK - 1) / BK);
-      t0 = static_cast<int>(max(int64_t(0), (sh.lo - pos + BK - 1) / BK));
-      t1 = static_cast<int>(min(static_cast<int64_t>(nt), (sh.hi - pos + BK - 1) / BK));
+      t0 = tiles(sh.lo - pos);
+      t1 = min(nt, tiles(min(sh.hi - pos, int64_t(0x7fffffff - BK))));
       if (t0 < t1) return;
       step();
       if (b >= dv.B) return;
@@ -229,7 +257,7 @@ struct Segments {
     hu = 0;
     do {
       if (++b >= dv.B) return;
-      s = seq_units<kOne>(bt, dv, b);
+      s = seq_units<kOne>(dv, load_seq(bt, b));
     } while (s.S == 0);
   }
 
@@ -478,6 +506,70 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
     }
     if (sub == 0 && lane == 0 && a.lse != nullptr) a.lse[lrow] = total == A(0) ? A(-INFINITY) : top + log_of(total);
   }
+}
+
+// The same for the chunk kernel's slots of 256 rows, laid out [slot][D / 4][row][4] so that its rows (one a thread) are
+// written, and read here, in whole lines.  Bound by L2: block (c, y) takes 32 rows, one a lane, and each of its 8 warps
+// D / 8 columns; a lane has two parts' statistics and columns in flight at a time (a unit seldom has more than three).
+// One warp a row with a lane per 4 columns took 17 us for 148 split units of 256 rows, bound by the latency of four
+// waves of blocks.
+constexpr int kWideRows = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kCombineThreads) combine_wide_kernel(const __grid_constant__ CombineArgs<float> a) {
+  constexpr int C4 = D / 32;  // float4 of a lane
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x;
+  const int status = *reinterpret_cast<volatile int*>(&g_cea_status);
+  const Meta m = a.meta[c];
+  if (status != 0 || m.last < 0) return;  // after a timeout parts may be missing
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.y * 32 + lane;
+  const int tok = m.blk * a.dv.tb + row / a.dv.group, head = m.hu * a.dv.group + row % a.dv.group;
+  if (row >= a.dv.tb * a.dv.group || tok >= m.n) return;
+  const int parts = m.last - c + 1;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc[C4];
+#pragma unroll
+  for (int j = 0; j < C4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < parts; i += 2) {
+    float lse[2];
+    float4 v[2][C4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t slot = i + k == 0 ? 2 * c + 1 : 2 * (c + min(i + k, parts - 1));
+      lse[k] = i + k < parts ? a.part_lse[slot * kWideRows + row] : -INFINITY;
+      const float4* src = reinterpret_cast<const float4*>(a.part_o) + (slot * (D / 4) + warp * C4) * kWideRows + row;
+#pragma unroll
+      for (int j = 0; j < C4; ++j) v[k][j] = src[j * kWideRows];
+    }
+    const float up = fmaxf(top, fmaxf(lse[0], lse[1])), ref = up == -INFINITY ? 0.f : up;
+    const float w = expf(top - ref), w0 = expf(lse[0] - ref), w1 = i + 1 < parts ? expf(lse[1] - ref) : 0.f;
+    top = up;
+    sum = sum * w + w0 + w1;
+#pragma unroll
+    for (int j = 0; j < C4; ++j) {
+      if (i + 1 >= parts) v[1][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      acc[j].x = acc[j].x * w + w0 * v[0][j].x + w1 * v[1][j].x;
+      acc[j].y = acc[j].y * w + w0 * v[0][j].y + w1 * v[1][j].y;
+      acc[j].z = acc[j].z * w + w0 * v[0][j].z + w1 * v[1][j].z;
+      acc[j].w = acc[j].w * w + w0 * v[0][j].w + w1 * v[1][j].w;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t trow = static_cast<int64_t>(m.row0) + tok;
+  const int64_t at = trow * a.o_ss + head * a.o_sh + warp * C4 * 4;
+#pragma unroll
+  for (int j = 0; j < C4; ++j) {
+    const float4 o = make_float4(acc[j].x * inv, acc[j].y * inv, acc[j].z * inv, acc[j].w * inv);
+    if (a.out_dtype == CEA_F32)
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at + j * 4) = o;
+    else
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at + j * 4) =
+          make_uint2(pack2(o.x, o.y, a.out_dtype == CEA_BF16), pack2(o.z, o.w, a.out_dtype == CEA_BF16));
+  }
+  if (warp == 0 && a.lse != nullptr)
+    a.lse[head * a.l_sh + trow * a.l_ss] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
 
 // ------------------------------------------------------------------ append

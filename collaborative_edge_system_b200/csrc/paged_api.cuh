@@ -170,9 +170,9 @@ cudaError_t launch_dependent(K kernel, dim3 grid, int threads, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename A, int RPB>
-int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const PagedPlan& pl, int head_groups,
-                   cudaStream_t s) {
+template <typename A>
+pg::CombineArgs<A> combine_args(const cea_paged_attn_params* p, const pg::Division& dv, const PagedPlan& pl,
+                                int head_groups) {
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::CombineArgs<A> c;
   c.dv = dv;
@@ -190,11 +190,29 @@ int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const
   c.out_dtype = p->out_dtype;
   c.heads_per_kv = p->Hq / p->Hkv;
   c.head_groups = head_groups;
-  // no unit has more rows than a sequence of the batch
-  const int rows = static_cast<int>(std::min<int64_t>(dv.tb, p->max_q_len) * dv.group);
-  const cudaError_t e = launch_dependent(pg::combine_kernel<A, RPB>, dim3(pl.grid, (rows + RPB - 1) / RPB),
-                                         pg::kCombineThreads, 0, s, c);
+  return c;
+}
+
+// rows of the largest unit: none has more than a sequence of the batch
+int unit_rows(const cea_paged_attn_params* p, const pg::Division& dv) {
+  return static_cast<int>(std::min<int64_t>(dv.tb, p->max_q_len) * dv.group);
+}
+
+template <typename A, int RPB>
+int launch_combine(const cea_paged_attn_params* p, const pg::Division& dv, const PagedPlan& pl, int head_groups,
+                   cudaStream_t s) {
+  const cudaError_t e =
+      launch_dependent(pg::combine_kernel<A, RPB>, dim3(pl.grid, (unit_rows(p, dv) + RPB - 1) / RPB),
+                       pg::kCombineThreads, 0, s, combine_args<A>(p, dv, pl, head_groups));
   return e == cudaSuccess ? CEA_OK : fail(CEA_ERR_CUDA, "combine_kernel: %s", cudaGetErrorString(e));
+}
+
+int launch_combine_wide(const cea_paged_attn_params* p, const pg::Division& dv, const PagedPlan& pl, cudaStream_t s) {
+  const cudaError_t e =
+      launch_dependent(p->D == 128 ? pg::combine_wide_kernel<128> : pg::combine_wide_kernel<64>,
+                       dim3(pl.grid, (unit_rows(p, dv) + 31) / 32), pg::kCombineThreads, 0, s,
+                       combine_args<float>(p, dv, pl, 1));
+  return e == cudaSuccess ? CEA_OK : fail(CEA_ERR_CUDA, "combine_wide_kernel: %s", cudaGetErrorString(e));
 }
 
 template <typename T, typename A, int DMAX>
@@ -349,7 +367,7 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStr
   }
 #undef CEA_PTC
   if (err != cudaSuccess) return fail(CEA_ERR_CUDA, "paged chunk_kernel: %s", cudaGetErrorString(err));
-  return launch_combine<float, 8>(p, a.dv, pl, 1, s);
+  return launch_combine_wide(p, a.dv, pl, s);
 }
 
 size_t paged_workspace(const cea_paged_attn_params* p, int kernels) {

@@ -38,6 +38,7 @@ static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kLaunchRegs * NUM_THR
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kPCol = 64;
 constexpr float kRescaleThreshold = 8.0f;
+static_assert(2 * BM == kWideRows, "rows of a slot");
 
 template <int D>
 struct Layout {
@@ -407,7 +408,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int head = g.hu * G + row_head;
       const int64_t trow = static_cast<int64_t>(g.row0) + tok;
       const int64_t obase = trow * p.o_ss + head * p.o_sh;
-      const int64_t prow = static_cast<int64_t>(slot) * (2 * BM) + h * p.half * G + row;
+      const int prow = h * p.half * G + row;  // of the slot: [D / 4][row][4]
+      float4* part = reinterpret_cast<float4*>(p.part_o) + static_cast<int64_t>(slot) * (D / 4) * kWideRows + prow;
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
@@ -417,8 +419,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         float f[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv_l;
-        if (slot >= 0 || p.out_dtype == CEA_F32) {
-          float* dst = slot >= 0 ? p.part_o + prow * D + c * 16 : reinterpret_cast<float*>(p.out) + obase + c * 16;
+        if (slot >= 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            part[(c * 4 + e) * kWideRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        } else if (p.out_dtype == CEA_F32) {
+          float* dst = reinterpret_cast<float*>(p.out) + obase + c * 16;
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
             *reinterpret_cast<float4*>(dst + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       tc_fence_before();
       if (row_in) {
-        if (slot >= 0) p.part_lse[prow] = lse_row;
+        if (slot >= 0) p.part_lse[static_cast<int64_t>(slot) * kWideRows + prow] = lse_row;
         else if (p.lse != nullptr) p.lse[head * p.l_sh + trow * p.l_ss] = lse_row;
       }
     }
