@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional, Sequence
 
@@ -772,21 +773,46 @@ def _append_chunks(B: int, n: int, toks: int):
                 yield b0, 1, s0, min(toks, n - s0)
 
 
-def _on_device(fn, p, device: torch.device, what: str) -> None:
-    """``fn(p, stream)`` on ``device``'s current stream, with ``device`` current while it launches."""
-    if device.index == torch.cuda.current_device():
-        _check(fn(ctypes.byref(p), _stream_ptr(device)), what)
-        return
-    with torch.cuda.device(device):
-        _check(fn(ctypes.byref(p), _stream_ptr(device)), what)
+# The paged operators run once per layer and token, so their calls are kept short: devices are compared by number and
+# the parameter structs filled from one packed record (the layout of the ctypes fields above).
+PAGED_ATTN_RECORD = struct.Struct("@8P13q10id3i")
+PAGED_APPEND_RECORD = struct.Struct("@7P11q8i")
 
 
-def paged_attn(p: PagedAttnParams, device: torch.device) -> None:
-    """Run cea_paged_attn on ``device``'s current stream with a fresh workspace."""
+def device_number(*tensors: torch.Tensor) -> int:
+    """The number of the CUDA device that holds all tensors; raises as :func:`require_cuda` does where none does."""
+    n = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != n:
+            n = -1
+            break
+    if n < 0:
+        require_cuda(*tensors)
+    return n
+
+
+def _on_device(fn, p, device: int, what: str) -> None:
+    """``fn(p, stream)`` on the device's current stream, with the device current while it launches."""
+    if device == torch.cuda.current_device():
+        code = fn(ctypes.byref(p), torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            code = fn(ctypes.byref(p), torch._C._cuda_getCurrentRawStream(device))
+    if code:
+        _check(code, what)
+
+
+def paged_attn(p: PagedAttnParams, like: torch.Tensor) -> None:
+    """Run cea_paged_attn on the current stream of ``like``'s device with a fresh workspace."""
     lib = _lib if _lib is not None else load()
-    need = lib.cea_paged_attn_workspace_size(ctypes.byref(p))
+    device = like.get_device()
+    if device != torch.cuda.current_device():  # the workspace's size goes by the current device
+        with torch.cuda.device(device):
+            need = lib.cea_paged_attn_workspace_size(ctypes.byref(p))
+    else:
+        need = lib.cea_paged_attn_workspace_size(ctypes.byref(p))
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = like.new_empty((need,), dtype=torch.uint8)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
     _on_device(lib.cea_paged_attn, p, device, "cea_paged_attn")
 
@@ -795,12 +821,12 @@ def paged_attn_kernels(p: PagedAttnParams) -> int:
     return load().cea_paged_attn_kernels(ctypes.byref(p))
 
 
-def paged_append(p: PagedAppendParams, device: torch.device) -> None:
+def paged_append(p: PagedAppendParams, device: int) -> None:
     lib = _lib if _lib is not None else load()
     _on_device(lib.cea_paged_append, p, device, "cea_paged_append")
 
 
-def copy_pages(p: CopyPagesParams, device: torch.device) -> None:
+def copy_pages(p: CopyPagesParams, device: int) -> None:
     lib = _lib if _lib is not None else load()
     _on_device(lib.cea_copy_pages, p, device, "cea_copy_pages")
 

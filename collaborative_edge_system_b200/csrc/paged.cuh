@@ -182,16 +182,18 @@ __device__ __forceinline__ Share divide(const Batch& bt, const Division& dv) {
   return sh;
 }
 
-// The last block that starts at or before r on a head's part of the axis: r = n0 + m ctx + tb m (m + 1) / 2 solved for
-// m (in the form without a difference of large numbers), then put right where the float was off.
+// The last block that starts at or before r on a head's part of the axis: r = n0 + (tb m^2 + a m) / 2 with
+// a = 2 (ctx + tb n0) + tb solved for m (in the form without a difference of large numbers), then put right where the
+// float was off.
 __device__ __forceinline__ int block_at(const SeqUnits& s, int64_t r, int tb, bool causal) {
   if (!causal) return static_cast<int>(Share::div64(r, max(1, s.len)));
   int i;
   if (r < s.n0) {
     i = static_cast<int>(r);
   } else {
-    const float a = 2.f * s.ctx + tb, x = static_cast<float>(r - s.n0);
-    const float m = s.n0 == 0 ? 4.f * x / (a + sqrtf(a * a + 8.f * tb * x)) : (sqrtf(a * a + 8.f * tb * x) - a) / (2.f * tb);
+    const float a = 2.f * (s.ctx + tb * s.n0) + tb, x = static_cast<float>(r - s.n0);
+    const float d = sqrtf(a * a + 8.f * tb * x);
+    const float m = a > 0.f ? 4.f * x / (a + d) : (d - a) / (2.f * tb);
     i = s.n0 + static_cast<int>(m);
   }
   i = min(max(i, 0), s.nb - 1);

@@ -2,6 +2,7 @@
 // helpers it uses.
 #pragma once
 
+#include <atomic>
 #include <numeric>
 #include <vector>
 
@@ -13,6 +14,8 @@
 namespace {
 
 namespace pg = cea::paged;
+
+int paged_sms();
 
 enum PagedKernel { kPagedTc = 1, kPagedDecode = 2, kPagedSimt = 4 };
 
@@ -134,7 +137,7 @@ int paged_simt_grid(const cea_paged_attn_params* p) {
   const size_t a = p->in_dtype == CEA_F64 ? 8 : 4;
   const int dmax = p->D <= 32 ? 32 : p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
   const size_t smem = a * (pg::simt::BQ * (dmax + 1) + 2 * pg::simt::BK * (dmax + 1) + pg::simt::BQ * (pg::simt::BK + 1));
-  return num_sms() * static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (smem + 1536))));
+  return paged_sms() * static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (smem + 1536))));
 }
 
 PagedPlan paged_simt_plan(const cea_paged_attn_params* p, size_t at) {
@@ -142,16 +145,29 @@ PagedPlan paged_simt_plan(const cea_paged_attn_params* p, size_t at) {
 }
 
 PagedPlan paged_decode_plan(const cea_paged_attn_params* p, size_t at) {
-  return paged_plan(num_sms(), pg::dec::ROWS, p->D, 4, at);
+  return paged_plan(paged_sms(), pg::dec::ROWS, p->D, 4, at);
 }
 
 PagedPlan paged_tc_plan(const cea_paged_attn_params* p, size_t at) {
-  return paged_plan(num_sms(), 2 * pg::tc::BM, p->D, 4, at);
+  return paged_plan(paged_sms(), 2 * pg::tc::BM, p->D, 4, at);
 }
 
 pg::Batch paged_batch(const cea_paged_attn_params* p) {
   return pg::Batch{p->q_offsets, p->seq_lens, p->page_table, p->table_stride, p->B, p->T, p->max_pages, p->num_pages,
                    p->page_size};
+}
+
+// SMs of the current device, asked for once per device
+int paged_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms();
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = num_sms();
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // a launch whose start may overlap the end of the kernel before it on the stream (it waits for it on the device)

@@ -30,6 +30,7 @@ outside the pool reads as zeros and is not written, a length that the table cann
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -51,21 +52,25 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
                          "[num_pages, Hkv, page_size, D] of one dtype")
-    if k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
-        raise ValueError("pages must be contiguous along the head dimension")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        if k_pages.shape[3] > 1:
+            raise ValueError("pages must be contiguous along the head dimension")
 
 
-def _check_batch(page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> None:
-    if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or q_offsets.dtype != torch.int32:
+def _check_batch(page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> Tuple[int, int]:
+    """``(B, max_pages)``"""
+    i32 = torch.int32
+    if page_table.dtype != i32 or seq_lens.dtype != i32 or q_offsets.dtype != i32:
         raise ValueError("page_table, seq_lens and q_offsets must be int32")
-    B = seq_lens.shape[0]
-    if page_table.dim() != 2 or seq_lens.dim() != 1 or q_offsets.dim() != 1 or page_table.shape[0] != B \
-            or q_offsets.shape[0] != B + 1:
-        raise ValueError(f"page_table {tuple(page_table.shape)}, seq_lens {tuple(seq_lens.shape)} and q_offsets "
-                         f"{tuple(q_offsets.shape)} must be [B, max_pages], [B] and [B + 1]")
-    if (B > 1 and seq_lens.stride(0) != 1) or (B > 0 and q_offsets.stride(0) != 1) or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError("page_table rows, seq_lens and q_offsets must be contiguous")
+    table, lens, offsets = page_table.shape, seq_lens.shape, q_offsets.shape
+    if len(table) != 2 or len(lens) != 1 or len(offsets) != 1 or table[0] != lens[0] or offsets[0] != lens[0] + 1:
+        raise ValueError(f"page_table {tuple(table)}, seq_lens {tuple(lens)} and q_offsets {tuple(offsets)} must be "
+                         "[B, max_pages], [B] and [B + 1]")
+    if seq_lens.stride(0) != 1 or q_offsets.stride(0) != 1 or page_table.stride(1) != 1:
+        if (lens[0] > 1 and seq_lens.stride(0) != 1) or (lens[0] > 0 and q_offsets.stride(0) != 1) or (
+                table[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table rows, seq_lens and q_offsets must be contiguous")
+    return lens[0], table[1]
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -74,42 +79,54 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
 
     Two tokens with one place (a page that two of the batch's sequences write) leave either's row there.
     """
-    dev = _lib.require_cuda(k, v, k_pages, v_pages, page_table, seq_lens, q_offsets)
+    dev = _lib.device_number(k, v, k_pages, v_pages, page_table, seq_lens, q_offsets)
     _check_pages(k_pages, v_pages)
-    _check_batch(page_table, seq_lens, q_offsets)
+    B, width = _check_batch(page_table, seq_lens, q_offsets)
     P, H, ps, D = k_pages.shape
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != D:
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [T, {H}, {D}]")
     if k.dtype != k_pages.dtype or v.dtype != v_pages.dtype:
         raise ValueError("k, v and the pages must share a dtype")
-    if D > 1 and (k.stride(2) != 1 or v.stride(2) != 1):
+    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    if D > 1 and (ks[2] != 1 or vs[2] != 1):
         raise ValueError("k and v must be contiguous along the head dimension")
-    T, ks, vs, kp, vp = k.shape[0], k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
-    p = _lib.PagedAppendParams(
+    _lib.paged_append(_lib.PagedAppendParams.from_buffer_copy(_lib.PAGED_APPEND_RECORD.pack(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_offsets.data_ptr(), seq_lens.data_ptr(),
-        page_table.data_ptr(), ks[:2], vs[:2], kp[:3], vp[:3], page_table.stride(0), seq_lens.shape[0], T, H, D, ps, P,
-        page_table.shape[1], k.element_size())
-    _lib.paged_append(p, dev)
+        page_table.data_ptr(), ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2],
+        page_table.stride(0), B, shape[0], H, D, ps, P, width, k.element_size())), dev)
+
+
+_TAIL = bytes(ctypes.sizeof(_lib.PagedAttnParams) - _lib.PAGED_ATTN_RECORD.size)  # the workspace's fields
 
 
 def _attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse, min_q_len, max_q_len, causal, scale):
-    T, Hq, D = q.shape
+    _check_pages(k_pages, v_pages)
+    B, width = _check_batch(page_table, seq_lens, q_offsets)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or dtype != k_pages.dtype:
+        raise ValueError(f"q must be [T, Hq, D] of the pages' dtype, got {tuple(shape)} of {dtype}")
+    T, Hq, D = shape
     P, H, ps, Dk = k_pages.shape
     if Dk != D:
-        raise ValueError(f"q {tuple(q.shape)} and the pages {tuple(k_pages.shape)} disagree on the head dim")
-    if out.shape != q.shape or (lse is not None and (lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] != T)):
-        raise ValueError(f"out must be {tuple(q.shape)} and lse [{Hq}, {T}]")
-    if D > 1 and (q.stride(2) != 1 or out.stride(2) != 1):
+        raise ValueError(f"q {tuple(shape)} and the pages {tuple(k_pages.shape)} disagree on the head dim")
+    if out.shape != shape or (lse is not None and (lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] != T)):
+        raise ValueError(f"out must be {tuple(shape)} and lse [{Hq}, {T}]")
+    qs, os, kp, vp = q.stride(), out.stride(), k_pages.stride(), v_pages.stride()
+    if D > 1 and (qs[2] != 1 or os[2] != 1):
         raise ValueError("q and out must be contiguous along the head dimension")
-    if lse is not None and lse.dtype != accumulation_dtype(q.dtype):
-        raise ValueError(f"lse must be {accumulation_dtype(q.dtype)} for {q.dtype} inputs")
-    return _lib.PagedAttnParams(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-        q_offsets.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), q.stride()[:2], k_pages.stride()[:3],
-        v_pages.stride()[:3], out.stride()[:2], (0, 0) if lse is None else lse.stride(), page_table.stride(0),
-        seq_lens.shape[0], T, Hq, H, D, ps, P, page_table.shape[1], min_q_len, T if max_q_len is None else max_q_len,
-        1.0 / math.sqrt(D) if scale is None else scale, bool(causal), _lib.dtype_code(q.dtype),
-        _lib.dtype_code(out.dtype))
+    if lse is None:
+        lp, l0, l1 = 0, 0, 0
+    else:
+        if lse.dtype != accumulation_dtype(dtype):
+            raise ValueError(f"lse must be {accumulation_dtype(dtype)} for {dtype} inputs")
+        lp, (l0, l1) = lse.data_ptr(), lse.stride()
+    return _lib.PagedAttnParams.from_buffer_copy(_lib.PAGED_ATTN_RECORD.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, q_offsets.data_ptr(),
+        seq_lens.data_ptr(), page_table.data_ptr(), qs[0], qs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], os[0], os[1],
+        l0, l1, page_table.stride(0), B, T, Hq, H, D, ps, P, width, min_q_len, T if max_q_len is None else max_q_len,
+        1.0 / math.sqrt(D) if scale is None else scale, bool(causal), _lib.dtype_code(dtype),
+        _lib.dtype_code(out.dtype)) + _TAIL)
 
 
 def paged_attend_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -123,13 +140,12 @@ def paged_attend_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     kernels and are promises (0 and ``None`` always hold): decoding sequences (at most 16 query rows per KV head) and
     chunks of prompts have a kernel each, and a batch that cannot hold one kind does not launch its kernel.
     """
-    dev = _lib.require_cuda(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse)
-    _check_pages(k_pages, v_pages)
-    _check_batch(page_table, seq_lens, q_offsets)
-    if q.dim() != 3 or q.dtype != k_pages.dtype:
-        raise ValueError(f"q must be [T, Hq, D] of the pages' dtype, got {tuple(q.shape)} of {q.dtype}")
+    if lse is None:
+        _lib.device_number(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out)
+    else:
+        _lib.device_number(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse)
     _lib.paged_attn(_attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse, min_q_len, max_q_len,
-                                 causal, scale), dev)
+                                 causal, scale), q)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -193,7 +209,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Indices, dst: 
     """Copy page ``src[i]`` to page ``dst[i]`` of both pools, ``[num_pages, Hkv, page_size, D]`` or with a leading
     layer dimension, all layers in one launch.  The indices are on the host; a destination may neither repeat nor be a
     source (``ValueError``, and nothing is copied)."""
-    dev = _lib.require_cuda(k_pages, v_pages)
+    dev = _lib.device_number(k_pages, v_pages)
     if k_pages.dim() not in (4, 5) or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
                          "[num_pages, Hkv, page_size, D] or [layers, num_pages, Hkv, page_size, D] of one dtype")

@@ -158,7 +158,7 @@ def test_operators_refuse_cpu_tensors():
 def anywhere(monkeypatch):
     """Checks that come before the kernels, on CPU tensors: what they let pass ends in ``reached``."""
     reached = []
-    monkeypatch.setattr(_lib, "require_cuda", lambda *t: CPU)
+    monkeypatch.setattr(_lib, "device_number", lambda *t: 0)
     for name in ("paged_attn", "paged_append", "copy_pages"):
         monkeypatch.setattr(_lib, name, lambda p, dev: reached.append(p))
     return reached
@@ -224,6 +224,22 @@ def test_copy_arguments(anywhere):
 
 
 # ------------------------------------------------------------------------------------------------ C ABI
+def test_records_have_the_layout_of_the_structs():
+    for record, cls in ((_lib.PAGED_ATTN_RECORD, _lib.PagedAttnParams), (_lib.PAGED_APPEND_RECORD, _lib.PagedAppendParams)):
+        flat, p = [], cls()
+        for name, kind in cls._fields_[:-2] if cls is _lib.PagedAttnParams else cls._fields_:
+            if hasattr(kind, "_length_"):
+                values = [len(flat) + 1 + i for i in range(kind._length_)]
+                setattr(p, name, tuple(values))
+            else:
+                values = [float(len(flat) + 1) if kind is ctypes.c_double else len(flat) + 1]
+                setattr(p, name, values[0])
+            flat += values
+        packed = record.pack(*flat)
+        assert bytes(p)[: len(packed)] == packed and ctypes.sizeof(cls) - len(packed) in (0, 16, 20)
+        assert not any(bytes(p)[len(packed):])
+
+
 FAKE = 1 << 20  # never dereferenced: every check here returns before any CUDA call
 
 
