@@ -12,7 +12,9 @@ sequence-parallel (SP) prefill and greedy decode go through, for one pipeline st
   tensor expressions do;
 * attention is :func:`ring_attention` / :func:`ulysses_attention` for prefill and
   :func:`ring_decode_attention` (ring) or per-head-shard attention + :func:`gather_heads` (Ulysses) for decode,
-  with K/V kept in :class:`KVCache`.
+  with K/V kept in :class:`KVCache`;
+* :meth:`LlamaModel.forward_paged` and :func:`generate_paged` serve ragged batches (pieces of prompts and decoding
+  sequences together, prompts with a common prefix) over a :class:`PagedKVCache`.
 
 :func:`forward_logits` and :func:`generate_greedy` follow ``CollabEngine.forward`` / ``generate`` for this
 configuration (``engine.py:301-347, 349-506``): left-padded prompts, positions from the attention mask (``-1`` on
@@ -34,6 +36,7 @@ from . import _lib
 from .attention import attention, gqa_group
 from .cache import KVCache, assign_tokens, ring_decode_attention
 from .comm import Communicator
+from .paged import PagedBatch, PagedKVCache
 from .partition import HeadShard, SequenceLayout, offsets_of, partition_heads, split_sizes
 from .sequence_parallel import gather_heads, gather_sequence, ring_attention, ulysses_attention
 
@@ -419,6 +422,27 @@ class LlamaModel:
 
         return self._layers(ids, self._attn_block(attend, positions))
 
+    def paged_cache(self, num_pages: int, page_size: int = 16) -> PagedKVCache:
+        """A paged KV cache for this model stage (its TP shard's KV heads), ``num_pages`` pages per layer."""
+        return PagedKVCache(self.config.num_layers, num_pages, page_size, self.shard.heads.kv_count,
+                            self.config.head_dim, dtype=self.dtype, device=self.device)
+
+    def forward_paged(self, ids: torch.Tensor, batch: PagedBatch, cache: PagedKVCache) -> torch.Tensor:
+        """Final hidden states ``[T, h]`` of a ragged batch of new tokens (``ids`` ``[T]``, in the order of ``batch``,
+        which :meth:`PagedKVCache.extend` made): their keys and values go into the cache's pages, and each token attends
+        to its sequence up to itself.  Pieces of prompts and decoding sequences may share a pass."""
+        if self.kv_map is not None:
+            raise ValueError("the paged cache needs query heads grouped evenly over this rank's KV heads")
+        if ids.dim() != 1 or ids.shape[0] != batch.num_tokens:
+            raise ValueError(f"ids {tuple(ids.shape)} for a batch of {batch.num_tokens} new tokens")
+        positions = batch.positions.view(1, -1)
+
+        def attend(idx, q, k, v):
+            cache.append(idx, k[0], v[0], batch)
+            return cache.attend(idx, q[0], batch).unsqueeze(0)
+
+        return self._layers(ids.view(1, -1), self._attn_block(attend, positions))[0]
+
     def _decode_sp_split(self, ids, positions, comm, cache, owner, sp_mode, head_shards, stage, sp_weights):
         d, me = self.config.head_dim, self.shard.heads
         parts = list(sp_weights) if sp_weights else comm.size
@@ -616,5 +640,102 @@ def generate_greedy(model: LlamaModel, prompts: Sequence[Sequence[int]], max_new
     return out, [stacked[b, : len(out[b])] for b in range(n)]
 
 
-__all__ = ["LayerWeights", "LlamaConfig", "LlamaModel", "TPShard", "forward_logits", "generate_greedy", "mask_positions",
-           "padded_batch"]
+def generate_paged(model: LlamaModel, prompts: Sequence[Sequence[int]], max_new_tokens: int, *,
+                   prefix: Sequence[int] = (), cache: Optional[PagedKVCache] = None, page_size: int = 16,
+                   chunk_tokens: int = 2048, return_scores: bool = False, eos_token_id: Optional[int] = None):
+    """Greedy generation over a paged KV cache: the results of :func:`generate_greedy` on ``prefix + prompt`` for each
+    prompt, without padding and with the prefix computed and kept once.
+
+    Every pass takes up to ``chunk_tokens`` new tokens: one of each decoding sequence, then pieces of the prompts that are
+    not through yet, in their order; a prompt's sequence is forked from the prefix's (its full pages are shared).  A
+    sequence ends with ``eos_token_id`` or after ``max_new_tokens``, and its pages become free.  With ``cache`` the
+    pages come from it (:class:`OutOfPages` if they do not suffice; the sequences made here are gone when the call
+    returns or raises).  Returns as :func:`generate_greedy` does."""
+    n = len(prompts)
+    if max_new_tokens <= 0:
+        return ([[] for _ in range(n)], [None] * n) if return_scores else [[] for _ in range(n)]
+    prefix, prompts = list(prefix), [list(p) for p in prompts]
+    if any(not prefix and not p for p in prompts):
+        raise ValueError("a sequence needs at least one token")
+    if chunk_tokens < 1:
+        raise ValueError("chunk_tokens must be >= 1")
+    dev = model.device
+    if cache is None:
+        def pages(tokens: int) -> int:
+            return -(-tokens // page_size)
+
+        # a fork has its own copy of a partly filled last page of the prefix
+        own = [pages(len(prefix) + len(p) + max_new_tokens - 1) - len(prefix) // page_size for p in prompts]
+        cache = model.paged_cache(pages(len(prefix)) + sum(own), page_size)
+    tokens: List[List[torch.Tensor]] = [[] for _ in range(n)]
+    scores: List[List[torch.Tensor]] = [[] for _ in range(n)]
+    live: Dict[int, int] = {}  # prompt -> its sequence in the cache
+    root: Optional[int] = None
+
+    def run(parts: List[Tuple[int, torch.Tensor]]) -> Tuple[torch.Tensor, PagedBatch]:
+        batch = cache.extend([s for s, _ in parts], [t.shape[0] for _, t in parts])
+        return model.forward_paged(torch.cat([t for _, t in parts]), batch, cache), batch
+
+    try:
+        last_of_prefix = None
+        if prefix:
+            root = cache.add()
+            ids = torch.tensor(prefix, dtype=torch.long, device=dev)
+            for part in ids.split(chunk_tokens):
+                hidden, _ = run([(root, part)])
+            last_of_prefix = hidden[-1]
+        todo = {i: torch.tensor(p, dtype=torch.long, device=dev) for i, p in enumerate(prompts)}
+        for i in range(n):
+            live[i] = cache.fork(root)[0] if root is not None else cache.add()
+        decoding: Dict[int, torch.Tensor] = {}  # prompt -> its newest token, on the device
+
+        def choose(which: List[int], hidden: torch.Tensor) -> None:
+            logits = model.logits(hidden)
+            chosen = logits.argmax(dim=-1)
+            ends = (chosen == eos_token_id).tolist() if eos_token_id is not None else [False] * len(which)
+            for row, i in enumerate(which):
+                tokens[i].append(chosen[row : row + 1])
+                scores[i].append(logits[row])
+                if ends[row] or len(tokens[i]) == max_new_tokens:
+                    decoding.pop(i, None)
+                    cache.free(live.pop(i))
+                else:
+                    decoding[i] = chosen[row : row + 1]
+
+        whole = [i for i in range(n) if not prompts[i]]  # prompts that are the prefix
+        if whole:
+            choose(whole, last_of_prefix.expand(len(whole), -1).contiguous())
+            for i in whole:
+                del todo[i]
+        while live:
+            parts = [(i, t) for i, t in decoding.items()][:chunk_tokens]
+            room = chunk_tokens - len(parts)
+            for i, rest in list(todo.items()):
+                if room == 0:
+                    break
+                piece, after = rest[:room], rest[room:]
+                room -= piece.shape[0]
+                parts.append((i, piece))
+                if after.shape[0]:
+                    todo[i] = after
+                else:
+                    del todo[i]
+            hidden, batch = run([(live[i], t) for i, t in parts])
+            through = [b for b, (i, _) in enumerate(parts) if i not in todo]
+            if len(through) > 0:
+                # sequences that decoded go behind the others next time, in case not all fit a pass
+                for b in through:
+                    decoding.pop(parts[b][0], None)
+                rows = torch.tensor([batch.last_rows[b] for b in through], device=dev)
+                choose([parts[b][0] for b in through], hidden[rows])
+    finally:
+        for s in [root] * (root is not None) + list(live.values()):
+            cache.free(s)
+    out = [torch.cat(t).tolist() for t in tokens]
+    if not return_scores:
+        return out
+    return out, [torch.stack(s) for s in scores]
+
+
+__all__ = ["LayerWeights", "LlamaConfig", "LlamaModel", "TPShard", "forward_logits", "generate_greedy", "generate_paged",
+           "mask_positions", "padded_batch"]

@@ -178,6 +178,8 @@ def paged_attention_with_lse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: to
 
 def _host_indices(x: Indices) -> torch.Tensor:
     if isinstance(x, torch.Tensor):
+        if x.dtype == torch.int32 and x.is_contiguous() and x.dim() == 1 and x.device.type == "cpu":
+            return x
         if x.device.type != "cpu" or x.dim() != 1:
             raise ValueError("page indices are a sequence of numbers or a 1-D tensor on the CPU")
         if x.dtype not in (torch.int32, torch.int64):
@@ -194,6 +196,8 @@ def _host_indices(x: Indices) -> torch.Tensor:
 def _page_block(pages: torch.Tensor) -> Tuple[int, int, int]:
     """``(layer stride, page stride, page elements)`` of ``[L, P, H, ps, D]`` pages, each of which must be one block
     of memory (in any order of its dimensions)."""
+    if pages.is_contiguous():
+        return pages.stride(0), pages.stride(1), pages.stride(1)
     n = 1
     for size, stride in sorted(zip(pages.shape[2:], pages.stride()[2:]), key=lambda x: x[1]):
         if size > 1:

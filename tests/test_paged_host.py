@@ -320,3 +320,74 @@ def test_append_and_copy_checks_of_the_c_abi():
     for src, dst in (([0], [6]), ([6], [0]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 2], [2, 3]), ([1], [1])):
         assert copy(src, dst) == _lib.CEA_ERR_INVALID, (src, dst)
     assert copy([0], [1], n=-1) == _lib.CEA_ERR_INVALID
+
+
+# ------------------------------------------------------------------------------------------------ generation
+class SumModel:
+    """Stands for a model: the next token is the sum of the sequence's tokens (read from the cache) modulo 17."""
+
+    device = CPU
+
+    def __init__(self):
+        self.passes = []
+
+    def paged_cache(self, num_pages, page_size):
+        self.cache = HostCache(1, num_pages, page_size, 1, 1)
+        return self.cache
+
+    def forward_paged(self, ids, batch, cache):
+        self.passes.append(batch.num_tokens)
+        out, ps = [], cache.page_size
+        for b in range(len(batch.seq_lens)):
+            n, r0, r1 = int(batch.seq_lens[b]), int(batch.q_offsets[b]), int(batch.q_offsets[b + 1])
+            at = lambda p: (0, int(batch.page_table[b, p // ps]), 0, p % ps, 0)  # noqa: E731
+            for i in range(r0, r1):
+                assert int(batch.positions[i]) == n - r1 + i
+                cache.k[at(n - r1 + i)] = float(ids[i])
+                out.append(sum(float(cache.k[at(p)]) for p in range(n - r1 + i + 1)))
+        return torch.tensor(out).view(-1, 1)
+
+    def logits(self, hidden):
+        return torch.nn.functional.one_hot(hidden[:, 0].long() % 17, 17).float()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_generation_schedules_every_token_once(seed):
+    from collaborative_edge_system_b200.llama import generate_paged
+
+    rnd = random.Random(seed)
+    prefix = [rnd.randrange(17) for _ in range(rnd.choice([0, 0, 3, 8, 11]))]
+    prompts = [[rnd.randrange(17) for _ in range(rnd.randint(0 if prefix else 1, 12))] for _ in range(rnd.randint(1, 7))]
+    most, eos, chunk = rnd.randint(1, 9), rnd.choice([None, 3, 5]), rnd.choice([1, 2, 5, 64])
+    want = []
+    for p in prompts:
+        seq, new = prefix + p, []
+        while len(new) < most and (not new or new[-1] != eos):
+            new.append(sum(seq) % 17)
+            seq = seq + new[-1:]
+        want.append(new)
+    model = SumModel()
+    got, scores = generate_paged(model, prompts, most, prefix=prefix, page_size=4, chunk_tokens=chunk, eos_token_id=eos,
+                                 return_scores=True)
+    assert got == want and [s.argmax(-1).tolist() for s in scores] == want
+    assert max(model.passes) <= chunk
+    assert sum(model.passes) == len(prefix) + sum(len(p) + len(w) - 1 for p, w in zip(prompts, want))
+    assert model.cache.num_free_pages == len(model.cache.pool.refs)
+
+
+def test_generation_refusals_leave_the_cache_as_it_was():
+    from collaborative_edge_system_b200.llama import generate_paged
+
+    model = SumModel()
+    cache = model.paged_cache(4, 4)
+    mine = cache.add()
+    cache.extend([mine], [5])
+    with pytest.raises(ValueError):
+        generate_paged(model, [[1], []], 2)
+    with pytest.raises(ValueError):
+        generate_paged(model, [[1]], 2, chunk_tokens=0)
+    with pytest.raises(cea.OutOfPages):
+        generate_paged(model, [[1] * 6, [2] * 3], 2, cache=cache)
+    assert cache.num_free_pages == 2 and cache.length(mine) == 5
+    assert generate_paged(model, [[1, 2]], 0) == [[]]
+    assert generate_paged(model, [[1, 2]], 3, cache=cache) == [[3, 6, 12]] and cache.num_free_pages == 2
