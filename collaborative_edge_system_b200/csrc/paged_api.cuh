@@ -133,11 +133,18 @@ PagedPlan paged_plan(int grid, int rows, int D, size_t elem, size_t at) {
 }
 
 // CTAs of the CUDA-core kernel: as many as fit the shared memory of an SM, at most 8
+template <typename A, int DMAX>
+int paged_simt_per_sm() {
+  return static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (pg::simt::Layout<A, DMAX>::BYTES + 1024))));
+}
+
 int paged_simt_grid(const cea_paged_attn_params* p) {
-  const size_t a = p->in_dtype == CEA_F64 ? 8 : 4;
-  const int dmax = p->D <= 32 ? 32 : p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
-  const size_t smem = a * (pg::simt::BQ * (dmax + 1) + 2 * pg::simt::BK * (dmax + 1) + pg::simt::BQ * (pg::simt::BK + 1));
-  return paged_sms() * static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (smem + 1536))));
+  const bool d = p->in_dtype == CEA_F64;
+  const int n = p->D <= 32    ? (d ? paged_simt_per_sm<double, 32>() : paged_simt_per_sm<float, 32>())
+                : p->D <= 64  ? (d ? paged_simt_per_sm<double, 64>() : paged_simt_per_sm<float, 64>())
+                : p->D <= 128 ? (d ? paged_simt_per_sm<double, 128>() : paged_simt_per_sm<float, 128>())
+                              : (d ? paged_simt_per_sm<double, 256>() : paged_simt_per_sm<float, 256>());
+  return paged_sms() * n;
 }
 
 PagedPlan paged_simt_plan(const cea_paged_attn_params* p, size_t at) {
@@ -266,7 +273,11 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   a.out_dtype = p->out_dtype;
   a.scale = p->scale;
   auto k = pg::simt::attn_kernel<T, A, DMAX>;
-  constexpr size_t bytes = pg::simt::smem_bytes<A, DMAX>();
+  constexpr size_t bytes = pg::simt::Layout<A, DMAX>::BYTES;
+  const int size = elem_bytes(p->in_dtype);
+  bool vec = aligned16(p->k_pages) && aligned16(p->v_pages) && p->D * size % 16 == 0;
+  for (int i = 0; i < 3; ++i) vec = vec && p->k_stride[i] * size % 16 == 0 && p->v_stride[i] * size % 16 == 0;
+  a.vec = vec;
   allow_smem(k, static_cast<int>(bytes));
   if (const cudaError_t e = launch_dependent(k, dim3(pl.grid), pg::simt::NT, bytes, s, a))
     return fail(CEA_ERR_CUDA, "paged attn_kernel: %s", cudaGetErrorString(e));
