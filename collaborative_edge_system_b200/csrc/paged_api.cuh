@@ -132,10 +132,11 @@ PagedPlan paged_plan(int grid, int rows, int D, size_t elem, size_t at) {
   return pl;
 }
 
-// CTAs of the CUDA-core kernel: as many as fit the shared memory of an SM, at most 8
+// CTAs of the CUDA-core kernel: as many as fit an SM's shared memory and registers (at 128 a thread); one more per SM
+// is a second wave (59 us instead of 33 us at the size of paged_simt.cuh)
 template <typename A, int DMAX>
 int paged_simt_per_sm() {
-  return static_cast<int>(std::max<size_t>(1, std::min<size_t>(8, 227 * 1024 / (pg::simt::Layout<A, DMAX>::BYTES + 1024))));
+  return static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, 227 * 1024 / (pg::simt::Layout<A, DMAX>::BYTES + 1024))));
 }
 
 int paged_simt_grid(const cea_paged_attn_params* p) {

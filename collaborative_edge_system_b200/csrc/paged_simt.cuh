@@ -74,7 +74,7 @@ __device__ __forceinline__ void cp16(const void* dst, const void* src) {
 }
 
 template <typename T, typename A, int DMAX>
-__global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params<A> p) {
+__global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn_kernel(const __grid_constant__ Params<A> p) {
   using L = Layout<A, DMAX>;
   constexpr int VN = L::VN, NC = DMAX / (VN * TPR);  // output words of a thread
   extern __shared__ __align__(16) uint8_t smem_raw[];
