@@ -133,7 +133,7 @@ PagedPlan paged_plan(int grid, int rows, int D, size_t elem, size_t at) {
 }
 
 // CTAs of the CUDA-core kernel: as many as fit an SM's shared memory and registers (at 128 a thread); one more per SM
-// is a second wave (59 us instead of 33 us at the size of paged_simt.cuh)
+// is a second wave (59 us instead of 44 us at the size in paged_simt.cuh)
 template <typename A, int DMAX>
 int paged_simt_per_sm() {
   return static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, 227 * 1024 / (pg::simt::Layout<A, DMAX>::BYTES + 1024))));
@@ -247,7 +247,7 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   pg::simt::Params<A> a;
   a.bt = paged_batch(p);
   a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, p->min_q_len, p->max_q_len, p->causal ? 1 : 0,
-                      5};
+                      pg::simt::Layout<A, DMAX>::BK == 64 ? 6 : 5};
   a.q = p->q;
   a.k = p->k_pages;
   a.v = p->v_pages;

@@ -2,15 +2,16 @@
 // alignment the tensor-core kernels do not take.  Right for every case; the arithmetic is the accumulation type's
 // throughout (probabilities are not rounded).
 //
-// A unit is up to 16 query rows (tokens x query heads of one KV head) against the keys of one sequence, in tiles of
-// 32 keys.  8 threads share a row: thread `sub` holds the scores of keys sub + 8 j and groups of 16-byte output
-// columns sub + 8 c, so K, V and Q are read from shared memory in 16-byte words without conflicts (rows are padded by
-// 16 bytes) and each word feeds 4 to 16 multiply-adds.  Online softmax: m' = max(m, max s),
+// A unit is up to 16 query rows (tokens x query heads of one KV head) against the keys of one sequence, in tiles of 64
+// keys (32 where a row is longer than 256 bytes).  16 threads share two rows, r and r + 8: thread `sub` holds the scores
+// of keys sub + 16 j and groups of 16-byte output columns sub + 16 c of both, so every 16-byte word of K and V that it
+// reads from shared memory feeds two rows (one row a thread was bound by those reads: 44 us at the size below).  Rows
+// are padded by 16 bytes, which keeps the reads free of conflicts.  Online softmax: m' = max(m, max s),
 // l' = l e^(m - m') + sum e^(s - m'), o' = o e^(m - m') + sum e^(s - m') v.
-// 4 threads fetch a key's K and V rows (one page lookup per tile and thread): by cp.async a tile ahead where the rows
-// are aligned and need no conversion, else element by element.  The division of the work over the grid is paged.cuh's;
-// several CTAs per SM hide one another's latencies.  Fetching element by element into one buffer, with scalar reads,
-// took 97 us where this takes the time in the table of the measurements (fp32, 4 sequences of up to 2048, 40 new tokens).
+// Several threads fetch a key's K and V rows (one page lookup per tile and thread): by cp.async a tile ahead where the
+// rows are aligned and need no conversion, else element by element.  The division of the work over the grid is
+// paged.cuh's; several CTAs per SM hide one another's latencies.  Fetching element by element into one buffer, with
+// scalar reads, took 97 us (fp32, 8 heads of 64, 4 sequences of up to 2048, up to 40 new tokens).
 #pragma once
 
 #include "paged.cuh"
@@ -19,7 +20,7 @@ namespace cea {
 namespace paged {
 namespace simt {
 
-constexpr int BQ = 16, BK = 32, TPR = 8, NT = BQ * TPR;
+constexpr int BQ = 16, TPR = 16, NT = BQ / 2 * TPR;
 
 template <typename A>
 struct Params {
@@ -45,6 +46,7 @@ struct Params {
 
 template <typename A, int DMAX>
 struct Layout {
+  static constexpr int BK = sizeof(A) * DMAX <= 256 ? 64 : 32;
   static constexpr int VN = 16 / sizeof(A);        // elements of a 16-byte word
   static constexpr int LD = DMAX + VN;             // of a row in shared memory
   static constexpr int NST = sizeof(A) * DMAX > 1024 ? 1 : 2;  // fp64 rows of 256: one stage is 133 KB
@@ -74,9 +76,11 @@ __device__ __forceinline__ void cp16(const void* dst, const void* src) {
 }
 
 template <typename T, typename A, int DMAX>
-__global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn_kernel(const __grid_constant__ Params<A> p) {
+__global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params<A> p) {
   using L = Layout<A, DMAX>;
-  constexpr int VN = L::VN, NC = DMAX / (VN * TPR);  // output words of a thread
+  constexpr int BK = L::BK, VN = L::VN, KPT = BK / TPR;
+  constexpr int NC = (DMAX + VN * TPR - 1) / (VN * TPR);  // output words of a thread and row
+  constexpr int FPK = NT / BK;                            // threads that fetch a key
   extern __shared__ __align__(16) uint8_t smem_raw[];
   A* qs = reinterpret_cast<A*>(smem_raw);
   A* kv = qs + BQ * L::LD;  // stages of K, then V
@@ -84,7 +88,7 @@ __global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn
   const T* q = reinterpret_cast<const T*>(p.q);
   const T* kp = reinterpret_cast<const T*>(p.k);
   const T* vp = reinterpret_cast<const T*>(p.v);
-  const int r = threadIdx.x / TPR, sub = threadIdx.x % TPR;
+  const int r0 = threadIdx.x / TPR, sub = threadIdx.x % TPR;  // rows r0 and r0 + 8
   const int words = (p.D + VN - 1) / VN;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -95,17 +99,21 @@ __global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn
   walk<BK, false>(p.bt, p.dv, false, p.meta, [&](const Seg& g) -> bool {  // every warp alike
     if (g.b < 0) return true;
     const int kvh = g.hu / p.head_groups, g0 = (g.hu % p.head_groups) * p.dv.group;
-    const int tok = g.blk * p.dv.tb + r / p.dv.group, gg = g0 + r % p.dv.group;
-    const bool in = r < p.dv.tb * p.dv.group && tok < g.n && gg < p.G;
-    const bool busy = __any_sync(0xffffffffu, in);  // some row of the warp exists
-    const int head = kvh * p.G + gg;
-    const int64_t row = static_cast<int64_t>(g.row0) + tok;
-    // keys 0 .. limit are visible to this row
-    const int limit = !in ? -1 : (p.dv.causal ? min(g.ctx + tok, g.len - 1) : g.len - 1);
-    // keys of tile t into stage `st`; a key behind the unit's last keeps what is there (its score is masked, its V row
-    // zeroed)
+    int64_t row[2];
+    int head[2], limit[2];  // keys 0 .. limit are visible to the row
+    bool in[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + 8 * h, tok = g.blk * p.dv.tb + r / p.dv.group, gg = g0 + r % p.dv.group;
+      in[h] = r < p.dv.tb * p.dv.group && tok < g.n && gg < p.G;
+      head[h] = kvh * p.G + gg;
+      row[h] = static_cast<int64_t>(g.row0) + tok;
+      limit[h] = !in[h] ? -1 : (p.dv.causal ? min(g.ctx + tok, g.len - 1) : g.len - 1);
+    }
+    const bool busy = __any_sync(0xffffffffu, in[0] || in[1]);  // some row of the warp exists
+    // keys of tile t into stage `st`; those behind the unit's last are zeros (their scores are masked)
     auto fetch = [&](int t, int st) {
-      const int j = threadIdx.x >> 2, part = threadIdx.x & 3, key = t * BK + j;
+      const int j = threadIdx.x / FPK, part = threadIdx.x % FPK, key = t * BK + j;
       A* ks = kv + st * 2 * BK * L::LD + j * L::LD;
       A* vs = ks + BK * L::LD;
       int page = -1, slot = 0;
@@ -119,35 +127,43 @@ __global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn
         }
       }
       if (page < 0) {
-        for (int d = part; d < p.D; d += 4) ks[d] = vs[d] = 0;
+        for (int d = part; d < p.D; d += FPK) ks[d] = vs[d] = 0;
         return;
       }
       const T* ksrc = kp + page * p.k_sp + kvh * p.k_sh + slot * p.k_ss;
       const T* vsrc = vp + page * p.v_sp + kvh * p.v_sh + slot * p.v_ss;
       if (sizeof(T) == sizeof(A) && p.vec) {
-        for (int w = part; w < words; w += 4) {
+        for (int w = part; w < words; w += FPK) {
           cp16(ks + w * VN, ksrc + w * VN);
           cp16(vs + w * VN, vsrc + w * VN);
         }
       } else {
-        for (int d = part; d < p.D; d += 4) {
+        for (int d = part; d < p.D; d += FPK) {
           ks[d] = widen(ksrc[d], A(0));
           vs[d] = widen(vsrc[d], A(0));
         }
       }
     };
     __syncthreads();  // the previous segment's reads of qs and of the stages
-    if (in)
-      for (int d = sub; d < p.D; d += TPR) qs[r * L::LD + d] = widen(q[row * p.q_ss + head * p.q_sh + d], A(0));
     if (L::NST == 2) {
       fetch(g.t0, g.t0 & 1);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    A m = -INFINITY, l = 0, o[NC][VN];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int h = 0; h < 2; ++h)
+      if (in[h])
+        for (int d = sub; d < p.D; d += TPR)
+          qs[(r0 + 8 * h) * L::LD + d] = widen(q[row[h] * p.q_ss + head[h] * p.q_sh + d], A(0));
+    A m[2], l[2], o[2][NC][VN];
 #pragma unroll
-      for (int e = 0; e < VN; ++e) o[c][e] = 0;
+    for (int h = 0; h < 2; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) o[h][c][e] = 0;
+    }
     for (int t = g.t0; t < g.t1; ++t) {
       const int st = L::NST == 2 ? t & 1 : 0;
       if (L::NST == 1) {
@@ -163,75 +179,89 @@ __global__ void __launch_bounds__(NT, sizeof(A) == 4 && DMAX <= 64 ? 4 : 1) attn
       if (!busy) continue;
       const A* ks = kv + st * 2 * BK * L::LD;
       const A* vs = ks + BK * L::LD;
-      A s[BK / TPR], top = -INFINITY;
+      A s[2][KPT];
 #pragma unroll
-      for (int j = 0; j < BK / TPR; ++j) s[j] = 0;
+      for (int j = 0; j < KPT; ++j) s[0][j] = s[1][j] = 0;
 #pragma unroll 2
       for (int w = 0; w < words; ++w) {
-        const Word<A> x = word(qs + r * L::LD + w * VN);
+        const Word<A> x0 = word(qs + r0 * L::LD + w * VN), x1 = word(qs + (r0 + 8) * L::LD + w * VN);
 #pragma unroll
-        for (int j = 0; j < BK / TPR; ++j) {
+        for (int j = 0; j < KPT; ++j) {
           const Word<A> y = word(ks + (sub + TPR * j) * L::LD + w * VN);
 #pragma unroll
-          for (int e = 0; e < VN; ++e) s[j] += x[e] * y[e];
+          for (int e = 0; e < VN; ++e) {
+            s[0][j] += x0[e] * y[e];
+            s[1][j] += x1[e] * y[e];
+          }
         }
       }
 #pragma unroll
-      for (int j = 0; j < BK / TPR; ++j) {
-        // a key behind the row's view does not count, whatever its product is
-        s[j] = t * BK + sub + TPR * j <= limit ? s[j] * static_cast<A>(p.scale) : A(-INFINITY);
-        top = max(top, s[j]);
+      for (int h = 0; h < 2; ++h) {
+        A top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          // a key behind the row's view does not count, whatever its product is
+          s[h][j] = t * BK + sub + TPR * j <= limit[h] ? s[h][j] * static_cast<A>(p.scale) : A(-INFINITY);
+          top = max(top, s[h][j]);
+        }
+#pragma unroll
+        for (int x = 1; x < TPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const A m_new = max(m[h], top), ref = m_new == A(-INFINITY) ? A(0) : m_new;
+        const A alpha = exp_of(m[h] - ref);
+        A add = 0;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          const A e = exp_of(s[h][j] - ref);
+          add += e;
+          ps[(r0 + 8 * h) * L::LP + sub + TPR * j] = e;
+        }
+        m[h] = m_new;
+        l[h] = l[h] * alpha + add;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) o[h][c][e] *= alpha;
       }
-#pragma unroll
-      for (int x = 1; x < TPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const A m_new = max(m, top), ref = m_new == A(-INFINITY) ? A(0) : m_new;
-      const A alpha = exp_of(m - ref);
-      A add = 0;
-#pragma unroll
-      for (int j = 0; j < BK / TPR; ++j) {
-        const A e = exp_of(s[j] - ref);
-        add += e;
-        ps[r * L::LP + sub + TPR * j] = e;
-      }
-      m = m_new;
-      l = l * alpha + add;
-      __syncwarp();  // a row's 8 threads are of one warp
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < VN; ++e) o[c][e] *= alpha;
+      __syncwarp();  // a row's 16 threads are of one warp
 #pragma unroll 2
       for (int j = 0; j < BK; j += VN) {
-        const Word<A> e4 = word(ps + r * L::LP + j);
+        const Word<A> e0 = word(ps + r0 * L::LP + j), e1 = word(ps + (r0 + 8) * L::LP + j);
 #pragma unroll
         for (int i = 0; i < VN; ++i)
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
             const int col = (sub + TPR * c) * VN;
+            if (DMAX % (VN * TPR) != 0 && col >= DMAX) continue;  // fp32 rows of 32: 8 words for 16 threads
             const Word<A> y = word(vs + (j + i) * L::LD + col);
 #pragma unroll
-            for (int e = 0; e < VN; ++e) o[c][e] += e4[i] * y[e];
+            for (int e = 0; e < VN; ++e) {
+              o[0][c][e] += e0[i] * y[e];
+              o[1][c][e] += e1[i] * y[e];
+            }
           }
       }
       __syncwarp();
     }
 #pragma unroll
-    for (int x = 1; x < TPR; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const A inv = l == A(0) ? A(0) : A(1) / l;  // no visible key: zeros and -inf
-    const A lse = l == A(0) ? A(-INFINITY) : m + log_of(l);
-    const int64_t at = row * p.o_ss + head * p.o_sh, part = static_cast<int64_t>(g.slot) * BQ + r;
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int x = 1; x < TPR; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+      const A inv = l[h] == A(0) ? A(0) : A(1) / l[h];  // no visible key: zeros and -inf
+      const A lse = l[h] == A(0) ? A(-INFINITY) : m[h] + log_of(l[h]);
+      const int64_t at = row[h] * p.o_ss + head[h] * p.o_sh, part = static_cast<int64_t>(g.slot) * BQ + r0 + 8 * h;
 #pragma unroll
-      for (int e = 0; e < VN; ++e) {
-        const int d = (sub + TPR * c) * VN + e;
-        if (d >= p.D) continue;
-        if (g.slot >= 0) p.part_o[part * p.D + d] = o[c][e] * inv;
-        else if (in) store_out<A>(p.out, at + d, o[c][e] * inv, p.out_dtype);
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          const int d = (sub + TPR * c) * VN + e;
+          if (d >= p.D) continue;
+          if (g.slot >= 0) p.part_o[part * p.D + d] = o[h][c][e] * inv;
+          else if (in[h]) store_out<A>(p.out, at + d, o[h][c][e] * inv, p.out_dtype);
+        }
+      if (sub == 0) {
+        if (g.slot >= 0) p.part_lse[part] = lse;
+        else if (in[h] && p.lse != nullptr) p.lse[head[h] * p.l_sh + row[h] * p.l_ss] = lse;
       }
-    if (sub == 0) {
-      if (g.slot >= 0) p.part_lse[part] = lse;
-      else if (in && p.lse != nullptr) p.lse[head * p.l_sh + row * p.l_ss] = lse;
     }
     return true;
   });
