@@ -5,10 +5,12 @@
 // tokens into the 128 rows of each of two MMA tiles ("halves"), so short chunks fill the rows and every K/V tile
 // is read once for all heads that share it.  Q rows (token, head) come from one TMA box of (64, G, 128 / G).
 //   warps 0-3 / 4-7   softmax and epilogue of half 0 / 1: one thread per query row (= TMEM lane)
-//   warp 8 / 10       the K / V ring: 128-key tiles, one TMA box per page (or part of one), one box per lane
+//   warp 8 / 10       the K / V ring: 64-key tiles, one TMA box per page (or part of one), one box per lane
 //   warp 9 / 11       MMA issuer of half 0 / 1 (one thread), which also loads its half's Q
-// The issuers take turns, each pushing PV_h(u - 1), S_h(u) for the running tile number u, as in the dense prefill
-// kernel (attn_tc2.cuh): one half's products run during the other's softmax.  The tile numbers and rings run on across
+// Tiles of 64 keys leave room in tensor memory for two S buffers per half (2 x (2 x 64 + D) columns), so an issuer keeps
+// S two tiles ahead of PV: S_h(c + 2) is pushed behind PV_h(c), whose P_h it overwrites, and a half's softmax finds the
+// next scores waiting instead of standing in the chain S -> softmax -> PV.  (With tiles of 128 keys and one buffer, as in
+// the dense prefill kernel, that chain set the pace.)  The tile numbers and rings run on across
 // segments.  A new segment needs no drain: its Q_h is loaded once the last S_h of the old one is complete, during that
 // tile's softmax; its first PV_h, which overwrites O_h, waits for a P_h that the softmax warps write after their
 // epilogue has read O_h.
@@ -27,41 +29,43 @@ namespace paged {
 namespace tc {
 
 using cea::tc2::umma_ts;
-using cea::tc2::warp_wait;
 
 constexpr int BM = 128;
-constexpr int BK = 128;
+constexpr int BK = 64;
 constexpr int NUM_THREADS = 384;
 constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 10, kMmaWarp1 = 11;
 constexpr int kLaunchRegs = 168, kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kLaunchRegs * NUM_THREADS, "register split");
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kPCol = 64;
+constexpr uint32_t kPCol = 32;  // P_h (pairs of 16 bit) within its S_h buffer
 constexpr float kRescaleThreshold = 8.0f;
 static_assert(2 * BM == kWideRows, "rows of a slot");
 
 template <int D>
 struct Layout {
   static constexpr int KBOX = D / 64;
-  static constexpr int BOX = 128 * 128;  // 64 columns of 128 rows
+  static constexpr int QBOX = BM * 128;  // 64 columns of 128 query rows
+  static constexpr int QTILE = KBOX * QBOX;
+  static constexpr int BOX = BK * 128;   // 64 columns of 64 keys
   static constexpr int TILE = KBOX * BOX;
-  static constexpr int KST = D == 128 ? 3 : 5;
-  static constexpr int VST = D == 128 ? 2 : 5;
+  static constexpr int KST = D == 128 ? 5 : 10;
+  static constexpr int VST = D == 128 ? 5 : 10;
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_K = OFF_Q + 2 * QTILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_BAR = OFF_V + VST * TILE;
-  static constexpr int B_QFULL = 0;  // x2
+  static constexpr int B_QFULL = 0;  // x2 (per half)
   static constexpr int B_KFULL = B_QFULL + 2;
   static constexpr int B_KEMPTY = B_KFULL + KST;
   static constexpr int B_VFULL = B_KEMPTY + KST;
   static constexpr int B_VEMPTY = B_VFULL + VST;
   static constexpr int B_VTAIL = B_VEMPTY + VST;  // a V tile that is zeroed behind its last key before it counts as full
-  static constexpr int B_SFULL = B_VTAIL + 1;     // x2
-  static constexpr int B_PFULL = B_SFULL + 2;     // x2
-  static constexpr int B_PVDONE = B_PFULL + 2;    // x2
-  static constexpr int B_TURN = B_PVDONE + 2;     // x2
-  static constexpr int B_QUEUE = B_TURN + 2;
+  // x4: [half][S buffer].  One barrier per buffer: each phase is met before its next one can begin, where a barrier for
+  // both would run two phases ahead of a waiter.
+  static constexpr int B_SFULL = B_VTAIL + 1;
+  static constexpr int B_PFULL = B_SFULL + 4;
+  static constexpr int B_PVDONE = B_PFULL + 4;
+  static constexpr int B_QUEUE = B_PVDONE + 4;
   static constexpr int NBAR = B_QUEUE + SegQueue::kBars;
   static constexpr int OFF_QUEUE = (OFF_BAR + NBAR * 8 + 15) / 16 * 16;
   static constexpr int OFF_MISC = OFF_QUEUE + SegQueue::kBytes;
@@ -86,6 +90,32 @@ struct Params {
   float scale_log2;
 };
 
+// One thread of a warp that runs in step.  The issuing warps keep in step and wrap only the tcgen05 instructions so:
+// their operands are then uniform over the warp and stay in uniform registers.  With a loop of one thread's own
+// (`lane == 0`) every product cost 75 to 90 cycles to issue, more than the 48 to 64 that it takes to run.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
+// Bounded wait of a whole warp (the contract of mbar_wait), short in code.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++n) {
+    if ((n & 63u) != 0u) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    const bool late = now - t0 > CEA_WAIT_LIMIT_NS;
+    if (__any_sync(0xffffffffu, late || *abort != 0)) {
+      if (late) record_error(code);
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -99,15 +129,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto bar = [&](int i) -> uint32_t { return sbase + L::OFF_BAR + 8 * i; };
   const SegQueue queue{smem + L::OFF_QUEUE, bar(L::B_QUEUE), bar(L::B_QUEUE + kQueue), abort_flag,
                        CEA_DEV_TIMEOUT_PRODUCER};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h) {
       mbar_init(bar(L::B_QFULL + h), 1);
-      mbar_init(bar(L::B_SFULL + h), 1);
-      mbar_init(bar(L::B_PFULL + h), 4);  // one arrival per softmax warp
-      mbar_init(bar(L::B_PVDONE + h), 1);
-      mbar_init(bar(L::B_TURN + h), 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(bar(L::B_SFULL + 2 * h + b), 1);
+        mbar_init(bar(L::B_PFULL + 2 * h + b), 4);  // one arrival per softmax warp
+        mbar_init(bar(L::B_PVDONE + 2 * h + b), 1);
+      }
     }
     for (int s = 0; s < L::KST; ++s) {
       mbar_init(bar(L::B_KFULL + s), 1);
@@ -169,8 +200,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               page = p.bt.num_pages;  // outside the tensor map: reads as zeros
             }
           }
-          bool ok = n == 0 || mbar_wait(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
-          if (!__all_sync(0xffffffffu, ok)) return false;
+          if (n > 0 && !wait_all(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER)) return false;
           const int boxes = __popc(__ballot_sync(0xffffffffu, load));
           const int left = g.keys - t * BK;
           const bool tail = !is_k && left < BK;
@@ -180,8 +210,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           __syncwarp();
           if (load) tma_load_4d(to + col * L::BOX + box * p.box * 128, map, fb, col * 64, slot, g.hu, page);
           if (tail) {
-            ok = mbar_wait(bar(L::B_VTAIL), tails & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER);
-            if (!__all_sync(0xffffffffu, ok)) return false;
+            if (!wait_all(bar(L::B_VTAIL), tails & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER)) return false;
             ++tails;
             uint8_t* tile = smem + L::OFF_V + st * L::TILE;
             for (int i = max(left, 0) * 8 + lane; i < BK * 8; i += 32)
@@ -207,91 +236,106 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         while (queue.get(i++, g, lane))
           if (!load_tiles(g)) break;
       }
-    } else if (lane == 0) {
-      // ---------------------------------------------------------- MMA issuer of half h (one thread)
+    } else {
+      // ---------------------------------------------------------- MMA issuer of half h: one elected thread, the warp in step
       const int h = warp == kMmaWarp ? 0 : 1;
       constexpr uint32_t kIdescQK = idesc_f16(kBF16, false, BM, BK);
       constexpr uint32_t kIdescPV = idesc_f16(kBF16, true, BM, D);
-      const uint32_t tS = tmem + 256 * h;
-      const uint32_t tP = tS + kPCol;
+      const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0) + 256 * h;  // two buffers of BK columns
       const uint32_t tO = tS + 128;
-      const uint64_t qdesc = sw128_desc(sbase + L::OFF_Q + h * L::TILE, 16, 1024);
+      const uint64_t qdesc = sw128_desc(sbase + L::OFF_Q + h * L::QTILE, 16, 1024);
       const uint64_t kdesc0 = sw128_desc(sbase + L::OFF_K, 16, 1024);
       const uint64_t vdesc0 = sw128_desc(sbase + L::OFF_V, L::BOX, 1024);
-      int u = 0;        // tile number, both halves alike
-      int cnt = 0;      // tiles this half computed
-      uint32_t nq = 0;  // segments this half loaded Q for
-      bool pend = false, pend_first = false;  // PV of tile u - 1 is to be issued; it begins its segment
-      bool ok = true;
-      // pair u: PV_h(u - 1), then S_h(u) if there is a tile u
-      auto pair = [&](bool has_s, bool act, bool first) -> bool {
-        if (has_s && !mbar_wait(bar(L::B_KFULL + u % L::KST), (u / L::KST) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA))
-          return false;
-        const int vs = (u - 1) % L::VST;
-        if (u > 0) {
-          if (pend && !mbar_spin(bar(L::B_PFULL + h), (cnt - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
-          if (!mbar_wait(bar(L::B_VFULL + vs), ((u - 1) / L::VST) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
-        }
-        const bool turn = h == 0 ? (u == 0 || mbar_spin(bar(L::B_TURN + 1), (u - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA))
-                                 : mbar_spin(bar(L::B_TURN + 0), u & 1, abort_flag, CEA_DEV_TIMEOUT_MMA);
-        if (!turn) return false;
-        tc_fence_after();
-        if (pend) {
+      const uint32_t b_s = bar(L::B_SFULL + 2 * h), b_p = bar(L::B_PFULL + 2 * h), b_pv = bar(L::B_PVDONE + 2 * h);
+      const uint32_t b_q = bar(L::B_QFULL + h);
+      int ks = 0, vs = 0;               // next stage of the K and V rings,
+      uint32_t kph = 0, vph = 0;        // and its phase
+      uint32_t sb = 0, sph = 0;         // next S buffer, and the phase that its S will complete
+      uint32_t pb = 0, pph = 0;         // the same of P
+      uint32_t qph = 0;
+      uint32_t pending = 0;             // tiles whose PV is to come, two bits each, the oldest low: 1 computed, 2 first
+      int npend = 0;
+      bool any = false, ok = true;
+      auto issue_pv = [&]() -> bool {
+        if (!wait_all(bar(L::B_VFULL) + 8 * vs, vph, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
+        if (pending & 1u) {
+          if (!wait_all(b_p + 8 * pb, pph, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
+          tc_fence_after();
           const uint64_t vdesc = vdesc0 + static_cast<uint64_t>((vs * L::TILE) >> 4);
+          const uint32_t tP = tS + BK * pb + kPCol;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            umma_ts(tO, tP + kk * 8, vdesc + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
-                    (!pend_first || kk > 0) ? 1u : 0u);
-          umma_commit(bar(L::B_PVDONE + h));
-          umma_commit(bar(L::B_VEMPTY + vs));
-        } else if (u > 0) {
-          mbar_arrive(bar(L::B_VEMPTY + vs));
-        }
-        if (has_s) {
-          const int ks = u % L::KST;
-          if (act) {
-            if (first && !mbar_wait(bar(L::B_QFULL + h), (nq - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
-            const uint64_t kdesc = kdesc0 + static_cast<uint64_t>((ks * L::TILE) >> 4);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t o = ((kk >> 2) * L::BOX + (kk & 3) * 32) >> 4;
-              umma_ss(tS, qdesc + o, kdesc + o, kIdescQK, kk > 0 ? 1u : 0u);
-            }
-            umma_commit(bar(L::B_SFULL + h));
-            umma_commit(bar(L::B_KEMPTY + ks));
-            ++cnt;
-          } else {
-            mbar_arrive(bar(L::B_KEMPTY + ks));
+            for (int kk = 0; kk < BK / 16; ++kk)
+              umma_ts(tO, tP + kk * 8, vdesc + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
+                      (!(pending & 2u) || kk > 0) ? 1u : 0u);
+            umma_commit(b_pv + 8 * pb);
+            umma_commit(bar(L::B_VEMPTY) + 8 * vs);
           }
+          __syncwarp();
+          pph ^= pb;
+          pb ^= 1u;
+        } else if (elect_one()) {
+          mbar_arrive(bar(L::B_VEMPTY) + 8 * vs);
         }
-        mbar_arrive(bar(L::B_TURN + h));
-        pend = has_s && act;
-        pend_first = first;
+        vs = vs + 1 == L::VST ? 0 : vs + 1;
+        vph ^= vs == 0 ? 1u : 0u;
+        pending >>= 2;
+        --npend;
         return true;
       };
       Seg g;
-      for (int i = 0; ok && queue.get1(i, g); ++i) {
-        const int tok = g.blk * p.dv.tb + h * p.half;
-        const bool act = tok < g.n || h == 0;
+      for (int i = 0; ok && queue.get(i, g, lane); ++i) {
+        const int tok = __shfl_sync(0xffffffffu, g.blk * p.dv.tb + h * p.half, 0);
+        const bool act = h == 0 || tok < __shfl_sync(0xffffffffu, g.n, 0);
+        const int t0 = __shfl_sync(0xffffffffu, g.t0, 0), t1 = __shfl_sync(0xffffffffu, g.t1, 0);
         if (act) {
           // Q_h is free once this half's last S is complete
-          if (cnt > 0 && !mbar_spin(bar(L::B_SFULL + h), (cnt - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_MMA)) {
+          if (any && !wait_all(b_s + 8 * (sb ^ 1u), sph ^ (sb ^ 1u), abort_flag, CEA_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(bar(L::B_QFULL + h), L::KBOX * 128 * p.half * p.dv.group);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(b_q, L::KBOX * 128 * p.half * p.dv.group);
 #pragma unroll
-          for (int kb = 0; kb < L::KBOX; ++kb)
-            tma_load_4d(sbase + L::OFF_Q + h * L::TILE + kb * L::BOX, &tmQ, bar(L::B_QFULL + h), kb * 64,
-                        g.hu * p.dv.group, g.row0 + tok, 0);
-          ++nq;
+            for (int kb = 0; kb < L::KBOX; ++kb)
+              tma_load_4d(sbase + L::OFF_Q + h * L::QTILE + kb * L::QBOX, &tmQ, b_q, kb * 64, g.hu * p.dv.group,
+                          g.row0 + tok, 0);
+          }
+          __syncwarp();
         }
-        for (int t = g.t0; ok && t < g.t1; ++t) {
-          ok = pair(true, act, t == g.t0);
-          ++u;
+        for (int t = t0; t < t1; ++t) {
+          // S runs two tiles ahead of PV; S(c + 2) follows PV(c) in this thread's order, hence overwrites P(c) behind it
+          if (npend == 2 && !(ok = issue_pv())) break;
+          if (!(ok = wait_all(bar(L::B_KFULL) + 8 * ks, kph, abort_flag, CEA_DEV_TIMEOUT_MMA))) break;
+          if (act) {
+            if (t == t0) {
+              if (!(ok = wait_all(b_q, qph, abort_flag, CEA_DEV_TIMEOUT_MMA))) break;
+              qph ^= 1u;
+            }
+            tc_fence_after();
+            const uint64_t kdesc = kdesc0 + static_cast<uint64_t>((ks * L::TILE) >> 4);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_ss(tS + BK * sb, qdesc + (((kk >> 2) * L::QBOX + (kk & 3) * 32) >> 4),
+                        kdesc + (((kk >> 2) * L::BOX + (kk & 3) * 32) >> 4), kIdescQK, kk > 0 ? 1u : 0u);
+              umma_commit(b_s + 8 * sb);
+              umma_commit(bar(L::B_KEMPTY) + 8 * ks);
+            }
+            __syncwarp();
+            sph ^= sb;
+            sb ^= 1u;
+            any = true;
+          } else if (elect_one()) {
+            mbar_arrive(bar(L::B_KEMPTY) + 8 * ks);
+          }
+          ks = ks + 1 == L::KST ? 0 : ks + 1;
+          kph ^= ks == 0 ? 1u : 0u;
+          pending |= ((act ? 1u : 0u) | (t == t0 ? 2u : 0u)) << (2 * npend);
+          ++npend;
         }
       }
-      if (ok && u > 0) pair(false, false, false);
+      while (ok && npend > 0) ok = issue_pv();
     }
   } else {
     // ================================================================ softmax + epilogue
@@ -316,14 +360,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int first_limit = p.dv.causal ? min(g.ctx + tok0, seen) : seen;  // of the half's first token
       float m = -INFINITY, l = 0.f;
       for (int t = g.t0; t < g.t1; ++t) {
-        if (!warp_wait(bar(L::B_SFULL + h), it & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
+        const int b = it & 1;
+        if (!wait_all(bar(L::B_SFULL + 2 * h + b), (it >> 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint32_t s[BK];
 #pragma unroll
-        for (int c = 0; c < BK / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        for (int c = 0; c < BK / 32; ++c) tmem_ld32(tS + BK * b + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         tmem_wait_ld();
         float mx[8];
 #pragma unroll
@@ -353,7 +398,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           m = m_new;
         }
         const float neg_m = (m == -INFINITY) ? 0.f : -m;
-        if (__any_sync(0xffffffffu, rescale)) {
+        if (__any_sync(0xffffffffu, rescale)) {  // not at a segment's first tile
+          // S_h(it) complete means PV_h(it - 2) complete: the parity wait for PV_h(it - 1) is unambiguous
+          if (!wait_all(bar(L::B_PVDONE + 2 * h + (b ^ 1)), ((it - 1) >> 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -369,25 +420,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (int a = 0; a < 4; ++a) rs2[a] = 0ull;
         const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
         const uint64_t negm2 = f2_pack(neg_m, neg_m);
+        {
 #pragma unroll
-        for (int c = 0; c < BK / 32; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < BK / 32; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])),
-                             scale2, negm2),
-                      x0, x1);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            rs2[e & 3] = f2_add(rs2[e & 3], f2_pack(p0, p1));
-            pk[e] = pack2(p0, p1, kBF16);
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t x = f2_fma(
+                  f2_pack(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])), scale2, negm2);
+              float p0, p1;
+              f2_unpack(x, p0, p1);
+              p0 = fast_exp2(p0);
+              p1 = fast_exp2(p1);
+              rs2[e & 3] = f2_add(rs2[e & 3], f2_pack(p0, p1));
+              pk[e] = pack2(p0, p1, kBF16);
+            }
+            tmem_st16(tS + BK * b + kPCol + c * 16, pk);
           }
-          tmem_st16(tS + kPCol + c * 16, pk);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::B_PFULL + h));
+        if (lane == 0) mbar_arrive(bar(L::B_PFULL + 2 * h + b));
         {
           const uint64_t r = f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3]));
           float r0, r1;
@@ -398,8 +452,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       if (!ok) break;
       // ---------------------------------------------------------------- epilogue of the segment
-      // S_h(it - 1) completed, hence PV_h(it - 2) did: the parity wait for PV_h(it - 1) is unambiguous
-      ok = warp_wait(bar(L::B_PVDONE + h), (it - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX);
+      // S_h(it - 1) completed, hence PV_h(it - 3) did: the parity wait for PV_h(it - 1) is unambiguous
+      ok = wait_all(bar(L::B_PVDONE + 2 * h + ((it - 1) & 1)), ((it - 1) >> 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX);
       if (!ok) break;
       tc_fence_after();
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
