@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
 
 // The same for the chunk kernel's slots of 256 rows, laid out [slot][D / 4][row][4] so that its rows (one a thread) are
 // written, and read here, in whole lines.  Bound by L2: block (c, y) takes 32 rows, one a lane, and each of its 8 warps
-// D / 8 columns; a lane has two parts' statistics and columns in flight at a time (a unit seldom has more than three).
+// D / 8 columns; a lane has four parts' statistics and columns in flight at a time.
 // One warp a row with a lane per 4 columns took 17 us for 148 split units of 256 rows, bound by the latency of four
 // waves of blocks.
 constexpr int kWideRows = 256;
@@ -534,28 +534,41 @@ __global__ void __launch_bounds__(kCombineThreads) combine_wide_kernel(const __g
   float4 acc[C4];
 #pragma unroll
   for (int j = 0; j < C4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < parts; i += 2) {
-    float lse[2];
-    float4 v[2][C4];
+  constexpr int P = 4;
+  for (int i = 0; i < parts; i += P) {
+    float lse[P], up = top;
+    float4 v[P][C4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int64_t slot = i + k == 0 ? 2 * c + 1 : 2 * (c + min(i + k, parts - 1));
-      lse[k] = i + k < parts ? a.part_lse[slot * kWideRows + row] : -INFINITY;
-      const float4* src = reinterpret_cast<const float4*>(a.part_o) + (slot * (D / 4) + warp * C4) * kWideRows + row;
+    for (int k = 0; k < P; ++k) {
+      lse[k] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < C4; ++j) v[k][j] = src[j * kWideRows];
+      for (int j = 0; j < C4; ++j) v[k][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i + k < parts) {
+        const int64_t slot = i + k == 0 ? 2 * c + 1 : 2 * (c + i + k);
+        lse[k] = a.part_lse[slot * kWideRows + row];
+        const float4* src = reinterpret_cast<const float4*>(a.part_o) + (slot * (D / 4) + warp * C4) * kWideRows + row;
+#pragma unroll
+        for (int j = 0; j < C4; ++j) v[k][j] = src[j * kWideRows];
+      }
     }
-    const float up = fmaxf(top, fmaxf(lse[0], lse[1])), ref = up == -INFINITY ? 0.f : up;
-    const float w = expf(top - ref), w0 = expf(lse[0] - ref), w1 = i + 1 < parts ? expf(lse[1] - ref) : 0.f;
-    top = up;
-    sum = sum * w + w0 + w1;
 #pragma unroll
-    for (int j = 0; j < C4; ++j) {
-      if (i + 1 >= parts) v[1][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      acc[j].x = acc[j].x * w + w0 * v[0][j].x + w1 * v[1][j].x;
-      acc[j].y = acc[j].y * w + w0 * v[0][j].y + w1 * v[1][j].y;
-      acc[j].z = acc[j].z * w + w0 * v[0][j].z + w1 * v[1][j].z;
-      acc[j].w = acc[j].w * w + w0 * v[0][j].w + w1 * v[1][j].w;
+    for (int k = 0; k < P; ++k) up = fmaxf(up, lse[k]);
+    const float ref = up == -INFINITY ? 0.f : up, w = expf(top - ref);
+    top = up;
+    sum *= w;
+#pragma unroll
+    for (int j = 0; j < C4; ++j) acc[j] = make_float4(acc[j].x * w, acc[j].y * w, acc[j].z * w, acc[j].w * w);
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const float wk = expf(lse[k] - ref);
+      sum += wk;
+#pragma unroll
+      for (int j = 0; j < C4; ++j) {
+        acc[j].x += wk * v[k][j].x;
+        acc[j].y += wk * v[k][j].y;
+        acc[j].z += wk * v[k][j].z;
+        acc[j].w += wk * v[k][j].w;
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -465,30 +465,31 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int prow = h * p.half * G + row;  // of the slot: [D / 4][row][4]
       float4* part = reinterpret_cast<float4*>(p.part_o) + static_cast<int64_t>(slot) * (D / 4) * kWideRows + prow;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        uint32_t o[16];
-        tmem_ld16(tO + c * 16, o);
+      for (int c = 0; c < D; c += 64) {
+        uint32_t o[64];
+        tmem_ld32(tO + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+        tmem_ld32(tO + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
         tmem_wait_ld();
         if (!row_in) continue;
-        float f[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv_l;
+        for (int e = 0; e < 64; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv_l);
+        auto f = [&](int e) { return __uint_as_float(o[e]); };
         if (slot >= 0) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            part[(c * 4 + e) * kWideRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          for (int e = 0; e < 64; e += 4)
+            part[((c + e) / 4) * kWideRows] = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
         } else if (p.out_dtype == CEA_F32) {
-          float* dst = reinterpret_cast<float*>(p.out) + obase + c * 16;
+          float* dst = reinterpret_cast<float*>(p.out) + obase + c;
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(dst + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          for (int e = 0; e < 64; e += 4)
+            *reinterpret_cast<float4*>(dst + e) = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
         } else {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + obase + c * 16;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + obase + c;
 #pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack2(f[e], f[e + 1], kBF16), pack2(f[e + 2], f[e + 3], kBF16),
-                                                            pack2(f[e + 4], f[e + 5], kBF16),
-                                                            pack2(f[e + 6], f[e + 7], kBF16));
+          for (int e = 0; e < 64; e += 8)
+            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack2(f(e), f(e + 1), kBF16), pack2(f(e + 2), f(e + 3), kBF16),
+                                                            pack2(f(e + 4), f(e + 5), kBF16),
+                                                            pack2(f(e + 6), f(e + 7), kBF16));
         }
       }
       tc_fence_before();
