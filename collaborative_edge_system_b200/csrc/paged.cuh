@@ -42,8 +42,10 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
 // ------------------------------------------------------------------ division of the attention work
 // A unit of work is one block of `tb` new tokens of one sequence for one KV head (or, in the generic kernel, for a
 // group of its query heads), over the keys its last token sees.  The units are laid end to end on one axis, each as
-// long as the keys it reads (at least 1), and CTA c of n takes the tiles that start in [W c / n, W (c + 1) / n):
-// every CTA gets the same number of tiles whatever the lengths are, with nothing known on the host.  A unit split
+// long as the keys it reads (at least 1) and `cost` more, and CTA c of n takes the tiles that start in its share of
+// the axis: every CTA gets the same work whatever the lengths are, with nothing known on the host.  `cost` is what a
+// unit takes besides its tiles (loading its queries, filling the pipeline, writing its result), in keys: without it
+// the CTAs that got many short units ended last (2048 tokens alone: 83 us, against 61 us with it).  A unit split
 // over CTAs leaves partial results, at most two a CTA (one that began before it, one that goes on behind it), which
 // combine_kernel joins; so the workspace depends on the grid alone.  A sequence's units form an arithmetic series
 // (block i of a causal chunk reads tb more keys than block i - 1), so its length and the block at a coordinate have
@@ -54,6 +56,7 @@ struct Division {
   int64_t max_rows, min_rows;  // sequences with n * group outside [min_rows, max_rows] belong to another kernel
   int min_n, max_n;  // what the caller promised of sequences with n > 0
   int causal;
+  int cost;             // of a unit besides its keys
   int min_share_log2;   // smallest share of the axis worth a CTA of its own; at least a tile
 };
 
@@ -62,11 +65,12 @@ struct SeqUnits {
   int64_t S;  // length on the axis of one head's units
 };
 
-__device__ __forceinline__ int64_t units_before(const SeqUnits& s, int i, int tb, bool causal) {
-  if (!causal) return static_cast<int64_t>(i) * max(1, s.len);
-  if (i <= s.n0) return i;
+__device__ __forceinline__ int64_t units_before(const SeqUnits& s, int i, const Division& dv) {
+  const int64_t cost = static_cast<int64_t>(i) * dv.cost;
+  if (!dv.causal) return static_cast<int64_t>(i) * max(1, s.len) + cost;
+  if (i <= s.n0) return i + cost;
   const int64_t m = i - s.n0;
-  return s.n0 + m * s.ctx + static_cast<int64_t>(tb) * (m * (2ll * s.n0 + m + 1) / 2);
+  return s.n0 + m * s.ctx + static_cast<int64_t>(dv.tb) * (m * (2ll * s.n0 + m + 1) / 2) + cost;
 }
 
 // keys that block i reads (its last token's view)
@@ -87,24 +91,28 @@ __device__ __forceinline__ SeqUnits seq_units(const Division& dv, const Seq& q) 
     s.nb = q.n > 0 && q.n <= dv.tb ? 1 : 0;
     s.n0 = 0;
     s.ctx = q.len - q.n;
-    s.S = s.nb * max(1, q.len);
+    s.S = s.nb * (max(1, q.len) + dv.cost);
     return s;
   }
   const int64_t rows = static_cast<int64_t>(q.n) * dv.group;
   s.nb = q.n > 0 && rows >= dv.min_rows && rows <= dv.max_rows ? (q.n + dv.tb - 1) / dv.tb : 0;
   s.ctx = q.len - q.n;  // may be negative: the first tokens then see nothing
   s.n0 = s.ctx < 0 ? min(static_cast<int>((-static_cast<int64_t>(s.ctx)) / dv.tb), max(s.nb - 1, 0)) : 0;
-  s.S = s.nb == 0 ? 0 : units_before(s, s.nb - 1, dv.tb, dv.causal) + max(1, unit_keys(s, s.nb - 1, dv.tb, dv.causal));
+  s.S = s.nb == 0 ? 0
+                  : units_before(s, s.nb - 1, dv) + max(1, unit_keys(s, s.nb - 1, dv.tb, dv.causal)) + dv.cost;
   return s;
+}
+
+// 64-bit division costs several hundred cycles, most axes fit 32 bits
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
 // CTA c's share of an axis of length W: [base c + min(c, rem), base (c + 1) + min(c + 1, rem)), W = base n + rem.
 struct Share {
-  int64_t W, lo, hi, base;
+  int64_t base;
   int n, rem;  // CTAs that take part
-  int b;       // sequence at lo
-  int64_t at;  // where that sequence starts
-  SeqUnits s;  // its units
 
   __device__ __forceinline__ int64_t start(int c) const { return base * c + min(c, rem); }
   // the CTA whose share holds x
@@ -112,167 +120,30 @@ struct Share {
     const int64_t wide = (base + 1) * rem;  // the first rem shares are one longer
     return x < wide ? static_cast<int>(div64(x, base + 1)) : rem + static_cast<int>(div64(x - wide, base));
   }
-  // 64-bit division costs several hundred cycles, most axes fit 32 bits
-  __device__ __forceinline__ static int64_t div64(int64_t a, int64_t b) {
-    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
-  }
 };
 
-// Called by one whole warp.
-template <bool kOne>
-__device__ __forceinline__ Share divide(const Batch& bt, const Division& dv) {
-  const int lane = threadIdx.x & 31;
-  const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
-  // 32 sequences: this lane's, its units' length together, and the end of that on an axis of the 32
-  Seq q;
-  int64_t w, end;
-  auto round = [&](int b0) {
-    const int b = b0 + lane;
-    q = Seq{0, 0, 0};
-    if (b < dv.B) q = load_seq(bt, b);
-    w = seq_units<kOne>(dv, q).S * dv.units_h;
-    end = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= o) end += up;
-    }
-  };
-  int64_t more = 0;  // behind the first 32
-  for (int b = lane; b < dv.B; b += 32) {
-    const Seq x = load_seq(bt, b);
-    if (b >= 32) more += seq_units<kOne>(dv, x).S * dv.units_h;
-    // a length that the table cannot hold, descending offsets, or a broken promise
-    const int raw = bt.lens[b], o0 = bt.q_off[b], o1 = bt.q_off[b + 1];
-    if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T || (x.n > 0 && (x.n < dv.min_n || x.n > dv.max_n)))
-      report(CEA_DEV_BAD_BATCH);
-  }
-  round(0);
-  Share sh;
-  sh.W = __shfl_sync(0xffffffffu, end, 31);
-  if (dv.B > 32) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
-    sh.W += more;
-  }
-  sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), sh.W >> dv.min_share_log2)));
-  sh.base = Share::div64(sh.W, sh.n);
-  sh.rem = static_cast<int>(sh.W - sh.base * sh.n);
-  const int c = min(static_cast<int>(blockIdx.x), sh.n);
-  sh.lo = sh.start(c);
-  sh.hi = sh.start(min(c + 1, sh.n));
-  // the sequence that holds lo, 32 at a time
-  sh.b = dv.B;
-  sh.at = sh.W;
-  int64_t before = 0;
-  for (int b0 = 0; b0 < dv.B && sh.lo < sh.hi; b0 += 32) {
-    if (b0 > 0) round(b0);
-    const unsigned hit = __ballot_sync(0xffffffffu, before + end > sh.lo);
-    if (hit != 0u) {
-      const int l = __ffs(hit) - 1;
-      sh.b = b0 + l;
-      sh.at = before + __shfl_sync(0xffffffffu, end - w, l);
-      sh.s = seq_units<kOne>(dv, Seq{__shfl_sync(0xffffffffu, q.row0, l), __shfl_sync(0xffffffffu, q.n, l),
-                                     __shfl_sync(0xffffffffu, q.len, l)});
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, end, 31);
-  }
-  return sh;
-}
-
-// The last block that starts at or before r on a head's part of the axis: r = n0 + (tb m^2 + a m) / 2 with
-// a = 2 (ctx + tb n0) + tb solved for m (in the form without a difference of large numbers), then put right where the
-// float was off.
-__device__ __forceinline__ int block_at(const SeqUnits& s, int64_t r, int tb, bool causal) {
-  if (!causal) return static_cast<int>(Share::div64(r, max(1, s.len)));
+// The last block that starts at or before r on a head's part of the axis: r = n0 + (tb m^2 + a m) / 2 + cost (n0 + m)
+// with a = 2 (ctx + tb n0) + tb solved for m (in the form without a difference of large numbers), then put right where
+// the float was off.
+__device__ __forceinline__ int block_at(const SeqUnits& s, int64_t r, const Division& dv) {
   int i;
-  if (r < s.n0) {
-    i = static_cast<int>(r);
+  if (!dv.causal) {
+    i = static_cast<int>(div64(r, max(1, s.len) + dv.cost));
   } else {
-    const float a = 2.f * (s.ctx + tb * s.n0) + tb, x = static_cast<float>(r - s.n0);
-    const float d = sqrtf(a * a + 8.f * tb * x);
-    const float m = a > 0.f ? 4.f * x / (a + d) : (d - a) / (2.f * tb);
-    i = s.n0 + static_cast<int>(m);
+    const int64_t r0 = static_cast<int64_t>(s.n0) * (1 + dv.cost);
+    if (r < r0) {
+      i = static_cast<int>(div64(r, 1 + dv.cost));
+    } else {
+      const float tb = dv.tb, a = 2.f * (s.ctx + dv.tb * s.n0) + tb + 2.f * dv.cost, x = static_cast<float>(r - r0);
+      const float d = sqrtf(a * a + 8.f * tb * x);
+      i = s.n0 + static_cast<int>(a > 0.f ? 4.f * x / (a + d) : (d - a) / (2.f * tb));
+    }
   }
   i = min(max(i, 0), s.nb - 1);
-  while (i + 1 < s.nb && units_before(s, i + 1, tb, true) <= r) ++i;
-  while (i > 0 && units_before(s, i, tb, true) > r) --i;
+  while (i + 1 < s.nb && units_before(s, i + 1, dv) <= r) ++i;
+  while (i > 0 && units_before(s, i, dv) > r) --i;
   return i;
 }
-
-// The segments (a unit and a range of its key tiles) of one CTA's share, in order.
-template <int BK, bool kOne>
-struct Segments {
-  const Batch& bt;
-  const Division& dv;
-  const Share& sh;
-  SeqUnits s;
-  int b, hu, blk;       // the unit
-  int64_t pos;          // its start
-  int keys, t0, t1, nt; // keys the unit reads; its tiles [t0, t1) of nt belong to this CTA
-
-  __device__ __forceinline__ Segments(const Batch& bt_, const Division& dv_, const Share& sh_)
-      : bt(bt_), dv(dv_), sh(sh_), s(sh_.s), b(sh_.b) {
-    if (sh.lo >= sh.hi || b >= dv.B) {
-      b = dv.B;
-      return;
-    }
-    int64_t r = sh.lo - sh.at;
-    hu = static_cast<int>(Share::div64(r, s.S));
-    r -= hu * s.S;
-    blk = kOne ? 0 : block_at(s, r, dv.tb, dv.causal);
-    pos = sh.at + hu * s.S + (kOne ? 0 : units_before(s, blk, dv.tb, dv.causal));
-    settle();
-  }
-
-  __device__ __forceinline__ bool done() const { return b >= dv.B; }
-
-  // tiles that start before x, of those whose first one starts at 0
-  __device__ __forceinline__ static int tiles(int64_t x) { return static_cast<int>((max(x, int64_t(0)) + BK - 1) / BK); }
-
-  // the current unit's tiles, or those of the next unit that has some here
-  __device__ __forceinline__ void settle() {
-    while (true) {
-      if (pos >= sh.hi) {
-        b = dv.B;
-        return;
-      }
-      keys = kOne ? s.len : unit_keys(s, blk, dv.tb, dv.causal);
-      nt = max(1, (keys + BK - 1) / BK);
-      t0 = tiles(sh.lo - pos);
-      t1 = min(nt, tiles(min(sh.hi - pos, int64_t(0x7fffffff - BK))));
-      if (t0 < t1) return;
-      step();
-      if (b >= dv.B) return;
-    }
-  }
-
-  __device__ __forceinline__ void step() {
-    pos += max(1, keys);
-    if (!kOne) {
-      if (++blk < s.nb) return;
-      blk = 0;
-    }
-    if (++hu < dv.units_h) return;
-    hu = 0;
-    do {
-      if (++b >= dv.B) return;
-      s = seq_units<kOne>(dv, load_seq(bt, b));
-    } while (s.S == 0);
-  }
-
-  __device__ __forceinline__ void next() {
-    step();
-    if (b < dv.B) settle();
-  }
-
-  // last CTA with a tile of this unit
-  __device__ __forceinline__ int last_cta() const {
-    return sh.cta_of(pos + static_cast<int64_t>(nt - 1) * BK);
-  }
-};
 
 // What the warps of a CTA need of a segment.
 struct alignas(16) Seg {
@@ -347,23 +218,103 @@ struct SegQueue {
 };
 
 // Walks this CTA's share: one whole warp, which hands every segment to `take` (and a Seg with b = -1 at the end); the
-// unit that goes on behind the share is described in `meta`.
+// unit that goes on behind the share is described in `meta`.  The code is met once per launch, from cold instruction
+// caches, so each piece of it stands here once.
 template <int BK, bool kOne, typename Take>
 __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool dead, Meta* meta, const Take& take) {
-  const Share sh = divide<kOne>(bt, dv);
+  const int lane = threadIdx.x & 31, cta = blockIdx.x;
+  const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
+  Share sh;
+  SeqUnits s;
+  int64_t W = 0, lo = 0, hi = 0, pos = 0;  // the axis, this CTA's share, and where on it the walk is
+  int b = dv.B;                            // sequence at lo
+  // the axis's length, then the sequence that holds lo: 32 sequences at a time, one a lane
+  Seq q = {0, 0, 0};
+  int64_t w = 0, end = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t before = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < dv.B; b0 += 32) {
+      if (pass == 0 || dv.B > 32) {
+        q = Seq{0, 0, 0};
+        if (b0 + lane < dv.B) {
+          q = load_seq(bt, b0 + lane);
+          // a length that the table cannot hold, descending offsets, or a broken promise
+          const int raw = bt.lens[b0 + lane], o0 = bt.q_off[b0 + lane], o1 = bt.q_off[b0 + lane + 1];
+          if (raw < 0 || raw > cap || o0 < 0 || o1 < o0 || o1 > bt.T || (q.n > 0 && (q.n < dv.min_n || q.n > dv.max_n)))
+            report(CEA_DEV_BAD_BATCH);
+        }
+        end = w = seq_units<kOne>(dv, q).S * dv.units_h;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t up = __shfl_up_sync(0xffffffffu, end, o);
+          if (lane >= o) end += up;
+        }
+      }
+      if (pass == 1) {
+        const unsigned hit = __ballot_sync(0xffffffffu, before + end > lo);
+        if (hit != 0u) {
+          const int l = __ffs(hit) - 1;
+          b = b0 + l;
+          pos = before + __shfl_sync(0xffffffffu, end - w, l);
+          q = Seq{__shfl_sync(0xffffffffu, q.row0, l), __shfl_sync(0xffffffffu, q.n, l),
+                  __shfl_sync(0xffffffffu, q.len, l)};
+          break;
+        }
+      }
+      before += __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (pass == 0) {
+      W = before;
+      sh.n = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(int64_t(1), W >> dv.min_share_log2)));
+      sh.base = div64(W, sh.n);
+      sh.rem = static_cast<int>(W - sh.base * sh.n);
+      lo = sh.start(min(cta, sh.n));
+      hi = sh.start(min(cta + 1, sh.n));
+      if (lo >= hi) break;
+    } else {
+      s = seq_units<kOne>(dv, q);
+    }
+  }
+
   Meta behind = {-1, 0, 0, 0, 0};
   int it = 0;
   bool ok = true;
-  if (!dead) {
-    for (Segments<BK, kOne> g(bt, dv, sh); ok && !g.done(); g.next()) {
-      const int cta = blockIdx.x, slot = g.t0 > 0 ? 2 * cta : g.t1 < g.nt ? 2 * cta + 1 : -1;
-      if (g.t0 == 0 && g.t1 < g.nt) behind = Meta{g.last_cta(), g.hu, g.blk, g.s.row0, g.s.n};
-      ok = take(Seg{g.b, g.hu, g.blk, g.s.row0, g.s.n, g.s.ctx, g.s.len, g.keys, g.t0, g.t1, slot, it});
-      it += g.t1 - g.t0;
+  if (b < dv.B && !dead) {
+    // from the start of the sequence to the unit that holds lo
+    int64_t r = lo - pos;
+    int hu = static_cast<int>(div64(r, s.S));
+    r -= hu * s.S;
+    int blk = kOne ? 0 : block_at(s, r, dv);
+    pos += hu * s.S + (kOne ? 0 : units_before(s, blk, dv));
+#pragma unroll 1
+    while (pos < hi) {
+      const int keys = kOne ? s.len : unit_keys(s, blk, dv.tb, dv.causal);
+      const int nt = max(1, (keys + BK - 1) / BK);
+      const int t0 = static_cast<int>((max(lo - pos, int64_t(0)) + BK - 1) / BK);
+      const int t1 = static_cast<int>(min(static_cast<int64_t>(nt), (hi - pos + BK - 1) / BK));
+      if (t0 < t1) {
+        const int slot = t0 > 0 ? 2 * cta : t1 < nt ? 2 * cta + 1 : -1;
+        if (t0 == 0 && t1 < nt) behind = Meta{sh.cta_of(pos + static_cast<int64_t>(nt - 1) * BK), hu, blk, s.row0, s.n};
+        ok = take(Seg{b, hu, blk, s.row0, s.n, s.ctx, s.len, keys, t0, t1, slot, it});
+        if (!ok) break;
+        it += t1 - t0;
+      }
+      pos += max(1, keys) + dv.cost;
+      if (!kOne && ++blk < s.nb) continue;
+      blk = 0;
+      if (++hu < dv.units_h) continue;
+      hu = 0;
+      do {
+        if (++b >= dv.B) break;
+        s = seq_units<kOne>(dv, load_seq(bt, b));
+      } while (s.S == 0);
+      if (b >= dv.B) break;
     }
   }
   if (ok) take(Seg{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
-  if ((threadIdx.x & 31) == 0) meta[blockIdx.x] = behind;
+  if (lane == 0) meta[cta] = behind;
 }
 
 template <typename A>
