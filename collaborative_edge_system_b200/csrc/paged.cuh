@@ -45,7 +45,8 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
 // long as the keys it reads (at least 1) and `cost` more, and CTA c of n takes the tiles that start in its share of
 // the axis: every CTA gets the same work whatever the lengths are, with nothing known on the host.  `cost` is what a
 // unit takes besides its tiles (loading its queries, filling the pipeline, writing its result), in keys: without it
-// the CTAs that got many short units ended last (2048 tokens alone: 83 us, against 61 us with it).  A unit split
+// the CTAs that got many short units ended last (2048 tokens alone: 83 us, against 58 us with
+// it; 192 keys in the decode kernel and 384 in the chunk kernel were the best of 64 to 512).  A unit split
 // over CTAs leaves partial results, at most two a CTA (one that began before it, one that goes on behind it), which
 // combine_kernel joins; so the workspace depends on the grid alone.  A sequence's units form an arithmetic series
 // (block i of a causal chunk reads tb more keys than block i - 1), so its length and the block at a coordinate have

@@ -246,7 +246,7 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   pg::simt::Params<A> a;
   a.bt = paged_batch(p);
-  a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 64,
+  a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 16,
                       pg::simt::Layout<A, DMAX>::BK == 64 ? 6 : 5};
   a.q = p->q;
   a.k = p->k_pages;
@@ -305,7 +305,7 @@ int launch_paged_decode(const cea_paged_attn_params* p, const PagedPlan& pl, cud
   a.bt = paged_batch(p);
   const PagedChoice choice = paged_choice(p);
   a.dv = pg::Division{p->B, p->Hkv, choice.few, G, choice.rows, 0, p->min_q_len, p->max_q_len,
-                      p->causal ? 1 : 0, 128, 7};
+                      p->causal ? 1 : 0, 192, 7};
   a.q = p->q;
   a.q_ss = p->q_stride[0];
   a.q_sh = p->q_stride[1];
@@ -368,7 +368,7 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStr
   a.bt = paged_batch(p);
   a.half = pg::tc::BM / G;
   a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, int64_t(paged_choice(p).few) * G + 1,
-                      p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 256, 8};
+                      p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 384, 8};
   a.box = std::gcd(p->page_size, pg::tc::BK);
   a.out = p->out;
   a.o_ss = p->o_stride[0];
