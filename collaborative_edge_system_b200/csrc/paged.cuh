@@ -30,9 +30,11 @@ struct Seq {
   int row0, n, len;
 };
 
+constexpr int64_t kMaxLen = 0x7fffff00;  // key indices, rounded up to a tile, stay in 32 bits
+
 __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
   Seq s;
-  const int64_t cap = min(static_cast<int64_t>(bt.max_pages) * bt.ps, int64_t(0x7fffffff));
+  const int64_t cap = min(static_cast<int64_t>(bt.max_pages) * bt.ps, kMaxLen);
   s.row0 = min(max(bt.q_off[b], 0), bt.T);
   s.n = min(max(bt.q_off[b + 1], s.row0), bt.T) - s.row0;
   s.len = static_cast<int>(min(static_cast<int64_t>(max(bt.lens[b], 0)), cap));
@@ -224,7 +226,7 @@ struct SegQueue {
 template <int BK, bool kOne, typename Take>
 __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool dead, Meta* meta, const Take& take) {
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
-  const int64_t cap = static_cast<int64_t>(bt.max_pages) * bt.ps;
+  const int64_t cap = min(static_cast<int64_t>(bt.max_pages) * bt.ps, kMaxLen);
   Share sh;
   SeqUnits s;
   int64_t W = 0, lo = 0, hi = 0, pos = 0;  // the axis, this CTA's share, and where on it the walk is

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <cmath>
 #include <numeric>
 #include <vector>
 
@@ -45,7 +46,7 @@ int paged_validate(const cea_paged_attn_params* p) {
     return fail(CEA_ERR_UNSUPPORTED, "%s: output dtype %d not available for input dtype %d", what, out, in);
   if (p->min_q_len < 0 || p->max_q_len < 0 || p->min_q_len > p->max_q_len)
     return fail(CEA_ERR_INVALID, "%s: new tokens per sequence between %d and %d", what, p->min_q_len, p->max_q_len);
-  if (!(p->scale == p->scale)) return fail(CEA_ERR_INVALID, "%s: scale is not a number", what);
+  if (!std::isfinite(p->scale)) return fail(CEA_ERR_INVALID, "%s: scale is not a finite number", what);
   if (p->B > 0 && p->T > 0 && p->Hq > 0 && p->max_q_len > 0) {
     if (p->q == nullptr || p->out == nullptr) return fail(CEA_ERR_INVALID, "%s: null q or out", what);
     if (p->num_pages > 0 && (p->k_pages == nullptr || p->v_pages == nullptr))
@@ -76,9 +77,9 @@ bool paged_decode_ok(const cea_paged_attn_params* p) {
          ((p->q_stride[0] | p->q_stride[1]) & 1) == 0;
 }
 
-// the chunk kernel reads Q by TMA and stores 16-byte vectors of a row
+// the chunk kernel reads Q by TMA, stores 16-byte vectors of a row, and scales the scores' maximum (not the scores)
 bool paged_tc_ok(const cea_paged_attn_params* p) {
-  if (!paged_tensor_ok(p) || p->Hq / p->Hkv > pg::tc::BM) return false;
+  if (!paged_tensor_ok(p) || p->Hq / p->Hkv > pg::tc::BM || !(static_cast<float>(p->scale) > 0.f)) return false;
   if (!aligned16(p->q) || !aligned16(p->out)) return false;
   const int vec = p->out_dtype == CEA_F32 ? 4 : 8;
   const int size[2] = {p->T, p->Hq};

@@ -28,7 +28,7 @@ def attention(q, k_pages, v_pages, table, lens, offsets, causal=True, scale=None
         v = v_pages[pages.to(v_pages.device)].to(where).double().transpose(1, 2).reshape(-1, H, D)[:n_all]
         k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
         s = torch.einsum("ihd,jhd->hij", q[r0:r1], k) * scale
-        big = torch.einsum("ihd,jhd->hij", q[r0:r1].abs(), k.abs()) * scale
+        big = torch.einsum("ihd,jhd->hij", q[r0:r1].abs(), k.abs()) * abs(scale)
         if causal:
             at = torch.arange(n_all - n, n_all, device=where)
             hidden = torch.arange(n_all, device=where)[None, :] > at[:, None]

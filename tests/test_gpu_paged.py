@@ -89,6 +89,14 @@ def test_accumulation_precision_output_and_scale(dtype, counts):
     assert torch.equal(cea.paged_attention(**x), _check(x))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_that_are_not_positive(dtype, scale):
+    x = R.batch([300, 111, 0, 5], [90, 1, 1, 9], heads=8, kv_heads=2, dim=64, page=16, dtype=TYPES[dtype], device=DEV, seed=5)
+    p = _check(x, scale=scale)
+    assert torch.isfinite(p[:91]).all()
+
+
 @pytest.mark.parametrize("counts", [[1, 1, 1], [100, 37, 64]], ids=["step", "chunk"])
 @pytest.mark.parametrize("case", ["slot_major", "fused_q", "odd_q_base", "odd_pages_base", "layer_slice"])
 def test_strides_and_alignment(case, counts):

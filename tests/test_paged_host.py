@@ -265,7 +265,7 @@ def test_attention_checks_of_the_c_abi():
     assert lib.cea_paged_attn(None, None) == _lib.CEA_ERR_INVALID
     for kw in ({"Hq": 3}, {"Hkv": 0}, {"D": 0}, {"page_size": 0}, {"B": -1}, {"T": -1}, {"q": None}, {"out": None},
                {"k_pages": None}, {"q_offsets": None}, {"page_table": None}, {"seq_lens": None}, {"in_dtype": 9},
-               {"min_q_len": 2}, {"min_q_len": -1}, {"max_q_len": -1}, {"scale": float("nan")}, {"num_pages": -1}):
+               {"min_q_len": 2}, {"min_q_len": -1}, {"max_q_len": -1}, {"scale": float("nan")}, {"scale": float("inf")}, {"num_pages": -1}):
         assert run(**kw) == _lib.CEA_ERR_INVALID, kw
     for kw in ({"D": 257}, {"out_dtype": _lib.F16}, {"in_dtype": _lib.F64, "out_dtype": _lib.F32}):
         assert run(**kw) == _lib.CEA_ERR_UNSUPPORTED, kw
@@ -290,6 +290,9 @@ def test_choice_of_kernels():
     for kw in ({"in_dtype": _lib.F32, "out_dtype": _lib.F32}, {"D": 80}, {"page_size": 12}, {"k_pages": FAKE + 2},
                {"v_stride": (2 * 16 * 128, 16 * 128, 132)}, {"num_pages": 0}):
         assert mask(**kw) == _lib.PAGED_SIMT, kw
+    assert mask(scale=-1.0) == _lib.PAGED_DECODE and mask(scale=0.0, max_q_len=5) == _lib.PAGED_SIMT
+    assert mask(max_q_len=3) == _lib.PAGED_DECODE and mask(min_q_len=3, max_q_len=5) == _lib.PAGED_TC
+    assert mask(Hq=32, max_q_len=1) == _lib.PAGED_DECODE and mask(Hq=32, max_q_len=2) == _lib.PAGED_DECODE | _lib.PAGED_TC
     assert mask(T=0) == 0 and mask(D=0) == -1
 
 
