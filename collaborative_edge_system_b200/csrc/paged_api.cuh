@@ -248,7 +248,7 @@ int launch_paged_simt(const cea_paged_attn_params* p, const PagedPlan& pl, cudaS
   pg::simt::Params<A> a;
   a.bt = paged_batch(p);
   a.dv = pg::Division{p->B, p->Hkv * groups, pg::simt::BQ / group, group, INT64_MAX, 0, p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 16,
-                      pg::simt::Layout<A, DMAX>::BK == 64 ? 6 : 5};
+                      5};
   a.q = p->q;
   a.k = p->k_pages;
   a.v = p->v_pages;

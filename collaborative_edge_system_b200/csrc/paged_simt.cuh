@@ -2,11 +2,11 @@
 // alignment the tensor-core kernels do not take.  Right for every case; the arithmetic is the accumulation type's
 // throughout (probabilities are not rounded).
 //
-// A unit is up to 16 query rows (tokens x query heads of one KV head) against the keys of one sequence, in tiles of 64
-// keys (32 where a row is longer than 256 bytes).  16 threads share two rows, r and r + 8: thread `sub` holds the scores
-// of keys sub + 16 j and groups of 16-byte output columns sub + 16 c of both, so every 16-byte word of K and V that it
-// reads from shared memory feeds two rows (one row a thread was bound by those reads: 44 us at the size below).  Rows
-// are padded by 16 bytes, which keeps the reads free of conflicts.  Online softmax: m' = max(m, max s),
+// A unit is up to 16 query rows (tokens x query heads of one KV head) against the keys of one sequence, in tiles of 32
+// keys.  16 threads share two rows, r and r + 8: thread `sub` holds the scores of keys sub + 16 j and groups of 16-byte
+// output columns sub + 16 c of both, so every 16-byte word of K and V that it reads from shared memory, which bounds the
+// kernel, feeds two rows (one row a thread: 44 us at the size below; tiles of 64 keys, with half the CTAs on an SM: 41;
+// this: 37).  Rows are padded by 16 bytes, which keeps the reads free of conflicts.  Online softmax: m' = max(m, max s),
 // l' = l e^(m - m') + sum e^(s - m'), o' = o e^(m - m') + sum e^(s - m') v.
 // Several threads fetch a key's K and V rows (one page lookup per tile and thread): by cp.async a tile ahead where the
 // rows are aligned and need no conversion, else element by element.  The division of the work over the grid is
@@ -20,7 +20,7 @@ namespace cea {
 namespace paged {
 namespace simt {
 
-constexpr int BQ = 16, TPR = 16, NT = BQ / 2 * TPR;
+constexpr int BQ = 16, BK = 32, TPR = 16, NT = BQ / 2 * TPR;
 
 template <typename A>
 struct Params {
@@ -46,7 +46,6 @@ struct Params {
 
 template <typename A, int DMAX>
 struct Layout {
-  static constexpr int BK = sizeof(A) * DMAX <= 256 ? 64 : 32;
   static constexpr int VN = 16 / sizeof(A);        // elements of a 16-byte word
   static constexpr int LD = DMAX + VN;             // of a row in shared memory
   static constexpr int NST = sizeof(A) * DMAX > 1024 ? 1 : 2;  // fp64 rows of 256: one stage is 133 KB
@@ -78,7 +77,7 @@ __device__ __forceinline__ void cp16(const void* dst, const void* src) {
 template <typename T, typename A, int DMAX>
 __global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params<A> p) {
   using L = Layout<A, DMAX>;
-  constexpr int BK = L::BK, VN = L::VN, KPT = BK / TPR;
+  constexpr int VN = L::VN, KPT = BK / TPR;
   constexpr int NC = (DMAX + VN * TPR - 1) / (VN * TPR);  // output words of a thread and row
   constexpr int FPK = NT / BK;                            // threads that fetch a key
   extern __shared__ __align__(16) uint8_t smem_raw[];
