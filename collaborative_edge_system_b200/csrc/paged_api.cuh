@@ -2,6 +2,7 @@
 // helpers it uses.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <numeric>
@@ -516,18 +517,21 @@ int cea_copy_pages(const cea_copy_pages_params* p, void* stream) {
     return fail(CEA_ERR_INVALID, "%s: negative size", what);
   if (p->n == 0) return CEA_OK;
   if (!p->src || !p->dst) return fail(CEA_ERR_INVALID, "%s: null indices", what);
+  for (int i = 0; i < p->n; ++i)
+    if (p->src[i] < 0 || p->src[i] >= p->num_pages || p->dst[i] < 0 || p->dst[i] >= p->num_pages)
+      return fail(CEA_ERR_INVALID, "%s: pair %d (%d -> %d) outside a pool of %d pages", what, i, p->src[i], p->dst[i],
+                  p->num_pages);
   // every destination once, and none that is also a source: the copies then commute
   try {
-    std::vector<uint8_t> mark(p->num_pages, 0);
-    for (int i = 0; i < p->n; ++i) {
-      if (p->src[i] < 0 || p->src[i] >= p->num_pages || p->dst[i] < 0 || p->dst[i] >= p->num_pages)
-        return fail(CEA_ERR_INVALID, "%s: pair %d (%d -> %d) outside a pool of %d pages", what, i, p->src[i], p->dst[i],
-                    p->num_pages);
-      if (mark[p->dst[i]]) return fail(CEA_ERR_INVALID, "%s: page %d is written twice", what, p->dst[i]);
-      mark[p->dst[i]] = 1;
+    std::vector<int32_t> dst(p->dst, p->dst + p->n), src(p->src, p->src + p->n);
+    std::sort(dst.begin(), dst.end());
+    std::sort(src.begin(), src.end());
+    const auto twice = std::adjacent_find(dst.begin(), dst.end());
+    if (twice != dst.end()) return fail(CEA_ERR_INVALID, "%s: page %d is written twice", what, *twice);
+    for (size_t i = 0, j = 0; i < src.size() && j < dst.size();) {
+      if (src[i] == dst[j]) return fail(CEA_ERR_INVALID, "%s: page %d is both read and written", what, src[i]);
+      if (src[i] < dst[j]) ++i; else ++j;
     }
-    for (int i = 0; i < p->n; ++i)
-      if (mark[p->src[i]]) return fail(CEA_ERR_INVALID, "%s: page %d is both read and written", what, p->src[i]);
   } catch (const std::exception& e) {
     return fail(CEA_ERR_INVALID, "%s: %s", what, e.what());
   }

@@ -6,7 +6,7 @@
 // is read once for all heads that share it.  Q rows (token, head) come from one TMA box of (64, G, 128 / G).
 //   warps 0-3 / 4-7   softmax and epilogue of half 0 / 1: one thread per query row (= TMEM lane)
 //   warp 8 / 10       the K / V ring: 64-key tiles, one TMA box per page (or part of one), one box per lane
-//   warp 9 / 11       MMA issuer of half 0 / 1 (one thread), which also loads its half's Q
+//   warp 9 / 11       MMA issuer of half 0 / 1, which also loads its half's Q
 // Tiles of 64 keys leave room in tensor memory for two S buffers per half (2 x (2 x 64 + D) columns), so an issuer keeps
 // S two tiles ahead of PV: S_h(c + 2) is pushed behind PV_h(c), whose P_h it overwrites, and a half's softmax finds the
 // next scores waiting instead of standing in the chain S -> softmax -> PV.  (With tiles of 128 keys and one buffer, as in
@@ -39,7 +39,7 @@ using cea::tc2::umma_ts;
 constexpr int BM = 128;
 constexpr int BK = 64;
 constexpr int NUM_THREADS = 384;
-constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 10, kMmaWarp1 = 11;
+constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 10;  // warp 11: the second issuer
 constexpr int kLaunchRegs = 168, kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kLaunchRegs * NUM_THREADS, "register split");
 constexpr uint32_t kTmemCols = 512;

@@ -695,7 +695,8 @@ def generate_paged(model: LlamaModel, prompts: Sequence[Sequence[int]], max_new_
             ends = (chosen == eos_token_id).tolist() if eos_token_id is not None else [False] * len(which)
             for row, i in enumerate(which):
                 tokens[i].append(chosen[row : row + 1])
-                scores[i].append(logits[row])
+                if return_scores:
+                    scores[i].append(logits[row])
                 if ends[row] or len(tokens[i]) == max_new_tokens:
                     decoding.pop(i, None)
                     cache.free(live.pop(i))

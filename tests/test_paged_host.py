@@ -325,6 +325,31 @@ def test_append_and_copy_checks_of_the_c_abi():
     assert copy([0], [1], n=-1) == _lib.CEA_ERR_INVALID
 
 
+def test_calls_run_with_their_tensors_device_current(monkeypatch):
+    seen, current = [], [0]
+
+    class Device:
+        def __init__(self, n):
+            self.n = n
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.n
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda n: 1000 + n, raising=False)
+    p = _lib.CopyPagesParams()
+    for device in (0, 3):
+        _lib._on_device(lambda ref, stream: seen.append((current[0], stream)) or 0, p, device, "call")
+    assert seen == [(0, 1000), (3, 1003)] and current == [0]
+    with pytest.raises(RuntimeError, match="call"):
+        _lib._on_device(lambda ref, stream: _lib.CEA_ERR_CUDA, p, 3, "call")
+    assert current == [0]
+
+
 # ------------------------------------------------------------------------------------------------ generation
 class SumModel:
     """Stands for a model: the next token is the sum of the sequence's tokens (read from the cache) modulo 17."""
