@@ -58,8 +58,7 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
             raise ValueError("pages must be contiguous along the head dimension")
 
 
-def _check_batch(page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> Tuple[int, int]:
-    """``(B, max_pages)``"""
+def _check_batch(page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> None:
     i32 = torch.int32
     if page_table.dtype != i32 or seq_lens.dtype != i32 or q_offsets.dtype != i32:
         raise ValueError("page_table, seq_lens and q_offsets must be int32")
@@ -71,7 +70,21 @@ def _check_batch(page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: to
         if (lens[0] > 1 and seq_lens.stride(0) != 1) or (lens[0] > 0 and q_offsets.stride(0) != 1) or (
                 table[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table rows, seq_lens and q_offsets must be contiguous")
-    return lens[0], table[1]
+
+
+def _checked(k_pages, v_pages, page_table, seq_lens, q_offsets):
+    """Pages' shape and strides, ``B``, ``max_pages`` and the table's row stride, all checked (what is as usual at once,
+    the rest by the functions above)."""
+    i32 = torch.int32
+    pages, kp, vp = k_pages.shape, k_pages.stride(), v_pages.stride()
+    table, ts, (B,) = page_table.shape, page_table.stride(), seq_lens.shape[:1] or (0,)
+    if not (len(pages) == 4 and pages == v_pages.shape and k_pages.dtype == v_pages.dtype and kp[3] == 1 and vp[3] == 1):
+        _check_pages(k_pages, v_pages)
+    if not (page_table.dtype == i32 and seq_lens.dtype == i32 and q_offsets.dtype == i32 and len(table) == 2
+            and table[0] == B and ts[1] == 1 and seq_lens.stride() == (1,) and q_offsets.stride() == (1,)
+            and q_offsets.shape[0] == B + 1):
+        _check_batch(page_table, seq_lens, q_offsets)
+    return pages, kp, vp, B, table[1], ts[0]
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -81,39 +94,35 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     Two tokens with one place (a page that two of the batch's sequences write) leave either's row there.
     """
     dev = _lib.device_number(k, v, k_pages, v_pages, page_table, seq_lens, q_offsets)
-    _check_pages(k_pages, v_pages)
-    B, width = _check_batch(page_table, seq_lens, q_offsets)
-    P, H, ps, D = k_pages.shape
-    shape = k.shape
+    pages, kp, vp, B, width, table = _checked(k_pages, v_pages, page_table, seq_lens, q_offsets)
+    P, H, ps, D = pages
+    shape, ks, vs = k.shape, k.stride(), v.stride()
     if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [T, {H}, {D}]")
     if k.dtype != k_pages.dtype or v.dtype != v_pages.dtype:
         raise ValueError("k, v and the pages must share a dtype")
-    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
     if D > 1 and (ks[2] != 1 or vs[2] != 1):
         raise ValueError("k and v must be contiguous along the head dimension")
     _lib.paged_append(_lib.PagedAppendParams.from_buffer_copy(_lib.PAGED_APPEND_RECORD.pack(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_offsets.data_ptr(), seq_lens.data_ptr(),
-        page_table.data_ptr(), ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2],
-        page_table.stride(0), B, shape[0], H, D, ps, P, width, k.element_size())), dev)
+        page_table.data_ptr(), ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], table, B, shape[0],
+        H, D, ps, P, width, k.element_size())), dev)
 
 
 _TAIL = bytes(ctypes.sizeof(_lib.PagedAttnParams) - _lib.PAGED_ATTN_RECORD.size)  # the workspace's fields
 
 
 def _attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse, min_q_len, max_q_len, causal, scale):
-    _check_pages(k_pages, v_pages)
-    B, width = _check_batch(page_table, seq_lens, q_offsets)
-    shape, dtype = q.shape, q.dtype
+    pages, kp, vp, B, width, table = _checked(k_pages, v_pages, page_table, seq_lens, q_offsets)
+    shape, dtype, qs, os = q.shape, q.dtype, q.stride(), out.stride()
     if len(shape) != 3 or dtype != k_pages.dtype:
         raise ValueError(f"q must be [T, Hq, D] of the pages' dtype, got {tuple(shape)} of {dtype}")
     T, Hq, D = shape
-    P, H, ps, Dk = k_pages.shape
+    P, H, ps, Dk = pages
     if Dk != D:
         raise ValueError(f"q {tuple(shape)} and the pages {tuple(k_pages.shape)} disagree on the head dim")
     if out.shape != shape or (lse is not None and (lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] != T)):
         raise ValueError(f"out must be {tuple(shape)} and lse [{Hq}, {T}]")
-    qs, os, kp, vp = q.stride(), out.stride(), k_pages.stride(), v_pages.stride()
     if D > 1 and (qs[2] != 1 or os[2] != 1):
         raise ValueError("q and out must be contiguous along the head dimension")
     if lse is None:
@@ -125,7 +134,7 @@ def _attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse,
     return _lib.PagedAttnParams.from_buffer_copy(_lib.PAGED_ATTN_RECORD.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, q_offsets.data_ptr(),
         seq_lens.data_ptr(), page_table.data_ptr(), qs[0], qs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], os[0], os[1],
-        l0, l1, page_table.stride(0), B, T, Hq, H, D, ps, P, width, min_q_len, T if max_q_len is None else max_q_len,
+        l0, l1, table, B, T, Hq, H, D, ps, P, width, min_q_len, T if max_q_len is None else max_q_len,
         1.0 / math.sqrt(D) if scale is None else scale, bool(causal), _lib.dtype_code(dtype),
         _lib.dtype_code(out.dtype)) + _TAIL)
 

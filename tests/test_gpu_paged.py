@@ -89,6 +89,16 @@ def test_accumulation_precision_output_and_scale(dtype, counts):
     assert torch.equal(cea.paged_attention(**x), _check(x))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(128, 1, 64, 16), (160, 1, 128, 8), (130, 2, 64, 1), (64, 64, 64, 32),
+                                                     (51, 17, 128, 64), (16, 1, 128, 16), (27, 3, 64, 8)])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 0, 3], [70, 1, 9]], ids=["step", "few", "mixed"])
+def test_head_groups_from_one_to_all(heads, kv_heads, dim, page, counts):
+    x = R.batch([150, 77, 260], counts, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=torch.bfloat16,
+                device=DEV, seed=heads)
+    _check(x, max_q_len=max(counts))
+    _check(x, causal=False)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("scale", [0.0, -0.2])
 def test_scales_that_are_not_positive(dtype, scale):
@@ -254,6 +264,56 @@ def test_captured_graph_serves_changing_batches(counts):
         assert torch.equal(out, again)
         R.check(out, None, ref, dtype=torch.bfloat16, out_dtype=torch.bfloat16, single_p=True)
     _lib.device_status(clear=True)  # positions before a short sequence's start were reported by the append
+
+
+def test_graph_of_a_whole_step_over_layers():
+    """Append and attention of several layers in one graph, replayed while lengths grow: the tokens of every step."""
+    L, H, D, ps, B = 3, 2, 64, 8, 4
+    cache = cea.PagedKVCache(L, 40, ps, H, D, dtype=torch.bfloat16, device=DEV)
+    seqs = [cache.add() for _ in range(B)]
+    first = cache.extend(seqs, [9, 1, 30, 16])
+    k0 = torch.randn(L, first.num_tokens, H, D, device=DEV).to(torch.bfloat16)
+    for layer in range(L):
+        cache.append(layer, k0[layer], k0[layer], first)
+    table = torch.zeros(B, 10, dtype=torch.int32, device=DEV)
+    lens, offs = torch.zeros(B, dtype=torch.int32, device=DEV), torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    q, k, v = (torch.zeros(L, B, h, D, dtype=torch.bfloat16, device=DEV) for h in (8, H, H))
+    out = torch.zeros_like(q)
+
+    def step():
+        for layer in range(L):
+            cea.paged_append(k[layer], v[layer], cache.k[layer], cache.v[layer], table, lens, offs)
+            cea.paged_attend_into(q[layer], cache.k[layer], cache.v[layer], table, lens, offs, out[layer], min_q_len=1,
+                                  max_q_len=1)
+
+    batch = cache.extend(seqs, [1] * B)
+    table[:, : batch.page_table.shape[1]] = batch.page_table
+    lens.copy_(batch.seq_lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(12):
+        if turn:
+            batch = cache.extend(seqs, [1] * B)
+            table.zero_()
+            table[:, : batch.page_table.shape[1]] = batch.page_table
+            lens.copy_(batch.seq_lens)
+        for t in (q, k, v):
+            t.normal_()
+        graph.replay()
+        for layer in range(L):
+            ref = R.attention(q[layer], cache.k[layer], cache.v[layer], table, lens, offs)
+            R.check(out[layer], None, ref, dtype=torch.bfloat16, out_dtype=torch.bfloat16, single_p=False)
+        pos = lens.long() - 1
+        at = table.long()[torch.arange(B, device=DEV), pos // ps]
+        assert torch.equal(cache.k[:, at, :, pos % ps], k.transpose(0, 1)) and torch.equal(
+            cache.v[:, at, :, pos % ps], v.transpose(0, 1))
+    assert _lib.device_status(clear=True) == 0
 
 
 def test_two_streams_at_once():
