@@ -9,6 +9,7 @@
 #pragma once
 
 #include "cea_common.cuh"
+#include "kv_cache.cuh"
 
 // First bad page or batch descriptor seen by a paged kernel; unlike g_cea_status it stops no later kernel.
 __device__ int g_cea_paged_status;
@@ -551,7 +552,8 @@ struct AppendArgs {
   uint8_t* dst[2];         // pages
   int64_t src_ss[2], src_sh[2];           // bytes: token, head
   int64_t dst_sp[2], dst_sh[2], dst_ss[2];  // bytes: page, head, slot
-  int H, units;            // units of U bytes per head row
+  int H;
+  kvc::FastDiv units;      // units of U bytes per head row
 };
 
 // sequence of row t: the last b with q_off[b] <= t (offsets ascend; empty sequences are passed over), -1 if none
@@ -574,9 +576,17 @@ constexpr int kAppendThreads = 128;
 constexpr int kAppendUnroll = 4;
 
 template <typename U>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   const int lane = threadIdx.x & 31;
-  const int per = a.H * a.units;  // units of one token's K (or V)
+  const int per = a.H * static_cast<int>(a.units.d);  // units of one token's K (or V)
+  // head and byte offset of this lane's units, the same for every token
+  int head[kAppendUnroll], byte[kAppendUnroll];
+  auto place = [&](int i, int& h, int& at) {
+    h = static_cast<int>(kvc::fdiv(i, a.units));
+    at = (i - h * static_cast<int>(a.units.d)) * static_cast<int>(sizeof(U));
+  };
+#pragma unroll
+  for (int j = 0; j < kAppendUnroll; ++j) place(j * 32 + lane, head[j], byte[j]);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int stride = gridDim.x * (kAppendThreads / 32);
   for (int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); t < a.bt.T; t += stride) {
@@ -584,17 +594,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int j = 0; j < kAppendUnroll; ++j) {
-        const int i = j * 32 + lane;
-        if (i < per)
-          val[x][j] = *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + (i / a.units) * a.src_sh[x] +
-                                                  static_cast<int64_t>(i % a.units) * sizeof(U));
-      }
+      for (int j = 0; j < kAppendUnroll; ++j)
+        if (j * 32 + lane < per)
+          val[x][j] = *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + head[j] * a.src_sh[x] + byte[j]);
     const int b = find_seq(a.bt, t, lane);
     if (b < 0 || b >= a.bt.B) continue;  // before the first or behind the last sequence
     const Seq s = load_seq(a.bt, b);
     const int64_t pos = static_cast<int64_t>(a.bt.lens[b]) - s.n + (t - s.row0);
-    const int64_t page_i = pos >= 0 ? pos / a.bt.ps : -1;
+    const int64_t page_i = pos < 0                ? -1
+                           : (pos >> 32) == 0 ? static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.bt.ps)
+                                              : pos / a.bt.ps;
     const int page = page_i >= 0 && page_i < a.bt.max_pages ? a.bt.table[b * a.bt.table_sb + page_i] : -1;
     if (page < 0 || page >= a.bt.num_pages) {
       if (lane == 0) report(CEA_DEV_BAD_PAGE);
@@ -605,16 +614,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     for (int x = 0; x < 2; ++x) {
       uint8_t* dst = a.dst[x] + page * a.dst_sp[x] + slot * a.dst_ss[x];
 #pragma unroll
-      for (int j = 0; j < kAppendUnroll; ++j) {
-        const int i = j * 32 + lane;
-        if (i < per)
-          *reinterpret_cast<U*>(dst + (i / a.units) * a.dst_sh[x] + static_cast<int64_t>(i % a.units) * sizeof(U)) =
-              val[x][j];
+      for (int j = 0; j < kAppendUnroll; ++j)
+        if (j * 32 + lane < per) *reinterpret_cast<U*>(dst + head[j] * a.dst_sh[x] + byte[j]) = val[x][j];
+      for (int i = kAppendUnroll * 32 + lane; i < per; i += 32) {  // rows longer than the loads in flight
+        int h, at;
+        place(i, h, at);
+        *reinterpret_cast<U*>(dst + h * a.dst_sh[x] + at) =
+            *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + h * a.src_sh[x] + at);
       }
-      for (int i = kAppendUnroll * 32 + lane; i < per; i += 32)
-        *reinterpret_cast<U*>(dst + (i / a.units) * a.dst_sh[x] + static_cast<int64_t>(i % a.units) * sizeof(U)) =
-            *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + (i / a.units) * a.src_sh[x] +
-                                        static_cast<int64_t>(i % a.units) * sizeof(U));
     }
   }
 }

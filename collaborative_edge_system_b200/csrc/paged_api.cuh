@@ -497,7 +497,7 @@ int cea_paged_append(const cea_paged_append_params* p, void* stream) {
   a.H = p->H;
   const int64_t units = static_cast<int64_t>(p->D) * eb / unit;
   if (units * p->H > 0x7fffffff) return fail(CEA_ERR_UNSUPPORTED, "%s: %d heads of %d elements", what, p->H, p->D);
-  a.units = static_cast<int>(units);
+  a.units = cea::kvc::make_fastdiv(static_cast<uint32_t>(units));
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (unit) {
