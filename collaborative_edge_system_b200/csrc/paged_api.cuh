@@ -94,8 +94,17 @@ bool paged_tc_ok(const cea_paged_attn_params* p) {
 
 // Which kernels serve a call.  Sequences of up to `few` new tokens go through the decode kernel, which is compiled for 8
 // or 16 query rows per KV head; the others through the chunk kernel.  A kernel is launched only if the promised
-// numbers of new tokens allow a sequence for it.  16 rows serve a call whose sequences all fit them; where chunks come
-// too, sequences of 9 to 16 rows join those, as the 16-row form costs every single token of the batch.
+// numbers of new tokens allow a sequence for it.  Times in us, bf16, 32 query and 8 KV heads where nothing else is said.
+// - 9 to 16 rows at D = 128, if no sequence of the call can have fewer: the chunk kernel, which pads them to a tile that
+//   the tensor cores take in their stride, while the 16-row form holds twice the accumulators.  Chunk kernel and 16-row
+//   form: 35 and 44 (8 sequences of 4096, 4 tokens each), 103 and 110 (32 of them), 40 and 60 (64 of 300 to 600),
+//   36 and 44 (32 of 4096, one token, groups of 16), 15 and 17 (one of those).
+// - 9 to 16 rows at D = 64: the 16-row form, 71 against 86 (32 of 4096, 4 tokens), 29 against 31 (groups of 16).
+// - up to 16 rows, some of them perhaps 8 or fewer: the 16-row form alone, 38 against 43 and 91 against 94 for the 8-row
+//   form with the chunk kernel after it (8 and 32 of 2000 to 4096, 1 to 4 tokens).
+// - where longer chunks come too: the 8-row form, and sequences of 9 to 16 rows join the chunks; the 16-row form costs
+//   every single token of the batch: 98 against 110 (18 single tokens and two chunks of 389, up to 6000 keys).
+// - up to 8 rows: the 8-row form, 44 against 58 for the 16-row form (64 of 600 to 900, one token).
 struct PagedChoice {
   int kernels;
   int rows;  // query rows of the decode kernel: 8 or 16
@@ -106,7 +115,8 @@ PagedChoice paged_choice(const cea_paged_attn_params* p) {
   PagedChoice c = {0, 8, 0};
   if (p->B == 0 || p->T == 0 || p->Hq == 0 || p->max_q_len == 0) return c;
   const int64_t G = p->Hq / p->Hkv, most = p->max_q_len * G;
-  c.rows = most <= 8 || (most > pg::dec::ROWS && G <= 8) ? 8 : pg::dec::ROWS;
+  const bool wide = p->D == 128 && std::max(p->min_q_len, 1) * G > 8 && paged_tc_ok(p);
+  c.rows = most <= 8 || (most > pg::dec::ROWS && G <= 8) || wide ? 8 : pg::dec::ROWS;
   c.few = static_cast<int>(c.rows / G);
   const bool few = std::max(p->min_q_len, 1) <= c.few, many = p->max_q_len > c.few;
   if ((!few || paged_decode_ok(p)) && (!many || paged_tc_ok(p)))

@@ -2,13 +2,13 @@
 // a decoding step and of a few proposed tokens.
 //
 // HBM-bound: K and V are read once, about 4 FLOP per byte at a group of 4 query heads.  One CTA per SM takes an
-// equal share of all key tiles of the batch (paged.cuh), so lengths may differ at will and no CTA idles; four
-// warps stream 64-key K and V tiles into a ring of 192 KB with TMA, one box per page (or part of one) and 64 columns,
-// each lane looking its box's page up; a warp takes about 60 ns a box and 0.5 us a tile, so four take the tiles in turn
-// (one warp for all of them: 2.8 TB/s at pages of 8 and 4.5 at 16; the boxes of each tile dealt to four warps: 5.3 and
-// 6.1, and 3.8 at D = 64; the tiles in turn: 6.5 and 6.5, and 6.0 at D = 64; 32 sequences of 16384, 8 KV heads);
-// the ring runs on across the segments of a share, so the loads do not
-// pause while the consumer warps join their results.  Two groups of four consumer warps take the tiles in turn, each
+// equal share of all key tiles of the batch (paged.cuh), so lengths may differ at will and no CTA idles.  Three
+// producer warps stream 64-key K and V tiles into a ring of 192 KB with TMA, one box per page (or part of one) and 64
+// columns, each lane looking its box's page up; a warp takes about 60 ns a box and 0.5 us a tile, so the warps take the
+// tiles in turn (one warp for all of them: 2.8 TB/s at pages of 8 and 4.5 at 16; the boxes of each tile dealt to four
+// warps: 5.3 and 6.1, and 3.8 at D = 64; the tiles in turn: 6.5 and 6.5, and 6.0 at D = 64; 32 sequences of 16384, 8 KV
+// heads).  A fourth warp finds the segments of the share ahead of the loads; the ring runs on across them, so the loads
+// do not pause while the consumer warps join their results.  Two groups of four consumer warps take the tiles in turn, each
 // warp 16 keys, transposed on mma.sync m16n8k16 so that the keys (and then the columns of V) fill the 16 rows and the few
 // query rows the 8 columns: S^T = K Q^T, online softmax in the log2 domain down the columns, O^T += V^T P^T.  With
 // the query rows on the 16-row side instead, half of each product was padding at 4 or 8 rows.  P is carried as the

@@ -147,8 +147,8 @@ def paged_attend_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     dtype) and, if given, ``lse`` ``[Hq, T]`` (accumulation dtype).
 
     ``min_q_len`` and ``max_q_len`` bound the number of new tokens of the sequences that have any; they choose the
-    kernels and are promises (0 and ``None`` always hold): decoding sequences (at most 16 query rows per KV head) and
-    chunks of prompts have a kernel each, and a batch that cannot hold one kind does not launch its kernel.
+    kernels and are promises (0 and ``None`` always hold): decoding sequences (up to 8 or 16 query rows per KV head)
+    and chunks of prompts have a kernel each, and a batch that cannot hold one kind does not launch its kernel.
     """
     if lse is None:
         _lib.device_number(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out)

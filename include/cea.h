@@ -354,9 +354,9 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * behind a sequence's length are never used, whatever they hold.  out_dtype is
  * the input dtype or F32 (F64 for F64); lse is F32 (F64 for F64).
  * min_q_len / max_q_len bound the n_b > 0 of the batch and choose the kernels
- * (0 and T are always right): sequences with n_b * Hq / Hkv <= 16 go through the
- * split decode kernel, others through the tcgen05 kernel, each where it applies
- * (bf16 / f16, D in {64, 128}, page_size a multiple of 8, 16-byte aligned rows);
+ * (0 and T are always right): sequences with n_b * Hq / Hkv <= 8 go through the
+ * split decode kernel, those with more than 16 through the tcgen05 kernel, those
+ * between through either, as measured; each where it applies (bf16 / f16, D in {64, 128}, page_size a multiple of 8, 16-byte aligned rows);
  * everything else through the CUDA-core kernel.  cea_paged_attn_kernels returns
  * the kernels of a call as a mask: 1 tcgen05, 2 split decode, 4 CUDA cores.
  */

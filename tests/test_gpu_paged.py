@@ -179,6 +179,30 @@ def test_broken_promises_are_reported():
         assert _lib.device_status(clear=True) == 0
 
 
+@pytest.mark.parametrize("lens,counts", [([1000, 9, 64], [3, 4, 3]), ([5000], [4]), ([300, 0, 65, 3, 700], [4, 0, 3, 3, 4])],
+                         ids=["ragged", "one", "empty"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [("bf16", 32, 8, 128, 16), ("f16", 12, 4, 128, 8),
+                                                           ("bf16", 8, 2, 64, 16)])
+def test_nine_to_sixteen_rows_with_and_without_the_promise(dtype, heads, kv_heads, dim, page, lens, counts, causal):
+    # at 128 columns the promise that no sequence has fewer rows changes the kernel
+    x = R.batch(lens, counts, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=TYPES[dtype], device=DEV,
+                seed=len(lens) * 3 + dim, extra_rows=2)
+    promised, open_ = dict(min_q_len=3, max_q_len=4), dict(max_q_len=4)
+    assert _kernels(x, **promised) == (_lib.PAGED_TC if dim == 128 else _lib.PAGED_DECODE)
+    assert _kernels(x, **open_) == _lib.PAGED_DECODE
+    _check(x, causal=causal, **promised)
+    _check(x, causal=causal, **open_)
+    _check(x, causal=causal, scale=-0.1, **promised)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_single_tokens_of_wide_groups_among_chunks(dim):
+    for lens, counts in (([700, 64, 1], [1, 1, 1]), ([700, 90, 33, 1], [1, 70, 2, 1])):
+        x = R.batch(lens, counts, heads=24, kv_heads=2, dim=dim, page=16, dtype=torch.bfloat16, device=DEV, seed=dim)
+        _check(x, max_q_len=max(counts))
+
+
 @pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 16)])
 def test_more_sequences_than_threads(dtype, dim):
     lens = [(i * 37) % 90 for i in range(1500)]

@@ -292,7 +292,14 @@ def test_choice_of_kernels():
         assert mask(**kw) == _lib.PAGED_SIMT, kw
     assert mask(scale=-1.0) == _lib.PAGED_DECODE and mask(scale=0.0, max_q_len=5) == _lib.PAGED_SIMT
     assert mask(max_q_len=3) == _lib.PAGED_DECODE and mask(min_q_len=3, max_q_len=5) == _lib.PAGED_TC
-    assert mask(Hq=32, max_q_len=1) == _lib.PAGED_DECODE and mask(Hq=32, max_q_len=2) == _lib.PAGED_DECODE | _lib.PAGED_TC
+    # 9 to 16 rows: the chunk kernel at 128 columns if no sequence may have fewer, as it wins there
+    assert mask(min_q_len=3, max_q_len=4) == _lib.PAGED_TC and mask(min_q_len=2, max_q_len=4) == _lib.PAGED_DECODE
+    assert mask(min_q_len=3, max_q_len=4, scale=-1.0) == _lib.PAGED_DECODE
+    assert mask(Hq=32, max_q_len=1) == _lib.PAGED_TC and mask(Hq=32, max_q_len=2) == _lib.PAGED_TC
+    assert mask(Hq=32, max_q_len=1, scale=-1.0) == _lib.PAGED_DECODE
+    narrow = {"D": 64, "k_stride": (2 * 16 * 64, 16 * 64, 64), "v_stride": (2 * 16 * 64, 16 * 64, 64)}
+    assert mask(min_q_len=3, max_q_len=4, **narrow) == _lib.PAGED_DECODE
+    assert mask(Hq=32, max_q_len=2, **narrow) == _lib.PAGED_DECODE | _lib.PAGED_TC
     assert mask(T=0) == 0 and mask(D=0) == -1
 
 
