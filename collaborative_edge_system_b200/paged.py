@@ -134,7 +134,8 @@ def _attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse,
     return _lib.PagedAttnParams.from_buffer_copy(_lib.PAGED_ATTN_RECORD.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, q_offsets.data_ptr(),
         seq_lens.data_ptr(), page_table.data_ptr(), qs[0], qs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], os[0], os[1],
-        l0, l1, table, B, T, Hq, H, D, ps, P, width, min_q_len, T if max_q_len is None else max_q_len,
+        l0, l1, table, B, T, Hq, H, D, ps, P, width, min_q_len,
+        max(T, min_q_len) if max_q_len is None else max_q_len,
         1.0 / math.sqrt(D) if scale is None else scale, bool(causal), _lib.dtype_code(dtype),
         _lib.dtype_code(out.dtype)) + _TAIL)
 

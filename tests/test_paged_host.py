@@ -196,6 +196,14 @@ def test_attention_arguments(anywhere):
     assert not anywhere
 
 
+def test_promise_of_the_least_number_holds_for_an_empty_pass(anywhere):
+    x = _good()
+    x["q"], x["q_offsets"] = x["q"][:0], torch.zeros(3, dtype=torch.int32)
+    cea.paged_attention(**x, min_q_len=1)  # says nothing of sequences without new tokens
+    p = anywhere.pop()
+    assert p.T == 0 and p.min_q_len <= p.max_q_len
+
+
 def test_append_arguments(anywhere):
     x = _good()
     x.pop("q")
