@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from operator import index
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -196,7 +197,7 @@ def _host_indices(x: Indices) -> torch.Tensor:
         if x.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"page indices must be whole numbers, got {x.dtype}")
     else:
-        x = torch.tensor([int(i) for i in x], dtype=torch.int64)
+        x = torch.tensor([index(i) for i in x], dtype=torch.int64)
     if x.dtype == torch.int64:
         if x.numel() and (int(x.min()) < 0 or int(x.max()) >= 1 << 31):
             raise ValueError("page index out of range")
@@ -388,7 +389,7 @@ class PagedKVCache:
         """``count`` new sequences that begin with the first ``length`` tokens of ``seq`` (all of them by default).
 
         Full pages are shared; a partly filled last page is copied for each fork, in all layers by one launch."""
-        n = self.length(seq) if length is None else int(length)
+        n = self.length(seq) if length is None else index(length)
         if n < 0 or n > self.length(seq):
             raise ValueError(f"{n} tokens of a sequence that has {self.length(seq)}")
         if count < 0:
@@ -413,6 +414,7 @@ class PagedKVCache:
 
     def truncate(self, seq: int, length: int) -> None:
         """Keep the first ``length`` tokens (rejected proposals leave, their pages become free)."""
+        length = index(length)
         if length < 0 or length > self.length(seq):
             raise ValueError(f"{length} tokens of a sequence that has {self.length(seq)}")
         keep = -(-length // self.page_size)
@@ -438,7 +440,7 @@ class PagedKVCache:
         A partly filled last page that another sequence shares (after :meth:`truncate`) is copied first, so that no
         sequence ever writes what another one reads.  Raises :class:`OutOfPages` and changes nothing when the pool
         does not have the pages."""
-        seqs, counts = list(seqs), [int(c) for c in counts]
+        seqs, counts = list(seqs), [index(c) for c in counts]
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError("extend takes each sequence once, with a count >= 0 for each")
         ps = self.page_size

@@ -231,6 +231,19 @@ def test_copy_arguments(anywhere):
     assert not anywhere
 
 
+def test_fractions_are_refused(anywhere):
+    k = torch.zeros(3, 5, 2, 4, 8)
+    with pytest.raises(TypeError):
+        cea.copy_pages(k, k, [0.5], [1])
+    c = HostCache(1, 4, 4, 1, 2)
+    s = c.add()
+    c.extend([s], [3])
+    for call in (lambda: c.extend([s], [1.5]), lambda: c.fork(s, 2.5), lambda: c.truncate(s, 2.5)):
+        with pytest.raises(TypeError):
+            call()
+    assert c.length(s) == 3 and c.num_free_pages == 3 and not anywhere
+
+
 # ------------------------------------------------------------------------------------------------ C ABI
 def test_records_have_the_layout_of_the_structs():
     for record, cls in ((_lib.PAGED_ATTN_RECORD, _lib.PagedAttnParams), (_lib.PAGED_APPEND_RECORD, _lib.PagedAppendParams)):
