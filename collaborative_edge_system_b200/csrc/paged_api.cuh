@@ -398,7 +398,13 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStr
       !paged_map(&mv, p, p->v_pages, p->v_stride, a.box))
     return fail(CEA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the queries or the pages");
   cudaError_t err = cudaSuccess;
-#define CEA_PTC(DD, BF)                                                                                    do {                                                                                                       auto k = pg::tc::chunk_kernel<DD, BF>;                                                                   if (int e = check_launch_regs(reinterpret_cast<const void*>(k), pg::tc::kLaunchRegs)) return e;          allow_smem(k, pg::tc::Layout<DD>::SMEM_ALLOC);                                                           k<<<pl.grid, pg::tc::NUM_THREADS, pg::tc::Layout<DD>::SMEM_ALLOC, s>>>(mq, mk, mv, a);                 } while (0)
+#define CEA_PTC(DD, BF)                                                                               \
+  do {                                                                                                \
+    auto k = pg::tc::chunk_kernel<DD, BF>;                                                            \
+    if (int e = check_launch_regs(reinterpret_cast<const void*>(k), pg::tc::kLaunchRegs)) return e;   \
+    allow_smem(k, pg::tc::Layout<DD>::SMEM_ALLOC);                                                    \
+    err = launch_dependent(k, dim3(pl.grid), pg::tc::NUM_THREADS, pg::tc::Layout<DD>::SMEM_ALLOC, s, mq, mk, mv, a); \
+  } while (0)
   const bool bf = p->in_dtype == CEA_BF16;
   if (p->D == 128) {
     if (bf) CEA_PTC(128, true); else CEA_PTC(128, false);
