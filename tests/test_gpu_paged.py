@@ -340,6 +340,30 @@ def test_graph_of_a_whole_step_over_layers():
     assert _lib.device_status(clear=True) == 0
 
 
+def test_calls_of_all_kernels_one_after_another():
+    """Launches overlap the end of the one before: nothing may be read or written before it is through."""
+    kinds = [([900, 64, 5000], [300, 64, 17]), ([700, 65, 3], [1, 1, 1]), ([3000, 40], [4, 3]), ([600, 900], [1, 120])]
+    xs = [R.batch(lens, counts, heads=32, kv_heads=8, dim=128, page=16, dtype=torch.bfloat16, device=DEV, seed=i)
+          for i, (lens, counts) in enumerate(kinds)]
+    alone = []
+    for x in xs:
+        alone.append(cea.paged_attention(**x))
+        torch.cuda.synchronize()
+    pages = [(torch.empty_like(x["k_pages"]), torch.empty_like(x["v_pages"])) for x in xs]
+    for _ in range(100):
+        outs = []
+        for x, (k, v) in zip(xs, pages):
+            # pages filled, read and spoilt again by neighbours in the stream
+            k.copy_(x["k_pages"])
+            v.copy_(x["v_pages"])
+            outs.append(cea.paged_attention(**{**x, "k_pages": k, "v_pages": v}))
+            k.fill_(float("nan"))
+            v.fill_(float("nan"))
+        for a, b in zip(outs, alone):
+            assert torch.equal(a, b)
+    assert _lib.device_status(True) == 0
+
+
 def test_two_streams_at_once():
     xs = [R.batch([700 + 50 * i, 90], [1, 40], heads=8, kv_heads=2, dim=64, page=16, dtype=torch.bfloat16, device=DEV,
                   seed=20 + i) for i in range(4)]
