@@ -210,14 +210,10 @@ struct SegQueue {
   // segment i, by a whole warp; false at the end of the share or after a timeout
   __device__ __forceinline__ bool get(int i, Seg& g, int lane) const {
     const bool ok = __all_sync(0xffffffffu, read(i, g));
+    // all lanes' reads come before lane 0's release of the slot: a vote orders no memory, this does
+    __syncwarp();
     if (ok && lane == 0) mbar_arrive(empty + 8 * (i % kQueue));
     return ok && g.b >= 0;
-  }
-  // the same by one thread
-  __device__ __forceinline__ bool get1(int i, Seg& g) const {
-    if (!read(i, g)) return false;
-    mbar_arrive(empty + 8 * (i % kQueue));
-    return g.b >= 0;
   }
 };
 

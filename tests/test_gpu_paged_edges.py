@@ -1,0 +1,38 @@
+"""Calls of the paged operators at the edges of what they allow: extreme weights and values, batches that do not fit, the
+state after a device-side timeout."""
+
+import math
+
+import pytest
+import torch
+
+import collaborative_edge_system_b200 as cea
+import paged_ref as R
+from collaborative_edge_system_b200 import _lib, paged
+
+pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
+DEV = torch.device("cuda", 0) if torch.cuda.is_available() else None
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "f64": torch.float64}
+
+
+def _kernels(x, **kw):
+    p = paged._attn_params(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"],
+                           torch.empty_like(x["q"]), None, kw.get("min_q_len", 0), kw.get("max_q_len"),
+                           kw.get("causal", True), kw.get("scale"))
+    return _lib.paged_attn_kernels(p)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,n", [("bf16", 16, 8, 64, 1), ("f16", 32, 8, 128, 4), ("bf16", 16, 8, 128, 19),
+                                                        ("f16", 8, 8, 64, 70)])
+def test_hundreds_of_short_segments_in_every_share(dtype, heads, kv_heads, dim, n):
+    """The queue between the warp that walks a share and the others turns over many times, with segments of one tile
+    whose readers keep up at different speeds."""
+    lens = [n + (i * 7) % 41 for i in range(2500)]
+    x = R.batch(lens, [n - i % 2 * (n > 1) for i in range(2500)], heads=heads, kv_heads=kv_heads, dim=dim, page=8,
+                dtype=TYPES[dtype], device=DEV, seed=n)
+    out = cea.paged_attention(**x, max_q_len=n)
+    for _ in range(30):
+        assert torch.equal(cea.paged_attention(**x, max_q_len=n), out)
+    ref = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"], where=DEV)
+    R.check(out, None, ref, dtype=TYPES[dtype], out_dtype=TYPES[dtype], single_p=bool(_kernels(x, max_q_len=n) & _lib.PAGED_TC))
+    assert _lib.device_status(clear=True) == 0
