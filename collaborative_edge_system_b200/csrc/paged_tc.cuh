@@ -476,33 +476,36 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_ld32(tO + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
         tmem_ld32(tO + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
         tmem_wait_ld();
-        if (!row_in) continue;
+        if (row_in) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv_l);
-        auto f = [&](int e) { return __uint_as_float(o[e]); };
-        if (slot >= 0) {
+          for (int e = 0; e < 64; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv_l);
+          auto f = [&](int e) { return __uint_as_float(o[e]); };
+          if (slot >= 0) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 4)
-            part[((c + e) / 4) * kWideRows] = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
-        } else if (p.out_dtype == CEA_F32) {
-          float* dst = reinterpret_cast<float*>(p.out) + obase + c;
+            for (int e = 0; e < 64; e += 4)
+              part[((c + e) / 4) * kWideRows] = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
+          } else if (p.out_dtype == CEA_F32) {
+            float* dst = reinterpret_cast<float*>(p.out) + obase + c;
 #pragma unroll
-          for (int e = 0; e < 64; e += 4)
-            *reinterpret_cast<float4*>(dst + e) = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
-        } else {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + obase + c;
+            for (int e = 0; e < 64; e += 4)
+              *reinterpret_cast<float4*>(dst + e) = make_float4(f(e), f(e + 1), f(e + 2), f(e + 3));
+          } else {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + obase + c;
 #pragma unroll
-          for (int e = 0; e < 64; e += 8)
-            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack2(f(e), f(e + 1), kBF16), pack2(f(e + 2), f(e + 3), kBF16),
-                                                            pack2(f(e + 4), f(e + 5), kBF16),
-                                                            pack2(f(e + 6), f(e + 7), kBF16));
+            for (int e = 0; e < 64; e += 8)
+              *reinterpret_cast<uint4*>(dst + e) = make_uint4(
+                  pack2(f(e), f(e + 1), kBF16), pack2(f(e + 2), f(e + 3), kBF16), pack2(f(e + 4), f(e + 5), kBF16),
+                  pack2(f(e + 6), f(e + 7), kBF16));
+          }
         }
+        __syncwarp();  // the next tcgen05.ld is for all lanes of the warp together
       }
       tc_fence_before();
       if (row_in) {
         if (slot >= 0) p.part_lse[static_cast<int64_t>(slot) * kWideRows + prow] = lse_row;
         else if (p.lse != nullptr) p.lse[head * p.l_sh + trow * p.l_ss] = lse_row;
       }
+      __syncwarp();
     }
   }
 

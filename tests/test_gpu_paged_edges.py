@@ -36,3 +36,22 @@ def test_hundreds_of_short_segments_in_every_share(dtype, heads, kv_heads, dim, 
     ref = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"], where=DEV)
     R.check(out, None, ref, dtype=TYPES[dtype], out_dtype=TYPES[dtype], single_p=bool(_kernels(x, max_q_len=n) & _lib.PAGED_TC))
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (15, 5, 128), (5, 1, 64), (14, 2, 128)])
+def test_warps_of_the_chunk_kernel_with_rows_of_no_token(heads, kv_heads, dim, out_dtype):
+    """Groups that do not divide a tile and chunks that end within a warp's rows, whole and split over the GPU: lanes
+    without a token stay in step with those that have one."""
+    lens, counts = [17, 40, 300, 9000, 129], [17, 33, 50, 21, 129]
+    x = R.batch(lens, counts, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=torch.bfloat16, device=DEV, seed=heads,
+                extra_rows=1)
+    ref = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"])
+    assert _kernels(x, min_q_len=17) == _lib.PAGED_TC
+    for _ in range(5):
+        out = torch.full(x["q"].shape, 77.0, dtype=out_dtype, device=DEV)
+        lse = torch.full((heads, out.shape[0]), 77.0, device=DEV)
+        cea.paged_attend_into(**x, out=out, lse=lse, min_q_len=17)
+        R.check(out, lse, ref, dtype=torch.bfloat16, out_dtype=out_dtype, single_p=True)
+        assert (out[-1] == 77.0).all() and (lse[:, -1] == 77.0).all()
+    assert _lib.device_status(clear=True) == 0
