@@ -31,7 +31,7 @@ struct Seq {
   int row0, n, len;
 };
 
-constexpr int64_t kMaxLen = 0x7fffff00;  // key indices, rounded up to a tile, stay in 32 bits
+constexpr int64_t kMaxLen = 0x7fffff00;  // key indices, rounded up to a tile, stay in 32 bits (places on the axis: 64)
 
 __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
   Seq s;
@@ -77,6 +77,12 @@ __device__ __forceinline__ int64_t units_before(const SeqUnits& s, int i, const 
   return s.n0 + m * s.ctx + static_cast<int64_t>(dv.tb) * (m * (2ll * s.n0 + m + 1) / 2) + cost;
 }
 
+// A unit's length on the axis.  In 64 bits: the keys alone may fill 31, and a length that came out negative would send
+// the walk back without end.
+__device__ __forceinline__ int64_t unit_span(int keys, const Division& dv) {
+  return static_cast<int64_t>(max(1, keys)) + dv.cost;
+}
+
 // keys that block i reads (its last token's view)
 __device__ __forceinline__ int unit_keys(const SeqUnits& s, int i, int tb, bool causal) {
   if (!causal) return s.len;
@@ -95,7 +101,7 @@ __device__ __forceinline__ SeqUnits seq_units(const Division& dv, const Seq& q) 
     s.nb = q.n > 0 && q.n <= dv.tb ? 1 : 0;
     s.n0 = 0;
     s.ctx = q.len - q.n;
-    s.S = s.nb * (max(1, q.len) + dv.cost);
+    s.S = s.nb * unit_span(q.len, dv);
     return s;
   }
   const int64_t rows = static_cast<int64_t>(q.n) * dv.group;
@@ -103,7 +109,7 @@ __device__ __forceinline__ SeqUnits seq_units(const Division& dv, const Seq& q) 
   s.ctx = q.len - q.n;  // may be negative: the first tokens then see nothing
   s.n0 = s.ctx < 0 ? min(static_cast<int>((-static_cast<int64_t>(s.ctx)) / dv.tb), max(s.nb - 1, 0)) : 0;
   s.S = s.nb == 0 ? 0
-                  : units_before(s, s.nb - 1, dv) + max(1, unit_keys(s, s.nb - 1, dv.tb, dv.causal)) + dv.cost;
+                  : units_before(s, s.nb - 1, dv) + unit_span(unit_keys(s, s.nb - 1, dv.tb, dv.causal), dv);
   return s;
 }
 
@@ -132,7 +138,7 @@ struct Share {
 __device__ __forceinline__ int block_at(const SeqUnits& s, int64_t r, const Division& dv) {
   int i;
   if (!dv.causal) {
-    i = static_cast<int>(div64(r, max(1, s.len) + dv.cost));
+    i = static_cast<int>(div64(r, unit_span(s.len, dv)));
   } else {
     const int64_t r0 = static_cast<int64_t>(s.n0) * (1 + dv.cost);
     if (r < r0) {
@@ -301,7 +307,7 @@ __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool d
         if (!ok) break;
         it += t1 - t0;
       }
-      pos += max(1, keys) + dv.cost;
+      pos += unit_span(keys, dv);
       if (!kOne && ++blk < s.nb) continue;
       blk = 0;
       if (++hu < dv.units_h) continue;

@@ -55,3 +55,31 @@ def test_warps_of_the_chunk_kernel_with_rows_of_no_token(heads, kv_heads, dim, o
         R.check(out, lse, ref, dtype=torch.bfloat16, out_dtype=out_dtype, single_p=True)
         assert (out[-1] == 77.0).all() and (lse[:, -1] == 77.0).all()
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+@pytest.mark.parametrize("dtype,n,kernel", [("f16", 40, _lib.PAGED_TC), ("bf16", 1, _lib.PAGED_DECODE), ("f32", 1, _lib.PAGED_SIMT)])
+def test_the_longest_sequence(dtype, n, kernel, causal):
+    """2^31 - 256 keys, one page under every entry of the table: a unit's keys and its cost are above 31 bits.
+
+    All scores are 0 and the values 0 or 1, so every sum of a share (below 2^24) is exact; what is left are the
+    statistics of the parts, off by three roundings of ln 2^24 at most, and their weights in the join."""
+    page, D, total = 65536, 64, 2**31 - 256
+    slot = torch.arange(page)[:, None] * torch.arange(1, D + 1)[None, :]
+    ones = (slot % 5 == 0).long()
+    x = {"q": torch.zeros(n, 1, D, dtype=TYPES[dtype], device=DEV),
+         "k_pages": torch.randn(1, 1, page, D, device=DEV).to(TYPES[dtype]),
+         "v_pages": ones.to(TYPES[dtype]).to(DEV)[None, None],
+         "page_table": torch.zeros(1, 2**31 // page, dtype=torch.int32, device=DEV),
+         "seq_lens": torch.tensor([total], dtype=torch.int32, device=DEV),
+         "q_offsets": torch.tensor([0, n], dtype=torch.int32, device=DEV)}
+    kw = {"min_q_len": n, "max_q_len": n, "causal": causal}
+    assert _kernels(x, **kw) == kernel
+    out, lse = cea.paged_attention_with_lse(**x, **kw)
+    seen = torch.arange(total - n + 1, total + 1) if causal else torch.full((n,), total)
+    ahead = torch.cat([torch.zeros(1, D, dtype=torch.long), ones.cumsum(0)])
+    want = (seen // page)[:, None] * ahead[-1] + ahead[seen % page]
+    bound = 2 * 3 * math.log(2**24) * 2.0**-24 + 2.0**-20
+    assert float((out[:, 0].double().cpu() / (want / seen[:, None].double()) - 1).abs().max()) <= bound
+    assert float((lse[0].double().cpu() - seen.double().log()).abs().max()) <= bound + math.log(2**31) * 2.0**-23
+    assert _lib.device_status(clear=True) == 0
