@@ -590,8 +590,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 #pragma unroll
   for (int j = 0; j < kAppendUnroll; ++j) place(j * 32 + lane, head[j], byte[j]);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int stride = gridDim.x * (kAppendThreads / 32);
-  for (int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); t < a.bt.T; t += stride) {
+  const unsigned stride = gridDim.x * (kAppendThreads / 32);
+  // unsigned: a stride behind the last of 2^31 - 1 rows is above an int
+  for (unsigned row = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); row < static_cast<unsigned>(a.bt.T);
+       row += stride) {
+    const int t = static_cast<int>(row);
     U val[2][kAppendUnroll];
 #pragma unroll
     for (int x = 0; x < 2; ++x)

@@ -83,3 +83,16 @@ def test_the_longest_sequence(dtype, n, kernel, causal):
     assert float((out[:, 0].double().cpu() / (want / seen[:, None].double()) - 1).abs().max()) <= bound
     assert float((lse[0].double().cpu() - seen.double().log()).abs().max()) <= bound + math.log(2**31) * 2.0**-23
     assert _lib.device_status(clear=True) == 0
+
+
+def test_append_of_as_many_rows_as_32_bits_count():
+    """Three rows of two sequences and 2^31 - 4 of none behind them, of a byte each."""
+    k = torch.zeros(2**31 - 1, 1, 1, dtype=torch.uint8, device=DEV)
+    k[:3, 0, 0] = torch.tensor([7, 8, 9], dtype=torch.uint8)
+    k_pages, v_pages = (torch.full((3, 1, 4, 1), 1, dtype=torch.uint8, device=DEV) for _ in range(2))
+    cea.paged_append(k, k, k_pages, v_pages, torch.tensor([[2, -1], [0, 1]], dtype=torch.int32, device=DEV),
+                     torch.tensor([4, 5], dtype=torch.int32, device=DEV), torch.tensor([0, 2, 3], dtype=torch.int32, device=DEV))
+    want = torch.full((3, 4), 1, dtype=torch.uint8)
+    want[2, 2], want[2, 3], want[1, 0] = 7, 8, 9
+    assert torch.equal(k_pages.view(3, 4).cpu(), want) and torch.equal(v_pages.view(3, 4).cpu(), want)
+    assert _lib.device_status(clear=True) == 0
