@@ -173,6 +173,23 @@ struct Meta {
   int hu, blk, row0, n;
 };
 
+// Wait, by a whole warp at the end of its part, for copies or products that it started: a CTA that gives up after a
+// timeout must not leave them running into memory that it has given back.  Bounded as the other waits are, but not cut
+// short by a sibling's abort.  Without a timeout all of it has long been waited for.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+    if ((n & 63u) != 0u) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > CEA_WAIT_LIMIT_NS) {
+      record_error(code);
+      break;
+    }
+  }
+  __syncwarp();
+}
+
 // The segments of a share pass from the one warp that walks them to the others through a short queue in shared
 // memory, so that the walk (64-bit positions) is done once and ahead of its use.
 constexpr int kQueue = 8;

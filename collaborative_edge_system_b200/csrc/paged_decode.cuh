@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t dst0 = is_v * L::TILE + half * L::BOX + box * p.box * 128;
     const int none = p.bt.num_pages;
     bool ok = true;
+    int last = -1;  // tile loaded last
     for (int i = 0; ok && queue.get(i, g, lane); ++i) {
       const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
       for (int t = g.t0 + (warp - NCW + NPW - g.it % NPW) % NPW; t < g.t1; t += NPW) {
@@ -168,8 +169,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (lane == 0) mbar_arrive_expect_tx(bar(L::B_FULL + st), boxes * p.box * 128);
         __syncwarp();
         if (load) tma_load_4d(sbase + st * L::STAGE + dst0, map, bar(L::B_FULL + st), half * 64, slot, g.hu, page);
+        last = at;
       }
     }
+    // the last load of each of this warp's stages
+    for (int at = last; at >= 0 && at > last - L::NSTAGE; at -= NPW)
+      drain(bar(L::B_FULL + at % L::NSTAGE), (at / L::NSTAGE) & 1, CEA_DEV_TIMEOUT_DECODE);
     return;
   }
 

@@ -71,7 +71,8 @@ struct Layout {
   static constexpr int B_SFULL = B_VTAIL + 1;
   static constexpr int B_PFULL = B_SFULL + 4;
   static constexpr int B_PVDONE = B_PFULL + 4;
-  static constexpr int B_QUEUE = B_PVDONE + 4;
+  static constexpr int B_DRAIN = B_PVDONE + 4;  // x2 (per half): all products are done
+  static constexpr int B_QUEUE = B_DRAIN + 2;
   static constexpr int NBAR = B_QUEUE + SegQueue::kBars;
   static constexpr int OFF_QUEUE = (OFF_BAR + NBAR * 8 + 15) / 16 * 16;
   static constexpr int OFF_MISC = OFF_QUEUE + SegQueue::kBytes;
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h) {
       mbar_init(bar(L::B_QFULL + h), 1);
+      mbar_init(bar(L::B_DRAIN + h), 1);
       for (int b = 0; b < 2; ++b) {
         mbar_init(bar(L::B_SFULL + 2 * h + b), 1);
         mbar_init(bar(L::B_PFULL + 2 * h + b), 4);  // one arrival per softmax warp
@@ -188,6 +190,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int box = lane % nbox, col = lane / nbox;
       const bool mine = col < L::KBOX;
       uint32_t tails = 0;
+      int loaded = 0;          // tiles whose full barrier completes by itself
+      bool tail_open = false;  // a tail was loaded and not waited for
       auto load_tiles = [&](const Seg& g) -> bool {
         const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
         for (int t = g.t0; t < g.t1; ++t) {
@@ -216,8 +220,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           __syncwarp();
           if (load) tma_load_4d(to + col * L::BOX + box * p.box * 128, map, fb, col * 64, slot, g.hu, page);
           if (tail) {
+            tail_open = true;
             if (!wait_all(bar(L::B_VTAIL), tails & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER)) return false;
             ++tails;
+            tail_open = false;
             uint8_t* tile = smem + L::OFF_V + st * L::TILE;
             for (int i = max(left, 0) * 8 + lane; i < BK * 8; i += 32)
 #pragma unroll
@@ -227,6 +233,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(b_full + st));
           }
+          loaded = u + 1;
         }
         return true;
       };
@@ -242,6 +249,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         while (queue.get(i++, g, lane))
           if (!load_tiles(g)) break;
       }
+      for (int u = max(0, loaded - nst); u < loaded; ++u)
+        drain(bar(b_full + u % nst), (u / nst) & 1, CEA_DEV_TIMEOUT_PRODUCER);
+      if (tail_open) drain(bar(L::B_VTAIL), tails & 1, CEA_DEV_TIMEOUT_PRODUCER);
     } else {
       // ---------------------------------------------------------- MMA issuer of half h: one elected thread, the warp in step
       const int h = warp == kMmaWarp ? 0 : 1;
@@ -262,6 +272,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint32_t pending = 0;             // tiles whose PV is to come, two bits each, the oldest low: 1 computed, 2 first
       int npend = 0;
       bool any = false, ok = true;
+      bool q_open = false;              // Q_h was loaded and not waited for
       auto issue_pv = [&]() -> bool {
         if (!wait_all(bar(L::B_VFULL) + 8 * vs, vph, abort_flag, CEA_DEV_TIMEOUT_MMA)) return false;
         if (pending & 1u) {
@@ -308,6 +319,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                           g.row0 + tok, 0);
           }
           __syncwarp();
+          q_open = true;
         }
         for (int t = t0; t < t1; ++t) {
           // S runs two tiles ahead of PV; S(c + 2) follows PV(c) in this thread's order, hence overwrites P(c) behind it
@@ -317,6 +329,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (t == t0) {
               if (!(ok = wait_all(b_q, qph, abort_flag, CEA_DEV_TIMEOUT_MMA))) break;
               qph ^= 1u;
+              q_open = false;
             }
             tc_fence_after();
             const uint64_t kdesc = kdesc0 + static_cast<uint64_t>((ks * L::TILE) >> 4);
@@ -342,6 +355,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       while (ok && npend > 0) ok = issue_pv();
+      if (q_open) drain(b_q, qph, CEA_DEV_TIMEOUT_MMA);
+      if (elect_one()) umma_commit(bar(L::B_DRAIN + h));
+      __syncwarp();
+      drain(bar(L::B_DRAIN + h), 0, CEA_DEV_TIMEOUT_MMA);
     }
   } else {
     // ================================================================ softmax + epilogue

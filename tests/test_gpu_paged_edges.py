@@ -96,3 +96,35 @@ def test_append_of_as_many_rows_as_32_bits_count():
     want[2, 2], want[2, 3], want[1, 0] = 7, 8, 9
     assert torch.equal(k_pages.view(3, 4).cpu(), want) and torch.equal(v_pages.view(3, 4).cpu(), want)
     assert _lib.device_status(clear=True) == 0
+
+
+def _time_out():
+    """A bounded wait on a flag that nothing sets: the exchange of two ranks of which one never comes."""
+    bufs = [torch.zeros(2 * 2 * 4 * 8, device=DEV) for _ in range(2)]
+    flags = [torch.zeros(2, dtype=torch.int64, device=DEV) for _ in range(2)]
+    out = torch.zeros(1, 1, 4, 4, device=DEV)
+    _lib.peer_merge(2, 0, [b.data_ptr() for b in bufs], [f.data_ptr() for f in flags], 1, 8, out, wait_limit_ns=1_000_000)
+    torch.cuda.synchronize()
+    assert _lib.device_status(clear=False) == _lib.DEV_TIMEOUT_PEER and out.isnan().all()
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [60, 1, 20]], ids=["step", "mixed"])
+def test_attention_computes_nothing_after_a_timeout(dtype, dim, counts):
+    x = R.batch([3000, 40, 500], counts, heads=8, kv_heads=2, dim=dim, page=16, dtype=TYPES[dtype], device=DEV, seed=23)
+    before = cea.paged_attention(**x)
+    _time_out()
+    try:
+        out = torch.full_like(before, 77.0)
+        lse = torch.full((8, out.shape[0]), 77.0, dtype=paged.accumulation_dtype(out.dtype), device=DEV)
+        cea.paged_attend_into(**x, out=out, lse=lse)
+        assert (out == 77.0).all() and (lse == 77.0).all()
+        # data movement depends on no wait and goes on
+        k = torch.randn(out.shape[0], 2, dim, device=DEV).to(TYPES[dtype])
+        copy = {n: x[n].clone() for n in ("k_pages", "v_pages")}
+        cea.paged_append(k, k, **copy, page_table=x["page_table"], seq_lens=x["seq_lens"], q_offsets=x["q_offsets"])
+        assert torch.equal(copy["k_pages"][int(x["page_table"][2, 499 // 16]), :, 499 % 16], k[-1])
+    finally:
+        assert _lib.device_status(clear=True) == _lib.DEV_TIMEOUT_PEER
+    assert torch.equal(cea.paged_attention(**x), before)
+    assert _lib.device_status(clear=True) == 0
