@@ -93,9 +93,10 @@ __global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params
   asm volatile("griddepcontrol.launch_dependents;");
   // columns behind D stay zero in every row
   for (int i = threadIdx.x; i < L::ELEMS; i += NT) qs[i] = 0;
-  __syncthreads();
+  // after a device-side timeout nothing is computed (one thread asks, as all warps must agree)
+  const bool dead = __syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&g_cea_status) != 0);
 
-  walk<BK, false>(p.bt, p.dv, false, p.meta, [&](const Seg& g) -> bool {  // every warp alike
+  walk<BK, false>(p.bt, p.dv, dead, p.meta, [&](const Seg& g) -> bool {  // every warp alike
     if (g.b < 0) return true;
     const int kvh = g.hu / p.head_groups, g0 = (g.hu % p.head_groups) * p.dv.group;
     int64_t row[2];

@@ -344,7 +344,9 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * table entry outside [0, num_pages) reads as zeros and is not written
  * (CEA_DEV_BAD_PAGE); descending offsets, a length that the table cannot hold
  * (it is cut) or a sequence with a number of new tokens outside [min_q_len,
- * max_q_len] (its rows are undefined) is CEA_DEV_BAD_BATCH.
+ * max_q_len] (its rows are undefined) is CEA_DEV_BAD_BATCH.  After a device-side
+ * timeout (CEA_DEV_TIMEOUT_*), until cea_device_status clears it, cea_paged_attn
+ * leaves out and lse as they are; append and copy, which wait for nothing, go on.
  *
  * cea_paged_attn: attention of the new tokens (n_b from 0 on, single tokens
  * included) over the cached ones; token i sees the keys at positions up to

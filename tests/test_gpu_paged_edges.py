@@ -108,7 +108,8 @@ def _time_out():
     assert _lib.device_status(clear=False) == _lib.DEV_TIMEOUT_PEER and out.isnan().all()
 
 
-@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("bf16", 64), ("f16", 128), ("f32", 64), ("f64", 64),
+                                       ("bf16", 80)])
 @pytest.mark.parametrize("counts", [[1, 1, 1], [60, 1, 20]], ids=["step", "mixed"])
 def test_attention_computes_nothing_after_a_timeout(dtype, dim, counts):
     x = R.batch([3000, 40, 500], counts, heads=8, kv_heads=2, dim=dim, page=16, dtype=TYPES[dtype], device=DEV, seed=23)
