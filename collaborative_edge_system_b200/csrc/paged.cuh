@@ -565,6 +565,8 @@ __global__ void __launch_bounds__(kCombineThreads) combine_wide_kernel(const __g
 // New token rows into their pages, bit for bit: one warp per token moves its K and its V rows.  Bound by HBM for
 // prompts and by latency for a decoding step, so the loads of the rows are issued before the walk from the token to
 // its page (sequence by a 32-way search of the offsets, then the table) and stored after it.
+// A row's position is counted back from its sequence's length and end, so rows that the caller's k and v lack change no
+// other row's place.  One block more than the rows need looks at all offsets and reports a batch that does not fit.
 struct AppendArgs {
   Batch bt;
   const uint8_t* src[2];   // k, v
@@ -607,7 +609,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 #pragma unroll
   for (int j = 0; j < kAppendUnroll; ++j) place(j * 32 + lane, head[j], byte[j]);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const unsigned stride = gridDim.x * (kAppendThreads / 32);
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int b = threadIdx.x; b < a.bt.B; b += kAppendThreads) {
+      const int o0 = a.bt.q_off[b], o1 = a.bt.q_off[b + 1];
+      if (o0 < 0 || o1 < o0 || o1 > a.bt.T) report(CEA_DEV_BAD_BATCH);
+    }
+    return;
+  }
+  const unsigned stride = (gridDim.x - 1) * (kAppendThreads / 32);
   // unsigned: a stride behind the last of 2^31 - 1 rows is above an int
   for (unsigned row = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5); row < static_cast<unsigned>(a.bt.T);
        row += stride) {
@@ -621,8 +630,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
           val[x][j] = *reinterpret_cast<const U*>(a.src[x] + t * a.src_ss[x] + head[j] * a.src_sh[x] + byte[j]);
     const int b = find_seq(a.bt, t, lane);
     if (b < 0 || b >= a.bt.B) continue;  // before the first or behind the last sequence
-    const Seq s = load_seq(a.bt, b);
-    const int64_t pos = static_cast<int64_t>(a.bt.lens[b]) - s.n + (t - s.row0);
+    const int64_t pos = static_cast<int64_t>(a.bt.lens[b]) - a.bt.q_off[b + 1] + t;
+    if (t >= a.bt.q_off[b + 1]) continue;  // offsets that descend
     const int64_t page_i = pos < 0                ? -1
                            : (pos >> 32) == 0 ? static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.bt.ps)
                                               : pos / a.bt.ps;

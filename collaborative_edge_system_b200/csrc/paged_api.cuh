@@ -427,7 +427,8 @@ size_t paged_workspace(const cea_paged_attn_params* p, int kernels) {
 template <typename U>
 cudaError_t launch_append(const pg::AppendArgs& a, cudaStream_t s) {
   constexpr int per = pg::kAppendThreads / 32;
-  const int grid = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(a.bt.T) + per - 1) / per, 148 * 16));
+  // and a block that checks the offsets
+  const int grid = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(a.bt.T) + per - 1) / per, 148 * 16)) + 1;
   return launch_dependent(pg::append_kernel<U>, dim3(grid), pg::kAppendThreads, 0, s, a);
 }
 

@@ -393,7 +393,10 @@ int cea_paged_attn_kernels(const cea_paged_attn_params* p);
 /*
  * cea_paged_append: the rows of k / v [T, H, D] (element strides token, head; D
  * contiguous) into their pages, bit for bit (any dtype of 1, 2, 4 or 8 bytes), at
- * the positions described above.
+ * the positions described above.  A token behind the table, before the sequence's
+ * start or without a page is dropped (CEA_DEV_BAD_PAGE); offsets that descend or go
+ * behind T are reported (CEA_DEV_BAD_BATCH), and the rows that are there go to the
+ * places they would have in the whole batch.
  */
 typedef struct cea_paged_append_params {
   const void* k;

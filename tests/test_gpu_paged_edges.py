@@ -129,3 +129,32 @@ def test_attention_computes_nothing_after_a_timeout(dtype, dim, counts):
         assert _lib.device_status(clear=True) == _lib.DEV_TIMEOUT_PEER
     assert torch.equal(cea.paged_attention(**x), before)
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("rows", [3, 7, 9, 12])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_append_of_fewer_rows_than_the_batch_has(dtype, rows):
+    """The rows that are there go to their own places, and the batch is reported."""
+    assert _lib.device_status(clear=True) == 0
+    x = R.batch([10, 20, 9], [5, 4, 3], heads=2, kv_heads=2, dim=16, page=4, dtype=dtype, device=DEV, seed=21, poison=False)
+    k = torch.randn(rows, 2, 16, device=DEV).to(dtype)
+    want = x["k_pages"].clone()
+    places = [(0, p) for p in range(5, 10)] + [(1, p) for p in range(16, 20)] + [(2, p) for p in range(6, 9)]
+    for row, (b, p) in enumerate(places[:rows]):
+        want[int(x["page_table"][b, p // 4]), :, p % 4] = k[row]
+    cea.paged_append(k, k, x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"])
+    assert torch.equal(x["k_pages"], want)
+    assert _lib.device_status(clear=True) == (0 if rows == 12 else _lib.DEV_BAD_BATCH)
+
+
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [-4, 1, 5, 9], [0, 5, 9, 400], [0, 2**31 - 1, 9, 9]])
+def test_append_reports_offsets_that_do_not_fit(offsets):
+    assert _lib.device_status(clear=True) == 0
+    x = R.batch([400, 400, 400], [1, 1, 1], heads=2, kv_heads=2, dim=16, page=4, dtype=torch.bfloat16, device=DEV, seed=22)
+    k = torch.randn(9, 2, 16, device=DEV).to(torch.bfloat16)
+    cea.paged_append(k, k, x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"],
+                     torch.tensor(offsets, dtype=torch.int32, device=DEV))
+    assert _lib.device_status(clear=True) in (_lib.DEV_BAD_BATCH, _lib.DEV_BAD_PAGE)
+    fine = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV)
+    cea.paged_append(k, k, x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], fine)
+    assert _lib.device_status(clear=True) == 0
