@@ -29,6 +29,7 @@ struct Batch {
 
 struct Seq {
   int row0, n, len;
+  int ctx;  // position of row0's token; may be negative: the first tokens then see nothing
 };
 
 constexpr int64_t kMaxLen = 0x7fffff00;  // key indices, rounded up to a tile, stay in 32 bits (places on the axis: 64)
@@ -39,6 +40,8 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
   s.row0 = min(max(bt.q_off[b], 0), bt.T);
   s.n = min(max(bt.q_off[b + 1], s.row0), bt.T) - s.row0;
   s.len = static_cast<int>(min(static_cast<int64_t>(max(bt.lens[b], 0)), cap));
+  // counted back from the sequence's end, which may lie behind T: the rows that are there keep their positions
+  s.ctx = s.n > 0 ? s.len - (bt.q_off[b + 1] - s.row0) : s.len;
   return s;
 }
 
@@ -100,13 +103,13 @@ __device__ __forceinline__ SeqUnits seq_units(const Division& dv, const Seq& q) 
   if constexpr (kOne) {
     s.nb = q.n > 0 && q.n <= dv.tb ? 1 : 0;
     s.n0 = 0;
-    s.ctx = q.len - q.n;
+    s.ctx = q.ctx;
     s.S = s.nb * unit_span(q.len, dv);
     return s;
   }
   const int64_t rows = static_cast<int64_t>(q.n) * dv.group;
   s.nb = q.n > 0 && rows >= dv.min_rows && rows <= dv.max_rows ? (q.n + dv.tb - 1) / dv.tb : 0;
-  s.ctx = q.len - q.n;  // may be negative: the first tokens then see nothing
+  s.ctx = q.ctx;
   s.n0 = s.ctx < 0 ? min(static_cast<int>((-static_cast<int64_t>(s.ctx)) / dv.tb), max(s.nb - 1, 0)) : 0;
   s.S = s.nb == 0 ? 0
                   : units_before(s, s.nb - 1, dv) + unit_span(unit_keys(s, s.nb - 1, dv.tb, dv.causal), dv);
@@ -252,7 +255,7 @@ __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool d
   int64_t W = 0, lo = 0, hi = 0, pos = 0;  // the axis, this CTA's share, and where on it the walk is
   int b = dv.B;                            // sequence at lo
   // the axis's length, then the sequence that holds lo: 32 sequences at a time, one a lane
-  Seq q = {0, 0, 0};
+  Seq q = {0, 0, 0, 0};
   int64_t w = 0, end = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
@@ -260,7 +263,7 @@ __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool d
 #pragma unroll 1
     for (int b0 = 0; b0 < dv.B; b0 += 32) {
       if (pass == 0 || dv.B > 32) {
-        q = Seq{0, 0, 0};
+        q = Seq{0, 0, 0, 0};
         if (b0 + lane < dv.B) {
           q = load_seq(bt, b0 + lane);
           // a length that the table cannot hold, descending offsets, or a broken promise
@@ -282,7 +285,7 @@ __device__ __forceinline__ void walk(const Batch& bt, const Division& dv, bool d
           b = b0 + l;
           pos = before + __shfl_sync(0xffffffffu, end - w, l);
           q = Seq{__shfl_sync(0xffffffffu, q.row0, l), __shfl_sync(0xffffffffu, q.n, l),
-                  __shfl_sync(0xffffffffu, q.len, l)};
+                  __shfl_sync(0xffffffffu, q.len, l), __shfl_sync(0xffffffffu, q.ctx, l)};
           break;
         }
       }

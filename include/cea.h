@@ -342,9 +342,10 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * belong to no sequence are left as they were.  What does not fit is bounded on the
  * device and reported through cea_device_status (it stops no later kernel): a
  * table entry outside [0, num_pages) reads as zeros and is not written
- * (CEA_DEV_BAD_PAGE); descending offsets, a length that the table cannot hold
- * (it is cut) or a sequence with a number of new tokens outside [min_q_len,
- * max_q_len] (its rows are undefined) is CEA_DEV_BAD_BATCH.  After a device-side
+ * (CEA_DEV_BAD_PAGE); offsets that descend or go behind T (the rows that are there
+ * keep their positions), a length that the table cannot hold (it is cut) or a
+ * sequence with a number of new tokens outside [min_q_len, max_q_len] (its rows are
+ * undefined) is CEA_DEV_BAD_BATCH.  After a device-side
  * timeout (CEA_DEV_TIMEOUT_*), until cea_device_status clears it, cea_paged_attn
  * leaves out and lse as they are; append and copy, which wait for nothing, go on.
  *

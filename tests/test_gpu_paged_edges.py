@@ -158,3 +158,18 @@ def test_append_reports_offsets_that_do_not_fit(offsets):
     fine = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV)
     cea.paged_append(k, k, x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], fine)
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 2, 24, 30])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("f32", 64)])
+def test_attention_of_fewer_rows_than_the_batch_has(dtype, dim, rows):
+    """The rows that are there keep their positions, and the batch is reported."""
+    assert _lib.device_status(clear=True) == 0
+    x = R.batch([700, 90, 33], [2, 60, 1], heads=8, kv_heads=4, dim=dim, page=16, dtype=TYPES[dtype], device=DEV, seed=24)
+    ref = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"])
+    x["q"] = x["q"][:rows]
+    assert _kernels(x) == (_lib.PAGED_SIMT if dtype == "f32" else _lib.PAGED_DECODE | (_lib.PAGED_TC if rows > 4 else 0))
+    out, lse = cea.paged_attention_with_lse(**x)
+    assert _lib.device_status(clear=True) == _lib.DEV_BAD_BATCH
+    R.check(out, lse, (ref[0][:rows], ref[1][:, :rows], ref[2][:rows], ref[3][:, :rows]), dtype=TYPES[dtype],
+            out_dtype=torch.float32, single_p=True)
