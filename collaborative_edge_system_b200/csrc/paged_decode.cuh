@@ -12,8 +12,11 @@
 // warp 16 keys, transposed on mma.sync m16n8k16 so that the keys (and then the columns of V) fill the 16 rows and the few
 // query rows the 8 columns: S^T = K Q^T, online softmax in the log2 domain down the columns, O^T += V^T P^T.  With
 // the query rows on the 16-row side instead, half of each product was padding at 4 or 8 rows.  P is carried as the
-// sum of two 16-bit numbers (the value's rounding and the rounding of what that leaves, 2^-17 of the value for bf16),
-// which doubles the PV products and makes the result as exact as fp32 probabilities.  TMA boxes behind the last
+// sum of two 16-bit numbers (the value's rounding and the rounding of what that leaves), which doubles the PV products:
+// what is lost is 2^-17 of a probability in bf16, and in f16 2^-22 of it or 2^-39 of the row's largest.  In f16 numbers
+// below 2^-14 lose bits and those below 2^-25 are 0, so the probabilities there are held as 2^14 times their ratio to the
+// running maximum (at most 2^14, of 65504); held with the maximum at 1, keys 17 to 18 nats below one that outweighs them
+// counted in the sum and not in the output.  TMA boxes behind the last
 // key are not loaded, and the V fragments of keys behind it are zeroed in registers, so slots that hold no token never
 // count, whatever they hold.
 #pragma once
@@ -81,6 +84,10 @@ struct Params {
   int out_dtype;
   float scale_log2;
 };
+
+// log2 of the probability that a row's running maximum is given
+template <bool kBF16>
+constexpr float kTopLog2 = kBF16 ? 0.f : 14.f;
 
 template <bool kBF16>
 __device__ __forceinline__ float round16(float x) {
@@ -262,11 +269,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float nm = fmaxf(m[nt][e], top[e]);
-            const float u = nm == -INFINITY ? 0.f : nm;
+            const float u = nm == -INFINITY ? 0.f : nm, u1 = u - kTopLog2<kBF16>;
             alpha[e] = fast_exp2(m[nt][e] - u);
             m[nt][e] = nm;
-            x[e] = fast_exp2(x[e] - u);
-            x[2 + e] = fast_exp2(x[2 + e] - u);
+            x[e] = fast_exp2(x[e] - u1);
+            x[2 + e] = fast_exp2(x[2 + e] - u1);
             l[nt][e] = l[nt][e] * alpha[e] + x[e] + x[2 + e];
           }
 #pragma unroll
@@ -364,8 +371,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           v[2] += w0 * f.z;
           v[3] += w1 * f.w;
         }
-        lse[0] = sum[0] == 0.f ? -INFINITY : (u0 + log2f(sum[0])) * kLn2;
-        lse[1] = sum[1] == 0.f ? -INFINITY : (u1 + log2f(sum[1])) * kLn2;
+        lse[0] = sum[0] == 0.f ? -INFINITY : (u0 + (log2f(sum[0]) - kTopLog2<kBF16>)) * kLn2;
+        lse[1] = sum[1] == 0.f ? -INFINITY : (u1 + (log2f(sum[1]) - kTopLog2<kBF16>)) * kLn2;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + c2 + e;

@@ -17,8 +17,10 @@
 // A row sees keys 0 .. limit; only tiles that reach behind the first token's limit are masked, with one compare per key.
 // Slots behind the unit's last key are not loaded or hold anything: their scores are masked, and their V rows are zeroed
 // in shared memory before the tile is released to the MMA (a probability of 0 does not silence a NaN).
-// P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16, independent per key), the sum is of the
-// unrounded fp32 values; S, statistics and O are fp32.
+// P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16 and 2^-11 for f16, independent per key),
+// the sum is of the unrounded fp32 values; S, statistics and O are fp32.  f16 numbers below 2^-14 lose bits and those below
+// 2^-25 are 0, so there P is 2^7 times the probability's ratio to its row's reference (at most 2^15 of 65504: the reference
+// may be 2^8 below the maximum): a key counts down to 2^-32 of the largest.
 // Measured (bf16, 32/8 heads of 128, pages of 16, GPU time): 4096 new tokens on 36864, 1.9 to 2.0 ms, 1165 to 1225
 // TFLOP/s with the clock pulled down to about 1.5 GHz by the power limit; 512 on 8700, 75 us, 950 TFLOP/s.  A pair of
 // 64-key tiles takes some 1600 cycles against 1280 of products and 1024 of exponentials.  Tried and slower: tiles of 128
@@ -45,6 +47,9 @@ static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kLaunchRegs * NUM_THR
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kPCol = 32;  // P_h (pairs of 16 bit) within its S_h buffer
 constexpr float kRescaleThreshold = 8.0f;
+template <bool kBF16>
+constexpr float kTopLog2 = kBF16 ? 0.f : 7.f;  // log2 of P at the row's reference
+static_assert(kRescaleThreshold + kTopLog2<false> <= 15.f, "f16 ends at 65504");
 static_assert(2 * BM == kWideRows, "rows of a slot");
 
 template <int D>
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           l *= alpha;
           m = m_new;
         }
-        const float neg_m = (m == -INFINITY) ? 0.f : -m;
+        const float neg_m = kTopLog2<kBF16> - (m == -INFINITY ? 0.f : m);
         if (__any_sync(0xffffffffu, rescale)) {  // not at a segment's first tile
           // S_h(it) complete means PV_h(it - 2) complete: the parity wait for PV_h(it - 1) is unambiguous
           if (!wait_all(bar(L::B_PVDONE + 2 * h + (b ^ 1)), ((it - 1) >> 1) & 1, abort_flag, CEA_DEV_TIMEOUT_SOFTMAX)) {
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       const float inv_l = l == 0.f ? 0.f : 1.f / l;
-      const float lse_row = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      const float lse_row = l == 0.f ? -INFINITY : (m + (log2f(l) - kTopLog2<kBF16>)) * kLn2;
       const int slot = g.slot;
       const int head = g.hu * G + row_head;
       const int64_t trow = static_cast<int64_t>(g.row0) + tok;

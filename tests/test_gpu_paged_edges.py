@@ -173,3 +173,54 @@ def test_attention_of_fewer_rows_than_the_batch_has(dtype, dim, rows):
     assert _lib.device_status(clear=True) == _lib.DEV_BAD_BATCH
     R.check(out, lse, (ref[0][:rows], ref[1][:, :rows], ref[2][:rows], ref[3][:, :rows]), dtype=TYPES[dtype],
             out_dtype=torch.float32, single_p=True)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tail", ["even", "spread"])
+@pytest.mark.parametrize("dim,group,n", [(64, 1, 1), (128, 4, 1), (64, 4, 4), (64, 1, 20), (128, 4, 33)])
+def test_one_key_far_above_a_long_tail(dtype, tail, dim, group, n):
+    """One key holds nearly all the weight and a value of 0; the output is what is left of the others, 2^-20 to 2^-26 of it
+    each.  Queries pick one column of the keys, so the scores are exact.
+
+    A weight's exponent (below 26 in magnitude, log2) takes three roundings of half a step of fp32, the hardware's exp2 is
+    good to 2^-22.  Rounded to 16 bits it is off by half a step, 2^-11 or 2^-8 (one number, the chunk kernel) or the square
+    of it, 2^-22 or 2^-17 with the second's rounding (two, the decode kernel), in f16 at least by 2^-25 of the unit that
+    the kernel holds it in: 2^-7 and 2^-14 of the largest weight.  Products of 16 keys are added one after another, each
+    sum cut to fp32 (2^-23), in the decode kernel for two numbers by each of eight warps."""
+    N, H, B, page = 32768, 32, 6, 64
+    t = TYPES[dtype]
+    g = torch.Generator(device=DEV).manual_seed(dim + n)
+    k = torch.zeros(N // page, H, page, dim, dtype=t, device=DEV)
+    score = torch.zeros(H, N, device=DEV) if tail == "even" else torch.rand(H, N, generator=g, device=DEV) * 4 - 1
+    score[:, 37] = 17.25
+    k[:, :, :, 0] = score.to(t).view(H, N // page, page).transpose(0, 1)
+    score = k[:, :, :, 0].transpose(0, 1).reshape(H, N).double()
+    v = torch.rand(N // page, H, page, dim, generator=g, device=DEV).to(t)
+    v[37 // page, :, 37 % page] = 0
+    q = torch.zeros(B * n, H * group, dim, dtype=t, device=DEV)
+    q[:, :, 0] = 1
+    x = {"q": q, "k_pages": k, "v_pages": v,
+         "page_table": torch.arange(N // page, dtype=torch.int32, device=DEV).expand(B, -1),  # all read the same pages
+         "seq_lens": torch.full((B,), N, dtype=torch.int32, device=DEV),
+         "q_offsets": torch.arange(0, B * n + 1, n, dtype=torch.int32, device=DEV)}
+    out = torch.empty(q.shape, device=DEV)
+    lse = torch.empty(H * group, B * n, device=DEV)
+    kw = {"scale": 1.0, "causal": False, "min_q_len": n, "max_q_len": n}
+    cea.paged_attend_into(**x, out=out, lse=lse, **kw)
+    single = _kernels(x, **kw)
+    assert single in (_lib.PAGED_TC, _lib.PAGED_DECODE)
+    single = single == _lib.PAGED_TC
+    p = torch.softmax(score, -1)
+    values = v.transpose(0, 1).reshape(H, N, dim).double()
+    want = torch.einsum("hj,hjd->hd", p, values)
+    e = 3 * 26 * 2.0**-24 * math.log(2) + 2.0**-22
+    half = torch.finfo(t).eps / 2
+    relative = (half if single else max(half * half, 2.0**-17 if dtype == "bf16" else 0)) + 2 * e
+    relative += (N / 16 if single else 2 * N / 128) * 2.0**-23 + N / 64 * 2.0**-24
+    absolute = (2.0**-25 * (2.0**-7 if single else 2.0**-14) * values.sum(1)) if dtype == "f16" else 0.0
+    tol = (want * (relative + 2.0**-24) + absolute).repeat_interleave(group, 0)
+    off = (out.double() - want.repeat_interleave(group, 0)).abs()
+    assert bool((off <= tol).all()), (float((off / tol).max()), float((off / want.repeat_interleave(group, 0)).max()))
+    stat = torch.logsumexp(score, -1).repeat_interleave(group, 0)[:, None]
+    assert float((lse.double() - stat).abs().max()) <= e + (N / 64 + 4 * 18) * 2.0**-24
+    assert _lib.device_status(clear=True) == 0
