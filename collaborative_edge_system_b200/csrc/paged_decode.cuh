@@ -95,6 +95,18 @@ __device__ __forceinline__ float round16(float x) {
   return __half2float(__float2half_rn(x));
 }
 
+// `x` with infinities and NaN replaced by zeros (of either sign).  A number times 0 is 0, an infinity or NaN the NaN 0x7fff,
+// so the product's bits are those to clear: one multiply-add and one logic operation for two numbers.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
+  uint32_t bad;
+  if constexpr (kBF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
+  return x & ~bad;
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -308,10 +320,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           a[2] &= keep1;
           a[3] &= keep1;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
-            mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
-          }
+          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
+          // an infinity counts in the first product only: the second's factor, a remainder, may be 0 or negative
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = finite_or_zero<kBF16>(a[e]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
         }
       }
       __syncwarp();

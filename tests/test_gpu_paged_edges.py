@@ -224,3 +224,26 @@ def test_one_key_far_above_a_long_tail(dtype, tail, dim, group, n):
     stat = torch.logsumexp(score, -1).repeat_interleave(group, 0)[:, None]
     assert float((lse.double() - stat).abs().max()) <= e + (N / 64 + 4 * 18) * 2.0**-24
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,counts", [
+    ("bf16", 8, 2, 128, [1, 1, 1]), ("f16", 8, 8, 64, [1, 2, 1]), ("bf16", 16, 4, 64, [4, 3, 1]), ("f16", 4, 1, 128, [30, 20, 1]),
+    ("bf16", 4, 4, 64, [70, 2, 1]), ("f32", 4, 2, 64, [3, 20, 1]), ("bf16", 4, 2, 80, [1, 5, 1])])
+def test_an_infinite_value_that_a_token_sees_gives_that_infinity(dtype, heads, kv_heads, dim, counts):
+    lens = [5000, 200, 1]
+    x = R.batch(lens, counts, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=TYPES[dtype], device=DEV, seed=dim)
+    plain = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"])
+    for b, key in enumerate([3111, 70, 0]):  # seen by every new token
+        page = int(x["page_table"][b, key // 16])
+        x["v_pages"][page, :, key % 16, 3] = math.inf
+        x["v_pages"][page, :, key % 16, 5] = -math.inf
+    for kw in ({}, {"causal": False}):
+        out, lse = cea.paged_attention_with_lse(**x, max_q_len=max(counts), **kw)
+        assert (out[..., 3] == math.inf).all() and (out[..., 5] == -math.inf).all()
+        assert torch.isfinite(lse).all()
+        assert torch.isfinite(out[..., [d for d in range(dim) if d not in (3, 5)]]).all()
+        if not kw:
+            keep = [d for d in range(dim) if d not in (3, 5)]
+            R.check(out[..., keep], lse, (plain[0][..., keep], plain[1], plain[2][..., keep], plain[3]), dtype=TYPES[dtype],
+                    out_dtype=torch.float32, single_p=bool(_kernels(x, max_q_len=max(counts)) & _lib.PAGED_TC))
+    assert _lib.device_status(clear=True) == 0
