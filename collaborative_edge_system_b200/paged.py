@@ -446,26 +446,25 @@ class PagedKVCache:
             raise ValueError("extend takes each sequence once, with a count >= 0 for each")
         ps = self.page_size
         need, split = 0, []
+        writers: Dict[int, int] = {}  # shared page -> sequences of this call that write it
         for s, c in zip(seqs, counts):
             n = self.length(s)
             need += -(-(n + c) // ps) - len(self._pages[s])
             if c and n % ps and self.pool.refs[self._pages[s][-1]] > 1:
                 split.append(s)
-        fresh = self.pool.alloc(need + len(split))
-        # several owners of one page may split from it in one call: the last of them keeps the page itself
-        src, dst, spare = [], [], []
+                writers[self._pages[s][-1]] = writers.get(self._pages[s][-1], 0) + 1
+        # where all owners of a page split from it in one call, the last of them keeps the page itself
+        fresh = self.pool.alloc(need + sum(min(n, self.pool.refs[p] - 1) for p, n in writers.items()))
+        src, dst = [], []
         for s in split:
             old = self._pages[s][-1]
-            new = fresh.pop()
             if self.pool.refs[old] == 1:
-                spare.append(new)
                 continue
             self.pool.release([old])
-            self._pages[s][-1] = new
+            self._pages[s][-1] = fresh.pop()
             src.append(old)
-            dst.append(new)
+            dst.append(self._pages[s][-1])
         self._copy(src, dst)
-        self.pool.release(spare)
         for s, c in zip(seqs, counts):
             self._lengths[s] += c
             grow = -(-self._lengths[s] // ps) - len(self._pages[s])
