@@ -61,7 +61,7 @@ def test_two_owners_of_a_page_split_with_one_free_page():
 @pytest.mark.parametrize("seed", range(12))
 def test_extension_is_refused_only_where_the_pages_are_missing(seed):
     rnd = random.Random(seed)
-    cache = HostCache(rnd.choice([5, 9, 14]), rnd.choice([2, 3, 4]))
+    cache = HostCache(rnd.choice([4, 5, 7, 14]), rnd.choice([2, 3, 4]))
     refused = 0
     for _ in range(400):
         ids = sorted(cache._lengths)
@@ -69,8 +69,8 @@ def test_extension_is_refused_only_where_the_pages_are_missing(seed):
         if move == "add" or not ids:
             cache.add()
         elif move == "extend":
-            some = rnd.sample(ids, rnd.randint(1, len(ids)))
-            counts = [rnd.randint(0, 3) for _ in some]
+            some = rnd.sample(ids, rnd.choice([len(ids), rnd.randint(1, len(ids))]))
+            counts = [rnd.randint(0, rnd.choice([1, 3])) for _ in some]
             need, free, before = _pages_needed(cache, some, counts), cache.num_free_pages, cache.state()
             if need > free:
                 with pytest.raises(cea.OutOfPages):
