@@ -473,11 +473,15 @@ class PagedKVCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
         """The new tokens' ``k`` / ``v`` ``[T, Hkv, D]`` of one layer into the pages."""
+        if k.shape[:1] != (batch.num_tokens,):
+            raise ValueError(f"k {tuple(k.shape)} for a batch of {batch.num_tokens} new tokens")
         paged_append(k, v, self.k[layer], self.v[layer], batch.page_table, batch.seq_lens, batch.q_offsets)
 
     def attend(self, layer: int, q: torch.Tensor, batch: PagedBatch, *, causal: bool = True,
                scale: Optional[float] = None) -> torch.Tensor:
         """Attention ``[T, Hq, D]`` of the new tokens over one layer's pages, theirs (appended before) included."""
+        if q.shape[:1] != (batch.num_tokens,):
+            raise ValueError(f"q {tuple(q.shape)} for a batch of {batch.num_tokens} new tokens")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         paged_attend_into(q, self.k[layer], self.v[layer], batch.page_table, batch.seq_lens, batch.q_offsets, out,
                           min_q_len=batch.min_q_len, max_q_len=batch.max_q_len, causal=causal, scale=scale)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import collaborative_edge_system_b200 as cea
-from collaborative_edge_system_b200 import paged
+from collaborative_edge_system_b200 import _lib, paged
 
 CPU = torch.device("cpu")
 
@@ -103,3 +103,30 @@ def test_extension_is_refused_only_where_the_pages_are_missing(seed):
                 counted[p] += 1
         assert counted == cache.pool.refs and cache.num_free_pages == counted.count(0)
     assert refused
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """Checks that come before the kernels, on CPU tensors: what they let pass ends in ``reached``."""
+    reached = []
+    monkeypatch.setattr(_lib, "device_number", lambda *t: 0)
+    for name in ("paged_attn", "paged_append", "copy_pages"):
+        monkeypatch.setattr(_lib, name, lambda p, dev: reached.append(p))
+    return reached
+
+
+def test_cache_refuses_rows_that_are_not_the_batchs(anywhere):
+    cache = HostCache(4, 4)
+    batch = cache.extend([cache.add(), cache.add()], [3, 2])
+    good = torch.zeros(5, 1, 1)
+    cache.append(0, good, good, batch)
+    cache.attend(0, good, batch)
+    assert [p.T for p in anywhere] == [5, 5]
+    anywhere.clear()
+    for rows in (0, 4, 6):
+        x = torch.zeros(rows, 1, 1)
+        for call in (lambda: cache.append(0, x, x, batch), lambda: cache.append(0, good, x, batch),
+                     lambda: cache.attend(0, x, batch)):
+            with pytest.raises(ValueError):
+                call()
+    assert not anywhere
