@@ -34,6 +34,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections import Counter
 from operator import index
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -245,7 +246,8 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Indices, dst: 
 
 # ------------------------------------------------------------------------------------------------ the cache
 class PageAllocator:
-    """Pages of one pool with reference counts (host only).  The lowest free page is handed out first."""
+    """Pages of one pool with reference counts (host only).  The lowest free page is handed out first.  A call that is
+    refused changes nothing."""
 
     def __init__(self, num_pages: int) -> None:
         if num_pages < 0:
@@ -257,7 +259,17 @@ class PageAllocator:
     def num_free(self) -> int:
         return len(self._free)
 
+    def _used(self, pages: Sequence[int], times: int = 1) -> None:
+        """Every page is of the pool and has at least ``times`` owners for each time that it stands in ``pages``."""
+        for p, n in Counter(pages).items():
+            if not 0 <= p < len(self.refs):
+                raise ValueError(f"no page {p} in a pool of {len(self.refs)}")
+            if self.refs[p] < max(1, times * n):
+                raise ValueError(f"page {p} is free" if self.refs[p] < 1 else f"page {p} has {self.refs[p]} owners")
+
     def alloc(self, count: int) -> List[int]:
+        if count < 0:
+            raise ValueError("count must be >= 0")
         if count > len(self._free):
             raise OutOfPages(f"{count} pages needed, {len(self._free)} of {len(self.refs)} free")
         pages = [self._free.pop() for _ in range(count)]
@@ -266,16 +278,14 @@ class PageAllocator:
         return pages
 
     def share(self, pages: Sequence[int]) -> None:
+        self._used(pages, 0)
         for p in pages:
-            if self.refs[p] < 1:
-                raise ValueError(f"page {p} is free")
             self.refs[p] += 1
 
     def release(self, pages: Sequence[int]) -> None:
+        self._used(pages)
         freed = []
         for p in pages:
-            if self.refs[p] < 1:
-                raise ValueError(f"page {p} is free")
             self.refs[p] -= 1
             if self.refs[p] == 0:
                 freed.append(p)
@@ -289,6 +299,9 @@ class PageAllocator:
         return src, sorted(p for p in self._free if p < used)
 
     def move(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        self._used(src)
+        if len(src) != len(dst) or len(set(src)) != len(src) or len(set(dst)) != len(dst) or not set(dst) <= set(self._free):
+            raise ValueError("pages in use move to as many free ones, each of them once")
         for s, d in zip(src, dst):
             self.refs[d], self.refs[s] = self.refs[s], 0
         self._free = [p for p in range(len(self.refs) - 1, -1, -1) if not self.refs[p]]

@@ -130,3 +130,19 @@ def test_cache_refuses_rows_that_are_not_the_batchs(anywhere):
             with pytest.raises(ValueError):
                 call()
     assert not anywhere
+
+
+def test_allocator_refusals_change_nothing():
+    a = cea.PageAllocator(4)
+    a.alloc(3)
+    a.share([1])
+    before = list(a.refs), a.num_free
+    for call in (lambda: a.release([0, 0]), lambda: a.release([0, 3]), lambda: a.release([1, 1, 1]), lambda: a.release([-1]),
+                 lambda: a.release([0, 4]), lambda: a.share([0, 3]), lambda: a.share([-2]), lambda: a.share([0, 4]),
+                 lambda: a.alloc(-1), lambda: a.move([0], [3, 3]), lambda: a.move([0], [1]), lambda: a.move([3], [0]),
+                 lambda: a.move([0, 1], [3, 3]), lambda: a.move([0, 0], [3, 2])):
+        with pytest.raises(ValueError):
+            call()
+        assert (list(a.refs), a.num_free) == before
+    a.release([0, 1, 1])
+    assert a.num_free == 3 and a.alloc(3) == [0, 1, 3]
