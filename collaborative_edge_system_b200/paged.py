@@ -34,6 +34,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from collections import Counter
 from operator import index
 from typing import Dict, List, Optional, Sequence, Tuple, Union
@@ -90,6 +91,13 @@ def _checked(k_pages, v_pages, page_table, seq_lens, q_offsets):
     return pages, kp, vp, B, table[1], ts[0]
 
 
+def _record(layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as e:  # a count, size or scale that is no number of its field
+        raise ValueError(f"an argument or a size does not fit the call: {e}") from None
+
+
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> None:
     """Write the new tokens' ``k`` / ``v`` (``[T, Hkv, D]``, any token and head strides) into their pages, bit for bit.
@@ -106,10 +114,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError("k, v and the pages must share a dtype")
     if D > 1 and (ks[2] != 1 or vs[2] != 1):
         raise ValueError("k and v must be contiguous along the head dimension")
-    _lib.paged_append(_lib.PagedAppendParams.from_buffer_copy(_lib.PAGED_APPEND_RECORD.pack(
-        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_offsets.data_ptr(), seq_lens.data_ptr(),
-        page_table.data_ptr(), ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], table, B, shape[0],
-        H, D, ps, P, width, k.element_size())), dev)
+    _lib.paged_append(_lib.PagedAppendParams.from_buffer_copy(_record(
+        _lib.PAGED_APPEND_RECORD, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_offsets.data_ptr(),
+        seq_lens.data_ptr(), page_table.data_ptr(), ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2],
+        table, B, shape[0], H, D, ps, P, width, k.element_size())), dev)
 
 
 _TAIL = bytes(ctypes.sizeof(_lib.PagedAttnParams) - _lib.PAGED_ATTN_RECORD.size)  # the workspace's fields
@@ -134,12 +142,12 @@ def _attn_params(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out, lse,
         if lse.dtype != accumulation_dtype(dtype):
             raise ValueError(f"lse must be {accumulation_dtype(dtype)} for {dtype} inputs")
         lp, (l0, l1) = lse.data_ptr(), lse.stride()
-    return _lib.PagedAttnParams.from_buffer_copy(_lib.PAGED_ATTN_RECORD.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, q_offsets.data_ptr(),
+    return _lib.PagedAttnParams.from_buffer_copy(_record(
+        _lib.PAGED_ATTN_RECORD, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, q_offsets.data_ptr(),
         seq_lens.data_ptr(), page_table.data_ptr(), qs[0], qs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], os[0], os[1],
         l0, l1, table, B, T, Hq, H, D, ps, P, width, min_q_len,
         max(T, min_q_len) if max_q_len is None else max_q_len,
-        1.0 / math.sqrt(D) if scale is None else scale, bool(causal), _lib.dtype_code(dtype),
+        1.0 / math.sqrt(max(D, 1)) if scale is None else scale, bool(causal), _lib.dtype_code(dtype),
         _lib.dtype_code(out.dtype)) + _TAIL)
 
 

@@ -146,3 +146,26 @@ def test_allocator_refusals_change_nothing():
         assert (list(a.refs), a.num_free) == before
     a.release([0, 1, 1])
     assert a.num_free == 3 and a.alloc(3) == [0, 1, 3]
+
+
+def _call(**kw):
+    x = {"q": torch.zeros(3, 4, 8), "k_pages": torch.zeros(5, 2, 4, 8), "v_pages": torch.zeros(5, 2, 4, 8),
+         "page_table": torch.zeros(2, 3, dtype=torch.int32), "seq_lens": torch.ones(2, dtype=torch.int32),
+         "q_offsets": torch.tensor([0, 1, 3], dtype=torch.int32)}
+    return cea.paged_attention(**{**x, **kw})
+
+
+@pytest.mark.parametrize("kw", [{"min_q_len": 2**31}, {"max_q_len": 2**40}, {"min_q_len": -(2**33)}, {"max_q_len": 1.5},
+                                {"min_q_len": 1.0}, {"min_q_len": "1"}, {"scale": "1"}, {"scale": None, "max_q_len": 3.0}])
+def test_numbers_that_are_no_count_or_scale_are_refused(anywhere, kw):
+    with pytest.raises((ValueError, TypeError)):
+        _call(**kw)
+    assert not anywhere
+
+
+def test_heads_without_columns_are_refused(monkeypatch):
+    monkeypatch.setattr(_lib, "device_number", lambda *t: 0)
+    codes = []
+    monkeypatch.setattr(_lib, "paged_attn", lambda p, like: codes.append(_lib.paged_attn_kernels(p)))
+    _call(q=torch.zeros(3, 4, 0), k_pages=torch.zeros(5, 2, 4, 0), v_pages=torch.zeros(5, 2, 4, 0))
+    assert codes == [-1]  # the library's own refusal, not a division by zero
