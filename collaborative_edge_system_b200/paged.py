@@ -102,7 +102,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  page_table: torch.Tensor, seq_lens: torch.Tensor, q_offsets: torch.Tensor) -> None:
     """Write the new tokens' ``k`` / ``v`` (``[T, Hkv, D]``, any token and head strides) into their pages, bit for bit.
 
-    Two tokens with one place (a page that two of the batch's sequences write) leave either's row there.
+    Two tokens with one place (a page that two of the batch's sequences write) leave any mix of their rows' parts there;
+    :class:`PagedKVCache` makes no such batch.
     """
     dev = _lib.device_number(k, v, k_pages, v_pages, page_table, seq_lens, q_offsets)
     pages, kp, vp, B, width, table = _checked(k_pages, v_pages, page_table, seq_lens, q_offsets)
@@ -161,6 +162,13 @@ def paged_attend_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     ``min_q_len`` and ``max_q_len`` bound the number of new tokens of the sequences that have any; they choose the
     kernels and are promises (0 and ``None`` always hold): decoding sequences (up to 8 or 16 query rows per KV head)
     and chunks of prompts have a kernel each, and a batch that cannot hold one kind does not launch its kernel.
+
+    16-bit inputs: the kernels differ in what is left of a probability when it is multiplied with the values, so a
+    sequence's result differs within these bounds with the bounds given and with the other sequences of the call.  The
+    decoding kernel keeps it to 2^-17 (bf16) or 2^-22 (f16), the chunk kernel rounds it to the input type (half a step,
+    2^-8 or 2^-11), as the dense prefill kernel does; the CUDA cores, which take the shapes outside both, keep fp32.
+    9 to 16 query rows at 128 columns go to the chunk kernel where ``min_q_len`` says that no sequence has fewer, and
+    to the decoding kernel where it does not.
     """
     if lse is None:
         _lib.device_number(q, k_pages, v_pages, page_table, seq_lens, q_offsets, out)

@@ -362,8 +362,11 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * min_q_len / max_q_len bound the n_b > 0 of the batch and choose the kernels
  * (0 and T are always right): sequences with n_b * Hq / Hkv <= 8 go through the
  * split decode kernel, those with more than 16 through the tcgen05 kernel, those
- * between through either, as measured; each where it applies (bf16 / f16, D in {64, 128}, page_size a multiple of 8, 16-byte aligned rows);
- * everything else through the CUDA-core kernel.  cea_paged_attn_kernels returns
+ * between through either, as measured; each where it applies (bf16 / f16, D in
+ * {64, 128}, page_size a multiple of 8, 16-byte aligned rows); everything else
+ * through the CUDA-core kernel.  A probability meets the values to 2^-17 (bf16) or
+ * 2^-22 (f16) in the decode kernel, rounded to the input type (2^-8, 2^-11) in the
+ * tcgen05 kernel, in fp32 on CUDA cores.  cea_paged_attn_kernels returns
  * the kernels of a call as a mask: 1 tcgen05, 2 split decode, 4 CUDA cores.
  */
 typedef struct cea_paged_attn_params {
