@@ -435,6 +435,8 @@ class LlamaModel:
             raise ValueError("the paged cache needs query heads grouped evenly over this rank's KV heads")
         if ids.dim() != 1 or ids.shape[0] != batch.num_tokens:
             raise ValueError(f"ids {tuple(ids.shape)} for a batch of {batch.num_tokens} new tokens")
+        if batch.num_tokens == 0:
+            return self.embed.new_empty((0, self.embed.shape[1]))
         positions = batch.positions.view(1, -1)
 
         def attend(idx, q, k, v):
