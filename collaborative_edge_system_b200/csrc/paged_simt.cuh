@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params
       row[h] = static_cast<int64_t>(g.row0) + tok;
       limit[h] = !in[h] ? -1 : (p.dv.causal ? min(g.ctx + tok, g.len - 1) : g.len - 1);
     }
+    // keys 0 .. all_see are visible to both rows, or to the one that exists
+    const int all_see = in[0] && in[1] ? min(limit[0], limit[1]) : max(limit[0], limit[1]);
     const bool busy = __any_sync(0xffffffffu, in[0] || in[1]);  // some row of the warp exists
     // keys of tile t into stage `st`; those behind the unit's last are zeros (their scores are masked)
     auto fetch = [&](int t, int st) {
@@ -223,22 +225,43 @@ __global__ void __launch_bounds__(NT) attn_kernel(const __grid_constant__ Params
           for (int e = 0; e < VN; ++e) o[h][c][e] *= alpha;
       }
       __syncwarp();  // a row's 16 threads are of one warp
+      if (min(t * BK + BK, g.keys) - 1 <= all_see) {  // slots behind the last key are zeros
 #pragma unroll 2
-      for (int j = 0; j < BK; j += VN) {
-        const Word<A> e0 = word(ps + r0 * L::LP + j), e1 = word(ps + (r0 + 8) * L::LP + j);
+        for (int j = 0; j < BK; j += VN) {
+          const Word<A> e0 = word(ps + r0 * L::LP + j), e1 = word(ps + (r0 + 8) * L::LP + j);
 #pragma unroll
-        for (int i = 0; i < VN; ++i)
+          for (int i = 0; i < VN; ++i)
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const int col = (sub + TPR * c) * VN;
-            if (DMAX % (VN * TPR) != 0 && col >= DMAX) continue;  // fp32 rows of 32: 8 words for 16 threads
-            const Word<A> y = word(vs + (j + i) * L::LD + col);
+            for (int c = 0; c < NC; ++c) {
+              const int col = (sub + TPR * c) * VN;
+              if (DMAX % (VN * TPR) != 0 && col >= DMAX) continue;  // fp32 rows of 32: 8 words for 16 threads
+              const Word<A> y = word(vs + (j + i) * L::LD + col);
 #pragma unroll
-            for (int e = 0; e < VN; ++e) {
-              o[0][c][e] += e0[i] * y[e];
-              o[1][c][e] += e1[i] * y[e];
+              for (int e = 0; e < VN; ++e) {
+                o[0][c][e] += e0[i] * y[e];
+                o[1][c][e] += e1[i] * y[e];
+              }
+            }
+        }
+      } else {
+        // keys that only some rows see: a probability of 0 does not silence an infinity or a NaN, so each row ends at its
+        // last key
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int end = min(BK, limit[h] - t * BK + 1);
+#pragma unroll 1
+          for (int j = 0; j < end; ++j) {
+            const A w = ps[(r0 + 8 * h) * L::LP + j];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const int col = (sub + TPR * c) * VN;
+              if (DMAX % (VN * TPR) != 0 && col >= DMAX) continue;
+              const Word<A> y = word(vs + j * L::LD + col);
+#pragma unroll
+              for (int e = 0; e < VN; ++e) o[h][c][e] += w * y[e];
             }
           }
+        }
       }
       __syncwarp();
     }

@@ -247,3 +247,69 @@ def test_an_infinite_value_that_a_token_sees_gives_that_infinity(dtype, heads, k
             R.check(out[..., keep], lse, (plain[0][..., keep], plain[1], plain[2][..., keep], plain[3]), dtype=TYPES[dtype],
                     out_dtype=torch.float32, single_p=bool(_kernels(x, max_q_len=max(counts)) & _lib.PAGED_TC))
     assert _lib.device_status(clear=True) == 0
+
+
+def _spoilt(lens, counts, heads, kv_heads, dim, dtype, seed, bad):
+    """A batch, its plain result, and the same batch with `bad` in some columns of the values of new tokens: of the last but
+    one of every sequence that has two, and of every fifth."""
+    x = R.batch(lens, counts, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=TYPES[dtype], device=DEV, seed=seed)
+    plain = R.attention(x["q"], x["k_pages"], x["v_pages"], x["page_table"], x["seq_lens"], x["q_offsets"])
+    sees = torch.zeros(sum(counts), dtype=torch.bool)
+    row = 0
+    for b, (n_all, n) in enumerate(zip(lens, counts)):
+        spoilt = [i for i in range(n) if n > 1 and n_all - n + i >= 0 and (i == n - 2 or (i % 5 == 3 and n > 6))]
+        for i in spoilt:
+            pos = n_all - n + i
+            x["v_pages"][int(x["page_table"][b, pos // 16]), :, pos % 16, 1::7] = bad
+        for i in range(n):
+            sees[row + i] = any(s <= i for s in spoilt)
+        row += n
+    return x, plain, sees
+
+
+LEAKS = {
+    _lib.PAGED_SIMT: [("f32", 8, 2, 64, [700, 33, 5], [40, 17, 2]), ("bf16", 4, 2, 80, [90, 300, 40], [3, 130, 40]),
+                      ("f64", 3, 3, 20, [50, 20], [9, 20]), ("f16", 6, 2, 64, [90, 9], [70, 9])],
+    _lib.PAGED_DECODE: [("bf16", 8, 8, 64, [5000, 8, 65, 1], [8, 8, 5, 1]), ("f16", 32, 8, 128, [700, 64, 2, 3], [2, 2, 2, 2]),
+                        ("bf16", 16, 4, 64, [300, 66, 4], [4, 3, 4]), ("f16", 12, 4, 128, [900, 5, 66, 2], [4, 4, 3, 1])],
+    _lib.PAGED_TC: [("bf16", 32, 8, 128, [9000, 90, 17, 64], [33, 70, 17, 64]), ("f16", 8, 8, 64, [700, 300, 1000], [700, 257, 20]),
+                    ("bf16", 15, 5, 128, [200, 130], [130, 66]), ("f16", 64, 1, 64, [2000, 9], [5, 9])],
+}
+
+
+def _leak_cases(kernel):
+    return pytest.mark.parametrize("dtype,heads,kv_heads,dim,lens,counts", LEAKS[kernel], ids=lambda v: str(v).replace(" ", ""))
+
+
+def _no_leak(kernel, dtype, heads, kv_heads, dim, lens, counts, bad):
+    x, plain, sees = _spoilt(lens, counts, heads, kv_heads, dim, dtype, dim + heads, bad)
+    if kernel == _lib.PAGED_SIMT and dtype == "f16":  # a shape of the tensor kernels whose rows are not aligned for them
+        for n in ("k_pages", "v_pages"):
+            flat = torch.empty(x[n].numel() + 1, dtype=x[n].dtype, device=DEV)
+            flat[1:] = x[n].flatten()
+            x[n] = flat[1:].view_as(x[n])
+    kw = {"min_q_len": min(counts), "max_q_len": max(counts)}
+    assert _kernels(x, **kw) == kernel
+    out, lse = cea.paged_attention_with_lse(**x, **kw)
+    keep = torch.ones(dim, dtype=torch.bool)
+    keep[1::7] = False
+    single = kernel == _lib.PAGED_TC
+    check = lambda cols, rows: R.check(  # noqa: E731
+        out[rows][..., cols], lse[:, rows], (plain[0][rows][..., cols], plain[1][:, rows], plain[2][rows][..., cols],
+                                            plain[3][:, rows]), dtype=TYPES[dtype], out_dtype=out.dtype, single_p=single)
+    rows = torch.arange(len(sees))
+    check(keep, rows)  # the other columns, of every token
+    if bool((~sees).any()):
+        check(~keep, rows[~sees])  # the spoilt ones, of the tokens that do not see them
+    seen = out[rows[sees]][..., ~keep]
+    assert seen.isnan().all() if math.isnan(bad) else (seen == bad).all()
+    assert _lib.device_status(clear=True) == 0
+
+
+BAD = pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf], ids=["nan", "inf", "-inf"])
+
+
+@BAD
+@_leak_cases(_lib.PAGED_SIMT)
+def test_values_that_a_token_does_not_see_never_reach_it_on_cuda_cores(dtype, heads, kv_heads, dim, lens, counts, bad):
+    _no_leak(_lib.PAGED_SIMT, dtype, heads, kv_heads, dim, lens, counts, bad)
