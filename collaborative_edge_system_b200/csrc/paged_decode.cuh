@@ -95,8 +95,8 @@ __device__ __forceinline__ float round16(float x) {
   return __half2float(__float2half_rn(x));
 }
 
-// `x` with infinities and NaN replaced by zeros (of either sign).  A number times 0 is 0, an infinity or NaN the NaN 0x7fff,
-// so the product's bits are those to clear: one multiply-add and one logic operation for two numbers.
+// Two numbers with infinities and NaN replaced by zeros (of either sign).  A number times 0 is 0, an infinity or NaN the
+// NaN 0x7fff, so the product's bits are those to clear: one multiply-add and one logic operation.
 template <bool kBF16>
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
   uint32_t bad;
@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
           keep1 = (k0 + 8 < left ? 0xffffu : 0u) | (k0 + 9 < left ? 0xffff0000u : 0u);
         }
+        uint32_t other = 0;  // not 0: some value is no finite number
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           uint32_t a[4];
@@ -320,12 +321,40 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           a[2] &= keep1;
           a[3] &= keep1;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
-          // an infinity counts in the first product only: the second's factor, a remainder, may be 0 or negative
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t f = finite_or_zero<kBF16>(a[e]);
+            other |= a[e] ^ f;
+            a[e] = f;
+          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = finite_or_zero<kBF16>(a[e]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
+            mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
+          }
+        }
+        // The products leave infinities and NaN out, as a factor (a probability that is masked, a remainder) may be 0 or
+        // of the wrong sign.  They make an infinity or NaN of the rows that see their key, whatever its probability is.
+        if (__any_sync(0xffffffffu, other != 0u)) {
+#pragma unroll 1
+          for (int k = 0; k < min(16, left - key0); ++k) {
+            const int key = t * BK + key0 + k;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int d = j * 16 + 8 * x + kr;
+                const uint16_t bits = *reinterpret_cast<const uint16_t*>(
+                    smem + (swz(vt, key0 + k, d >> 3) - sbase) + (d & 7) * 2);
+                const float v = kBF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
+                                      : __half2float(__ushort_as_half(bits));
+                if (finite_or_zero<kBF16>(bits) == bits) continue;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (key <= lim[nt][e]) o[nt][j][2 * x + e] += v;
+              }
+          }
         }
       }
       __syncwarp();

@@ -313,3 +313,9 @@ BAD = pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf], ids=["nan"
 @_leak_cases(_lib.PAGED_SIMT)
 def test_values_that_a_token_does_not_see_never_reach_it_on_cuda_cores(dtype, heads, kv_heads, dim, lens, counts, bad):
     _no_leak(_lib.PAGED_SIMT, dtype, heads, kv_heads, dim, lens, counts, bad)
+
+
+@BAD
+@_leak_cases(_lib.PAGED_DECODE)
+def test_values_that_a_token_does_not_see_never_reach_it_in_the_decode_kernel(dtype, heads, kv_heads, dim, lens, counts, bad):
+    _no_leak(_lib.PAGED_DECODE, dtype, heads, kv_heads, dim, lens, counts, bad)
