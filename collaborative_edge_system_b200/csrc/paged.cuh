@@ -45,6 +45,24 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b) {
   return s;
 }
 
+// Two numbers with infinities and NaN replaced by zeros (of either sign).  A number times 0 is 0, an infinity or NaN the
+// NaN 0x7fff, so the product's bits are those to clear: one multiply-add and one logic operation.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
+  uint32_t bad;
+  if constexpr (kBF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
+  return x & ~bad;
+}
+
+// one 16-bit number
+template <bool kBF16>
+__device__ __forceinline__ float widen16(uint32_t bits) {
+  return kBF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
 // ------------------------------------------------------------------ division of the attention work
 // A unit of work is one block of `tb` new tokens of one sequence for one KV head (or, in the generic kernel, for a
 // group of its query heads), over the keys its last token sees.  The units are laid end to end on one axis, each as

@@ -382,6 +382,10 @@ int launch_paged_tc(const cea_paged_attn_params* p, const PagedPlan& pl, cudaStr
   a.dv = pg::Division{p->B, p->Hkv, 2 * a.half, G, INT64_MAX, int64_t(paged_choice(p).few) * G + 1,
                       p->min_q_len, p->max_q_len, p->causal ? 1 : 0, 384, 8};
   a.box = std::gcd(p->page_size, pg::tc::BK);
+  a.v = static_cast<const uint16_t*>(p->v_pages);
+  a.v_sp = p->v_stride[0];
+  a.v_sh = p->v_stride[1];
+  a.v_ss = p->v_stride[2];
   a.out = p->out;
   a.o_ss = p->o_stride[0];
   a.o_sh = p->o_stride[1];

@@ -95,18 +95,6 @@ __device__ __forceinline__ float round16(float x) {
   return __half2float(__float2half_rn(x));
 }
 
-// Two numbers with infinities and NaN replaced by zeros (of either sign).  A number times 0 is 0, an infinity or NaN the
-// NaN 0x7fff, so the product's bits are those to clear: one multiply-add and one logic operation.
-template <bool kBF16>
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
-  uint32_t bad;
-  if constexpr (kBF16)
-    asm("fma.rn.bf16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
-  else
-    asm("fma.rn.f16x2 %0, %1, %2, %2;" : "=r"(bad) : "r"(x), "r"(0u));
-  return x & ~bad;
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -345,8 +333,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 const int d = j * 16 + 8 * x + kr;
                 const uint16_t bits = *reinterpret_cast<const uint16_t*>(
                     smem + (swz(vt, key0 + k, d >> 3) - sbase) + (d & 7) * 2);
-                const float v = kBF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
-                                      : __half2float(__ushort_as_half(bits));
+                const float v = widen16<kBF16>(bits);
                 if (finite_or_zero<kBF16>(bits) == bits) continue;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)

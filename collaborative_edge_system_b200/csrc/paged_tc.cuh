@@ -16,7 +16,10 @@
 // epilogue has read O_h.
 // A row sees keys 0 .. limit; only tiles that reach behind the first token's limit are masked, with one compare per key.
 // Slots behind the unit's last key are not loaded or hold anything: their scores are masked, and their V rows are zeroed
-// in shared memory before the tile is released to the MMA (a probability of 0 does not silence a NaN).
+// in shared memory before the tile is released to the MMA (a probability of 0 does not silence a NaN).  For the same reason
+// the tiles that not all rows see whole are searched for infinities and NaN, which become zeros there and are added by
+// the epilogue to the rows that see them, from the pages (a rare path; the search is one pass of the V producer over the
+// last one to five tiles of a unit).
 // P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16 and 2^-11 for f16, independent per key),
 // the sum is of the unrounded fp32 values; S, statistics and O are fp32.  f16 numbers below 2^-14 lose bits and those below
 // 2^-25 are 0, so there P is 2^7 times the probability's ratio to its row's reference (at most 2^15 of 65504: the reference
@@ -70,7 +73,7 @@ struct Layout {
   static constexpr int B_KEMPTY = B_KFULL + KST;
   static constexpr int B_VFULL = B_KEMPTY + KST;
   static constexpr int B_VEMPTY = B_VFULL + VST;
-  static constexpr int B_VTAIL = B_VEMPTY + VST;  // a V tile that is zeroed behind its last key before it counts as full
+  static constexpr int B_VTAIL = B_VEMPTY + VST;  // a V tile that is looked at before it counts as full
   // x4: [half][S buffer].  One barrier per buffer: each phase is met before its next one can begin, where a barrier for
   // both would run two phases ahead of a waiter.
   static constexpr int B_SFULL = B_VTAIL + 1;
@@ -91,6 +94,8 @@ struct Params {
   Division dv;  // tb = 2 * half
   int half;     // tokens of a half: 128 / G
   int box;      // slots of a TMA box: divides the page and the tile
+  const uint16_t* v;
+  int64_t v_sp, v_sh, v_ss;  // page, head, slot
   void* out;
   int64_t o_ss, o_sh;
   float* lse;
@@ -109,6 +114,11 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t one;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
+}
+
+// The first tile of the unit that its rows do not all see whole (the first token sees the fewest keys).
+__device__ __forceinline__ int first_parted(const Params& p, const Seg& g) {
+  return max(0, p.dv.causal ? g.ctx + g.blk * p.dv.tb + 1 : g.len) / BK;
 }
 
 // Bounded wait of a whole warp (the contract of mbar_wait), short in code.
@@ -138,6 +148,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t sbase = smem_u32(smem);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  volatile int* other_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 8);  // a value that is no finite number was met
   auto bar = [&](int i) -> uint32_t { return sbase + L::OFF_BAR + 8 * i; };
   const SegQueue queue{smem + L::OFF_QUEUE, bar(L::B_QUEUE), bar(L::B_QUEUE + kQueue), abort_flag,
                        CEA_DEV_TIMEOUT_PRODUCER};
@@ -164,6 +175,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(bar(L::B_VTAIL), 1);
     queue.init(8 + 3);  // the softmax warps, the V producer and the issuers
     *abort_flag = 0;
+    *other_flag = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -199,6 +211,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       bool tail_open = false;  // a tail was loaded and not waited for
       auto load_tiles = [&](const Seg& g) -> bool {
         const int32_t* table = p.bt.table + g.b * p.bt.table_sb;
+        const int parted = is_k ? INT32_MAX : first_parted(p, g);
         for (int t = g.t0; t < g.t1; ++t) {
           const int u = g.it + (t - g.t0);
           const int st = u % nst;
@@ -218,7 +231,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           if (n > 0 && !wait_all(bar(b_empty + st), (n - 1) & 1, abort_flag, CEA_DEV_TIMEOUT_PRODUCER)) return false;
           const int boxes = __popc(__ballot_sync(0xffffffffu, load));
           const int left = g.keys - t * BK;
-          const bool tail = !is_k && left < BK;
+          const bool tail = t >= parted;  // a V tile that is looked at before it is released
           const uint32_t to = off + st * L::TILE;
           const uint32_t fb = tail ? bar(L::B_VTAIL) : bar(b_full + st);
           if (lane == 0) mbar_arrive_expect_tx(fb, boxes * p.box * 128);
@@ -234,6 +247,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
               for (int c = 0; c < L::KBOX; ++c)
                 *reinterpret_cast<uint4*>(tile + c * L::BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            __syncwarp();
+            uint32_t other = 0;
+            for (int i = lane; i < BK * 8 * L::KBOX; i += 32) {
+              uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
+              const uint4 w = *at;
+              const uint4 f = make_uint4(finite_or_zero<kBF16>(w.x), finite_or_zero<kBF16>(w.y),
+                                         finite_or_zero<kBF16>(w.z), finite_or_zero<kBF16>(w.w));
+              const uint32_t off_by = (w.x ^ f.x) | (w.y ^ f.y) | (w.z ^ f.z) | (w.w ^ f.w);
+              if (off_by != 0u) *at = f;
+              other |= off_by;
+            }
+            if (other != 0u) *other_flag = 1;
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(b_full + st));
@@ -492,6 +517,41 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int64_t obase = trow * p.o_ss + head * p.o_sh;
       const int prow = h * p.half * G + row;  // of the slot: [D / 4][row][4]
       float4* part = reinterpret_cast<float4*>(p.part_o) + static_cast<int64_t>(slot) * (D / 4) * kWideRows + prow;
+      // the flag was set before the tile was released, hence before the products that were waited for above
+      if (__any_sync(0xffffffffu, *other_flag != 0)) {
+        // the keys of searched tiles that this row sees
+        const int from = max(g.t0, first_parted(p, g)) * BK, to = min(limit + 1, g.t1 * BK);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(tO + c, o);
+          tmem_wait_ld();
+#pragma unroll 1
+          for (int key = from; key < to; ++key) {
+            const int page_i = key / p.bt.ps, page = p.bt.table[g.b * p.bt.table_sb + page_i];
+            if (page < 0 || page >= p.bt.num_pages) continue;
+            const uint4* src = reinterpret_cast<const uint4*>(p.v + page * p.v_sp + g.hu * p.v_sh +
+                                                              (key - page_i * p.bt.ps) * p.v_ss + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint4 w = src[e];
+              const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t bad = x[k] ^ finite_or_zero<kBF16>(x[k]);
+                float lo = __uint_as_float(o[e * 8 + 2 * k]), hi = __uint_as_float(o[e * 8 + 2 * k + 1]);
+                if (bad & 0xffffu) lo += widen16<kBF16>(x[k] & 0xffffu);
+                if (bad >> 16) hi += widen16<kBF16>(x[k] >> 16);
+                o[e * 8 + 2 * k] = __float_as_uint(lo);
+                o[e * 8 + 2 * k + 1] = __float_as_uint(hi);
+              }
+            }
+          }
+          __syncwarp();
+          tmem_st32(tO + c, o);
+        }
+        tmem_wait_st();
+      }
 #pragma unroll 1
       for (int c = 0; c < D; c += 64) {
         uint32_t o[64];

@@ -19,9 +19,8 @@ place.
 
   over the keys at positions up to the token's own (``causal``) or over all of them.  A token that sees no key gives
   ``out = 0`` and ``lse = -inf``; rows of no sequence are left as they were; slots behind a sequence's length never
-  count, whatever they hold.  An infinite value that a token sees gives that infinity (NaN where its probability is 0 in
-  the kernel's arithmetic).  (An infinity or NaN in the values of a new token may reach earlier new tokens of its
-  sequence in the same pass, as 0 times infinity in a product with masked weights; its keys do not.);
+  count, whatever they hold, and neither do keys and values that a token does not see.  An infinite value that it sees
+  gives that infinity (or NaN, where the kernel's arithmetic has a probability of 0);
 * :func:`copy_pages` copies pages in every layer at once.
 
 Nothing here synchronises the host.  Indices that the host cannot see are bounded on the device: a page table entry

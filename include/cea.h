@@ -354,11 +354,10 @@ int cea_kv_append(const cea_kv_append_params* p, void* stream);
  * its own (causal) or all seq_lens[b].  q / out [T, Hq, D] (strides token, head),
  * lse [Hq, T] natural log (strides head, token) or NULL.  A token that sees no key
  * (position below 0, or an empty sequence) gives out = 0 and lse = -inf.  Slots
- * behind a sequence's length are never used, whatever they hold.  An infinite value
- * that a token sees gives that infinity (NaN where its probability is 0 in the
- * kernel's arithmetic); one of a later new token of the sequence in the same call may
- * give NaN (0 times infinity), its keys do not.  out_dtype is
- * the input dtype or F32 (F64 for F64); lse is F32 (F64 for F64).
+ * behind a sequence's length, and keys and values that a token does not see, never
+ * count, whatever they hold.  An infinite value that it sees gives that infinity (or
+ * NaN, where the kernel's arithmetic has a probability of 0).  out_dtype is the input
+ * dtype or F32 (F64 for F64); lse is F32 (F64 for F64).
  * min_q_len / max_q_len bound the n_b > 0 of the batch and choose the kernels
  * (0 and T are always right): sequences with n_b * Hq / Hkv <= 8 go through the
  * split decode kernel, those with more than 16 through the tcgen05 kernel, those

@@ -319,3 +319,9 @@ def test_values_that_a_token_does_not_see_never_reach_it_on_cuda_cores(dtype, he
 @_leak_cases(_lib.PAGED_DECODE)
 def test_values_that_a_token_does_not_see_never_reach_it_in_the_decode_kernel(dtype, heads, kv_heads, dim, lens, counts, bad):
     _no_leak(_lib.PAGED_DECODE, dtype, heads, kv_heads, dim, lens, counts, bad)
+
+
+@BAD
+@_leak_cases(_lib.PAGED_TC)
+def test_values_that_a_token_does_not_see_never_reach_it_in_the_chunk_kernel(dtype, heads, kv_heads, dim, lens, counts, bad):
+    _no_leak(_lib.PAGED_TC, dtype, heads, kv_heads, dim, lens, counts, bad)
