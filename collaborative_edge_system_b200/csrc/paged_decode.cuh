@@ -299,7 +299,40 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
           keep1 = (k0 + 8 < left ? 0xffffu : 0u) | (k0 + 9 < left ? 0xffff0000u : 0u);
         }
-        uint32_t other = 0;  // not 0: some value is no finite number
+        // Keys that not all rows see: a probability of 0 does not silence an infinity or a NaN.  They are added to the rows
+        // that see them here, and zeros take their place in this warp's part of the tile.
+        if (t * BK + key0 + min(16, left - key0) > (p.dv.causal ? g.ctx : g.len - 1) + 1) {
+          uint32_t other = 0;
+          for (int i = lane; i < 16 * (D / 8); i += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(smem + (swz(vt, key0 + (i & 15), i >> 4) - sbase));
+            other |= (w.x ^ finite_or_zero<kBF16>(w.x)) | (w.y ^ finite_or_zero<kBF16>(w.y)) |
+                     (w.z ^ finite_or_zero<kBF16>(w.z)) | (w.w ^ finite_or_zero<kBF16>(w.w));
+          }
+          if (__any_sync(0xffffffffu, other != 0u)) {
+#pragma unroll 1
+            for (int k = 0; k < min(16, left - key0); ++k) {
+              const int key = t * BK + key0 + k;
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const int d = j * 16 + 8 * x + kr;
+                  uint16_t* at = reinterpret_cast<uint16_t*>(smem + (swz(vt, key0 + k, d >> 3) - sbase) + (d & 7) * 2);
+                  const uint32_t bits = *at;
+                  __syncwarp();  // four lanes share a column
+                  if (finite_or_zero<kBF16>(bits) == bits) continue;
+                  *at = 0;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                      if (key <= lim[nt][e]) o[nt][j][2 * x + e] += widen16<kBF16>(bits);
+                }
+              __syncwarp();
+            }
+            fence_async_smem();  // the stage's next load comes behind these writes
+          }
+        }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           uint32_t a[4];
@@ -309,39 +342,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           a[2] &= keep1;
           a[3] &= keep1;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t f = finite_or_zero<kBF16>(a[e]);
-            other |= a[e] ^ f;
-            a[e] = f;
-          }
+          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
+          // an infinity counts in the first product only: the second's factor, a remainder, may be 0 or negative
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<kBF16>(o[nt][j], a, pb[nt][0], pb[nt][1]);
-            mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
-          }
-        }
-        // The products leave infinities and NaN out, as a factor (a probability that is masked, a remainder) may be 0 or
-        // of the wrong sign.  They make an infinity or NaN of the rows that see their key, whatever its probability is.
-        if (__any_sync(0xffffffffu, other != 0u)) {
-#pragma unroll 1
-          for (int k = 0; k < min(16, left - key0); ++k) {
-            const int key = t * BK + key0 + k;
+          for (int e = 0; e < 4; ++e) a[e] = finite_or_zero<kBF16>(a[e]);
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int d = j * 16 + 8 * x + kr;
-                const uint16_t bits = *reinterpret_cast<const uint16_t*>(
-                    smem + (swz(vt, key0 + k, d >> 3) - sbase) + (d & 7) * 2);
-                const float v = widen16<kBF16>(bits);
-                if (finite_or_zero<kBF16>(bits) == bits) continue;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e)
-                    if (key <= lim[nt][e]) o[nt][j][2 * x + e] += v;
-              }
-          }
+          for (int nt = 0; nt < NT; ++nt) mma16816<kBF16>(o[nt][j], a, pl[nt][0], pl[nt][1]);
         }
       }
       __syncwarp();
