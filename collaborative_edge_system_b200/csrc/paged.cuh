@@ -57,6 +57,15 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
   return x & ~bad;
 }
 
+// `sum`, which starts at 0, stays 0 as long as both numbers of every x are finite
+template <bool kBF16>
+__device__ __forceinline__ void note_other(uint32_t x, uint32_t& sum) {
+  if constexpr (kBF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+}
+
 // one 16-bit number
 template <bool kBF16>
 __device__ __forceinline__ float widen16(uint32_t bits) {

@@ -305,8 +305,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           uint32_t other = 0;
           for (int i = lane; i < 16 * (D / 8); i += 32) {
             const uint4 w = *reinterpret_cast<const uint4*>(smem + (swz(vt, key0 + (i & 15), i >> 4) - sbase));
-            other |= (w.x ^ finite_or_zero<kBF16>(w.x)) | (w.y ^ finite_or_zero<kBF16>(w.y)) |
-                     (w.z ^ finite_or_zero<kBF16>(w.z)) | (w.w ^ finite_or_zero<kBF16>(w.w));
+            note_other<kBF16>(w.x, other);
+            note_other<kBF16>(w.y, other);
+            note_other<kBF16>(w.z, other);
+            note_other<kBF16>(w.w, other);
           }
           if (__any_sync(0xffffffffu, other != 0u)) {
 #pragma unroll 1

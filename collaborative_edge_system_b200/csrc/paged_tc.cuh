@@ -248,17 +248,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               for (int c = 0; c < L::KBOX; ++c)
                 *reinterpret_cast<uint4*>(tile + c * L::BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
             __syncwarp();
-            uint32_t other = 0;
+            uint32_t other[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 4
             for (int i = lane; i < BK * 8 * L::KBOX; i += 32) {
-              uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
-              const uint4 w = *at;
-              const uint4 f = make_uint4(finite_or_zero<kBF16>(w.x), finite_or_zero<kBF16>(w.y),
-                                         finite_or_zero<kBF16>(w.z), finite_or_zero<kBF16>(w.w));
-              const uint32_t off_by = (w.x ^ f.x) | (w.y ^ f.y) | (w.z ^ f.z) | (w.w ^ f.w);
-              if (off_by != 0u) *at = f;
-              other |= off_by;
+              const uint4 w = *reinterpret_cast<const uint4*>(tile + i * 16);
+              note_other<kBF16>(w.x, other[0]);
+              note_other<kBF16>(w.y, other[1]);
+              note_other<kBF16>(w.z, other[2]);
+              note_other<kBF16>(w.w, other[3]);
             }
-            if (other != 0u) *other_flag = 1;
+            if ((other[0] | other[1] | other[2] | other[3]) != 0u) {  // among what this lane has read
+              *other_flag = 1;
+#pragma unroll 1
+              for (int i = lane; i < BK * 8 * L::KBOX; i += 32) {
+                uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
+                const uint4 w = *at;
+                *at = make_uint4(finite_or_zero<kBF16>(w.x), finite_or_zero<kBF16>(w.y), finite_or_zero<kBF16>(w.z),
+                                 finite_or_zero<kBF16>(w.w));
+              }
+            }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(b_full + st));
