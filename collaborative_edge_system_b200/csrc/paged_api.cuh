@@ -97,14 +97,14 @@ bool paged_tc_ok(const cea_paged_attn_params* p) {
 // numbers of new tokens allow a sequence for it.  Times in us, bf16, 32 query and 8 KV heads where nothing else is said.
 // - 9 to 16 rows at D = 128, if no sequence of the call can have fewer: the chunk kernel, which pads them to a tile that
 //   the tensor cores take in their stride, while the 16-row form holds twice the accumulators.  Chunk kernel and 16-row
-//   form: 35 and 44 (8 sequences of 4096, 4 tokens each), 103 and 110 (32 of them), 40 and 60 (64 of 300 to 600),
-//   36 and 44 (32 of 4096, one token, groups of 16), 15 and 17 (one of those).
-// - 9 to 16 rows at D = 64: the 16-row form, 71 against 86 (32 of 4096, 4 tokens), 29 against 31 (groups of 16).
-// - up to 16 rows, some of them perhaps 8 or fewer: the 16-row form alone, 38 against 43 and 91 against 94 for the 8-row
+//   form: 36 and 41 (8 sequences of 4096, 4 tokens each), 103 and 106 (32 of them), 40 and 57 (64 of 300 to 600),
+//   36 and 41 (32 of 4096, one token, groups of 16), 15 and 17 (one of those).
+// - 9 to 16 rows at D = 64: the 16-row form, 76 against 85 (32 of 4096, 4 tokens), 29.5 against 30.4 (groups of 16).
+// - up to 16 rows, some of them perhaps 8 or fewer: the 16-row form alone, 35 against 44 and 87 against 97 for the 8-row
 //   form with the chunk kernel after it (8 and 32 of 2000 to 4096, 1 to 4 tokens).
 // - where longer chunks come too: the 8-row form, and sequences of 9 to 16 rows join the chunks; the 16-row form costs
-//   every single token of the batch: 98 against 110 (18 single tokens and two chunks of 389, up to 6000 keys).
-// - up to 8 rows: the 8-row form, 44 against 58 for the 16-row form (64 of 600 to 900, one token).
+//   every single token of the batch: 101 against 108 (18 single tokens and two chunks of 389, up to 6000 keys).
+// - up to 8 rows: the 8-row form, 44 against 56 for the 16-row form (64 of 600 to 900, one token).
 struct PagedChoice {
   int kernels;
   int rows;  // query rows of the decode kernel: 8 or 16

@@ -6,7 +6,8 @@
 // keys.  16 threads share two rows, r and r + 8: thread `sub` holds the scores of keys sub + 16 j and groups of 16-byte
 // output columns sub + 16 c of both, so every 16-byte word of K and V that it reads from shared memory, which bounds the
 // kernel, feeds two rows (one row a thread: 44 us at the size below; tiles of 64 keys, with half the CTAs on an SM: 41;
-// this: 37).  Rows are padded by 16 bytes, which keeps the reads free of conflicts.  Online softmax: m' = max(m, max s),
+// this: 37, and 38 with the rows of a tile that they see different parts of taken one by one).  Rows are padded by 16
+// bytes, which keeps the reads free of conflicts.  Online softmax: m' = max(m, max s),
 // l' = l e^(m - m') + sum e^(s - m'), o' = o e^(m - m') + sum e^(s - m') v.
 // Several threads fetch a key's K and V rows (one page lookup per tile and thread): by cp.async a tile ahead where the
 // rows are aligned and need no conversion, else element by element.  The division of the work over the grid is

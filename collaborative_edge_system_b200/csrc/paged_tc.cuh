@@ -20,12 +20,14 @@
 // the tiles that not all rows see whole are searched for infinities and NaN, which become zeros there and are added by
 // the epilogue to the rows that see them, from the pages (a rare path; the search is one pass of the V producer over the
 // last one to five tiles of a unit).
-// P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16 and 2^-11 for f16, independent per key),
-// the sum is of the unrounded fp32 values; S, statistics and O are fp32.  f16 numbers below 2^-14 lose bits and those below
+// P is rounded to the input type (the MMA's operand; half a step, 2^-8 for bf16 and 2^-11 for f16, independent per key; a
+// second term, as the decode kernel has it, would double the PV products, and products bound this kernel), the sum is of
+// the unrounded fp32 values; S, statistics and O are fp32.  f16 numbers below 2^-14 lose bits and those below
 // 2^-25 are 0, so there P is 2^7 times the probability's ratio to its row's reference (at most 2^15 of 65504: the reference
 // may be 2^8 below the maximum): a key counts down to 2^-32 of the largest.
-// Measured (bf16, 32/8 heads of 128, pages of 16, GPU time): 4096 new tokens on 36864, 1.9 to 2.0 ms, 1165 to 1225
-// TFLOP/s with the clock pulled down to about 1.5 GHz by the power limit; 512 on 8700, 75 us, 950 TFLOP/s.  A pair of
+// Measured (bf16, 32/8 heads of 128, pages of 16): 4096 new tokens on 36864, 2.27 to 2.30 ms a call among others, 1015 to
+// 1030 TFLOP/s, with the clock pulled down by the power limit (1.99 ms, 1176 TFLOP/s, for a few calls in a captured graph);
+// 512 on 8700, 75 us of GPU time, 940 TFLOP/s, 83 to 84 us a call.  A pair of
 // 64-key tiles takes some 1600 cycles against 1280 of products and 1024 of exponentials.  Tried and slower: tiles of 128
 // keys with one S buffer (91 us for the 512), one issuing warp for both halves, the halves' exponentials by turns,
 // a quarter to a half of the exponentials by a polynomial on the multiply-add pipe, the row maximum computed between the

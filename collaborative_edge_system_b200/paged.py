@@ -163,9 +163,10 @@ def paged_attend_into(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     and chunks of prompts have a kernel each, and a batch that cannot hold one kind does not launch its kernel.
 
     16-bit inputs: the kernels differ in what is left of a probability when it is multiplied with the values, so a
-    sequence's result differs within these bounds with the bounds given and with the other sequences of the call.  The
+    sequence's result differs within the following with the bounds given and with the other sequences of the call.  The
     decoding kernel keeps it to 2^-17 (bf16) or 2^-22 (f16), the chunk kernel rounds it to the input type (half a step,
-    2^-8 or 2^-11), as the dense prefill kernel does; the CUDA cores, which take the shapes outside both, keep fp32.
+    2^-8 or 2^-11), as the dense prefill kernel does; the CUDA cores, which take the shapes outside both, keep fp32.  In
+    f16 no kernel loses more of a key than 2^-39 (decoding) or 2^-32 (chunks) of its row's largest probability.
     9 to 16 query rows at 128 columns go to the chunk kernel where ``min_q_len`` says that no sequence has fewer, and
     to the decoding kernel where it does not.
     """
